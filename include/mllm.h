@@ -220,6 +220,98 @@ int mllm_gemm_q4(const uint8_t* d_packed, const float* d_scales, const float* d_
 int mllm_gemm_q4_noalloc(const uint8_t* d_packed, const float* d_scales, const float* d_x, float* d_y, int rows,
                          int cols, int n_act, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Paged serving operators (no counterpart in the reference, which decodes one sequence per engine
+ * from a contiguous cache, engine/infer.js:348-358, and chooses ids greedily, engine/infer.js:240-287).
+ * All work on device pointers and the caller's stream, allocate nothing, and may be captured in a
+ * CUDA graph.  A refused call returns MLLM_ERR_ARG or MLLM_ERR_UNSUPPORTED before any launch, with its
+ * reason in mllm_last_error(NULL).
+ *
+ * One layer's K/V page pool.  A page holds page_len positions of every kv head; position p of a
+ * sequence is row p % page_len of page table[p / page_len].  Element (page, head, position, d) of k and
+ * of v sits at page * page_stride + head * head_stride + position * pos_stride + d (strides in
+ * elements), so that pages may be kv-head-major or position-major and a pool may be a slice of a larger
+ * allocation.  k, v and every row must be 16-byte aligned; head_dim is a multiple of 8, 8 to 256.
+ * dtype: MLLM_DTYPE_F32, MLLM_DTYPE_F16 or MLLM_DTYPE_BF16.
+ * --------------------------------------------------------------------------------------------- */
+typedef struct {
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, pos_stride;
+  int32_t dtype, n_pages, page_len, n_kv_heads, head_dim;
+} mllm_paged_kv;
+
+/*
+ * Position step of a paged cache: for each of n_tok rows [q heads | k heads | v heads] of d_qkv (row
+ * t at d_qkv + t * row_stride, n_heads + 2 n_kv_heads heads of head_dim, of type `dtype`), in one pass:
+ *   - each q and k head is divided by sqrt(mean of squares + eps) and multiplied by d_q_gain /
+ *     d_k_gain (f32 [head_dim]; both NULL: no norm);
+ *   - its first rope_dim elements are rotated by the token's position: pairs (i, i + rope_dim / 2), or
+ *     (2 i, 2 i + 1) when interleaved, by d_cos / d_sin (f32 [n_pos][rope_dim / 2]: any frequencies, so
+ *     tables scaled for long contexts too; rope_dim 0: no rotation, tables may be NULL);
+ *   - q is written to d_q + t * q_stride ([n_heads][head_dim], `dtype`), k and v are rounded to the
+ *     cache's type and written into the token's page row.
+ * d_pos [n_tok]: positions.  d_seq [n_tok]: sequence of each row, its pages in d_table + seq *
+ * table_stride; NULL: row t belongs to sequence t.  A row with a negative sequence is padding: nothing
+ * of it is read or written.  A row whose sequence, position or page id is out of range writes no cache
+ * row, and its q is NaN.  No two rows may have the same sequence and position.  `dtype` is f32 or the
+ * cache's type.  d_q may be the q part of d_qkv itself.  Sums and rotations are f32.
+ */
+int mllm_rope_append(const mllm_paged_kv* kv, int dtype, const void* d_qkv, int64_t row_stride, int n_tok, int n_heads,
+                     const int32_t* d_seq, const int32_t* d_pos, const int32_t* d_table, int n_seq, int table_stride,
+                     const float* d_q_gain, const float* d_k_gain, float eps, const float* d_cos, const float* d_sin,
+                     int n_pos, int rope_dim, int interleaved, void* d_q, int64_t q_stride, void* stream);
+
+/*
+ * Attention of one new token per sequence over its paged cache: with g = n_heads / n_kv_heads, query
+ * head h of sequence s reads kv head h / g at positions 0 .. d_len[s] - 1:
+ *   out[s][h] = sum_p softmax_p(scale q[s][h] . k_p) v_p,  lse[s][h] = log sum_p exp(scale q[s][h] . k_p)
+ * d_q + s * q_stride and d_out + s * out_stride are [n_heads][head_dim] of `dtype`: the cache's type, or
+ * f32 over a cache of any type.  d_lse (nullable) is f32 [n_seq][n_heads].  A length of zero (or below)
+ * gives out = 0 and lse = -inf.  Cache rows past a sequence's length, and table entries past its last
+ * page, are never read.  A sequence whose length exceeds table_stride pages, or with a page id outside
+ * the pool, gives NaN.  n_heads / n_kv_heads <= 64.  Scores, sums and the join are f32.
+ * d_ws: mllm_paged_attn_workspace bytes, 16-byte aligned, zeroed once before its first use (each call
+ * leaves its counters at zero again); one workspace serves one stream at a time.  The result does not
+ * depend on timing: the length's parts are joined in a fixed order.
+ */
+int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d_q, int64_t q_stride, int n_seq, int n_heads,
+                    const int32_t* d_len, const int32_t* d_table, int table_stride, float scale, void* d_out,
+                    int64_t out_stride, float* d_lse, void* d_ws, size_t ws_bytes, void* stream);
+
+/* Workspace bytes of mllm_paged_attn for up to n_seq sequences and n_heads query heads of head_dim on
+ * any device (0 when an argument is out of range). */
+size_t mllm_paged_attn_workspace(int n_seq, int n_heads, int head_dim);
+
+/*
+ * Copy pages src[i] -> dst[i] (host arrays, i < n) of n_layers pools that lie layer_stride elements apart
+ * (k and v alike), for forks that are about to be written and for compaction.  Pages must be contiguous
+ * (kv-head-major or position-major without gaps).  Every page id must be in the pool, no page may be
+ * written twice, and no page may be both read and written (MLLM_ERR_ARG): the copies run in no order.
+ * The ids are read before the call returns.
+ */
+int mllm_copy_pages(const mllm_paged_kv* kv, int n_layers, int64_t layer_stride, const int32_t* src,
+                    const int32_t* dst, int n, void* stream);
+
+/*
+ * Draw one id per logits row from given uniform numbers.  Row r is d_logits + r * row_stride ([vocab]
+ * of `dtype`: f32, f16 or bf16); NaN counts as -inf.  With x the row, m its maximum and T the row's
+ * temperature, token i weighs w_i = floor(2^40 exp((x_i - m) (1 / T))).  By falling x, ties by rising
+ * index: the first top_k tokens are kept; of those, each one before which less than top_p of their
+ * weight lies (the first always); of those, each one with w_i >= min_p 2^40.  The drawn id is the first
+ * in index order at which the running kept weight passes floor(u Z), Z the kept weight.  Weights are
+ * integers: no result depends on the order of a sum.
+ * d_temperature, d_top_k, d_top_p, d_min_p: one value per row, each nullable (1, off, off, off).
+ * T <= 0 (or NaN) takes the top token, lowest index on ties, as engine/infer.js:240-250; top_k <= 0 or
+ * >= vocab, top_p >= 1 and min_p <= 0 are off.  d_u [rows]: in [0, 1).
+ * Out: d_id [rows]; nullable d_logprob [rows] (of the drawn id in the kept distribution), d_kept [rows]
+ * (tokens kept), d_probs [rows][vocab] f32 (the kept distribution).  A row that keeps no token (every
+ * logit -inf or NaN, or min_p above 1) gives id -1, logprob -inf, kept 0 and probs 0.  vocab <= 524,288.
+ */
+int mllm_sample(int dtype, const void* d_logits, int64_t row_stride, int rows, int vocab, const float* d_temperature,
+                const int32_t* d_top_k, const float* d_top_p, const float* d_min_p, const float* d_u, int32_t* d_id,
+                float* d_logprob, int32_t* d_kept, float* d_probs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,94 @@
+// Page copies of a paged cache (mllm_copy_pages): page dst[i] of every layer, k and v, becomes a copy of
+// page src[i].  Nothing is computed: bound by HBM (each byte read and written once), or by launch
+// latency for a few pages.  The page ids travel as kernel parameters, so a call needs no device copy of
+// them, takes no workspace and may be captured.
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "paged.cuh"
+
+namespace mllm {
+namespace {
+
+using namespace paged;
+
+constexpr int kCopyThreads = 256;
+
+template <int N>
+struct CopyArgs {
+  uint4 *k, *v;
+  int64_t page_stride, layer_stride;  // 16-byte units
+  int page_units;
+  int32_t src[N], dst[N];
+};
+
+// grid: (moves, layers, k or v)
+template <int N>
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs<N> a) {
+  uint4* pool = (blockIdx.z ? a.v : a.k) + (int64_t)blockIdx.y * a.layer_stride;
+  const uint4* from = pool + (int64_t)a.src[blockIdx.x] * a.page_stride;
+  uint4* to = pool + (int64_t)a.dst[blockIdx.x] * a.page_stride;
+  for (int i = threadIdx.x; i < a.page_units; i += kCopyThreads) to[i] = from[i];
+}
+
+template <int N>
+void launch_copy(const mllm_paged_kv* kv, int layers, int64_t layer_stride, const int32_t* src, const int32_t* dst,
+                 int n, cudaStream_t st) {
+  const int per = 16 / esize(kv->dtype);
+  CopyArgs<N> a;
+  a.k = static_cast<uint4*>(kv->k);
+  a.v = static_cast<uint4*>(kv->v);
+  a.page_stride = kv->page_stride / per;
+  a.layer_stride = layer_stride / per;
+  a.page_units = kv->n_kv_heads * kv->page_len * (kv->head_dim / per);
+  std::copy(src, src + n, a.src);
+  std::copy(dst, dst + n, a.dst);
+  copy_pages_kernel<N><<<dim3(n, layers, 2), kCopyThreads, 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace mllm
+
+extern "C" int mllm_copy_pages(const mllm_paged_kv* kv, int n_layers, int64_t layer_stride, const int32_t* src,
+                               const int32_t* dst, int n, void* stream) {
+  using namespace mllm;
+  using namespace mllm::paged;
+  if (int rc = check_kv(kv)) return rc;
+  if (n < 0 || n_layers < 1 || n_layers > 65535) return refuse(MLLM_ERR_ARG, "mllm_copy_pages: bad page or layer count");
+  const int64_t page = (int64_t)kv->n_kv_heads * kv->page_len * kv->head_dim;
+  const bool by_head = kv->pos_stride == kv->head_dim && kv->head_stride == (int64_t)kv->page_len * kv->head_dim;
+  const bool by_pos = kv->head_stride == kv->head_dim && kv->pos_stride == (int64_t)kv->n_kv_heads * kv->head_dim;
+  if (!(by_head || by_pos) || kv->page_stride < page)
+    return refuse(MLLM_ERR_UNSUPPORTED, "mllm_copy_pages: pages must be contiguous");
+  if (page > (int64_t)1 << 30) return refuse(MLLM_ERR_UNSUPPORTED, "mllm_copy_pages: pages above 2^30 elements");
+  const int per = 16 / esize(kv->dtype);
+  if (n_layers > 1 && (layer_stride < page || layer_stride % per))
+    return refuse(MLLM_ERR_ARG, "mllm_copy_pages: layer_stride below a page, or not 16-byte aligned");
+  if (n == 0) return MLLM_OK;
+  if (!src || !dst) return refuse(MLLM_ERR_ARG, "mllm_copy_pages: null page list");
+  try {
+    std::vector<uint8_t> used(kv->n_pages, 0);  // 1: read, 2: written
+    for (int i = 0; i < n; ++i) {
+      if (src[i] < 0 || src[i] >= kv->n_pages || dst[i] < 0 || dst[i] >= kv->n_pages)
+        return refuse(MLLM_ERR_ARG, "mllm_copy_pages: page id outside the pool");
+      used[src[i]] |= 1;
+    }
+    for (int i = 0; i < n; ++i) {
+      if (used[dst[i]]) return refuse(MLLM_ERR_ARG, "mllm_copy_pages: a page is written twice, or read and written");
+      used[dst[i]] = 2;
+    }
+  } catch (const std::bad_alloc&) {
+    return MLLM_ERR_OOM;
+  }
+  constexpr int kFew = 32, kMany = 2048;  // 16 KB of parameters
+  for (int i = 0; i < n; i += kMany) {
+    const int m = std::min(kMany, n - i);
+    if (m <= kFew)
+      launch_copy<kFew>(kv, n_layers, layer_stride, src + i, dst + i, m, (cudaStream_t)stream);
+    else
+      launch_copy<kMany>(kv, n_layers, layer_stride, src + i, dst + i, m, (cudaStream_t)stream);
+    if (int rc = launched("mllm_copy_pages: launch failed")) return rc;
+  }
+  return MLLM_OK;
+}

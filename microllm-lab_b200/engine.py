@@ -31,7 +31,8 @@ EXPORTS = ["mllm_create", "mllm_destroy", "mllm_last_error", "mllm_config", "mll
            "mllm_cache_len", "mllm_forward", "mllm_generate", "mllm_generate_stream", "mllm_generate_device",
            "mllm_generate_batch",
            "mllm_selftest_timeout",
-           "mllm_gemv_q4", "mllm_gemv", "mllm_gemm_q4", "mllm_gemm_q4_noalloc"]
+           "mllm_gemv_q4", "mllm_gemv", "mllm_gemm_q4", "mllm_gemm_q4_noalloc",
+           "mllm_rope_append", "mllm_paged_attn", "mllm_paged_attn_workspace", "mllm_copy_pages", "mllm_sample"]
 
 
 class MllmError(RuntimeError):
@@ -87,6 +88,13 @@ def load_library(path: str = LIB_PATH):
     L.mllm_gemv.argtypes = [I, P, P, P, P, I, I, I, P]
     L.mllm_gemm_q4.argtypes = [P, P, P, P, I, I, I, P]
     L.mllm_gemm_q4_noalloc.argtypes = [P, P, P, P, I, I, I, P]
+    F, S = ctypes.c_float, ctypes.c_int64
+    L.mllm_rope_append.argtypes = [P, I, P, S, I, I, P, P, P, I, I, P, P, F, P, P, I, I, I, P, S, P]
+    L.mllm_paged_attn.argtypes = [P, I, P, S, I, I, P, P, I, F, P, S, P, P, Z, P]
+    L.mllm_paged_attn_workspace.argtypes = [I, I, I]
+    L.mllm_paged_attn_workspace.restype = Z
+    L.mllm_copy_pages.argtypes = [P, I, S, P, P, I, P]
+    L.mllm_sample.argtypes = [I, P, S, I, I, P, P, P, P, P, P, P, P, P, P]
     L.mllm_selftest_timeout.argtypes = [P, I]
     L.mllm_set_stream.argtypes = [P, P]
     _LIB = L
