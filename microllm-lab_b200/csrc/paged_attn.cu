@@ -2,10 +2,19 @@
 //
 //   out = sum_p softmax_p(scale q . k_p) v_p,   lse = log sum_p exp(scale q . k_p)
 //
-// Two multiply-adds per cached element and query head of its group: bound by the bytes of the cache.
-// One pass with the running maximum m and sum l of the softmax: a new score s turns (m, l, o) into
-// (m', l e^(m - m') + e^(s - m'), o e^(m - m') + e^(s - m') v).  One CTA per query head; its warps take
-// every fourth position and join their (m, l, o) at the end.
+// One pass with the running maximum m and sum l of the softmax: a block of scores with maximum m' turns
+// (m, l, o) into (M, l e^(m - M) + sum e^(s - M), o e^(m - M) + sum e^(s - M) v), M = max(m, m').  Two
+// multiply-adds per cached element and query head of its group: bound by the bytes of the cache.
+//
+// Work is cut into blocks of 32 positions of one (sequence, kv head, group of query heads), numbered in
+// that order over the whole batch.  Every CTA takes an equal run of them, whatever the lengths: it sums
+// the lengths itself, so that they may live on the device and the grid does not depend on them.  A run
+// covers parts of a segment (a sequence's kv head) or several; the warps of a CTA take its blocks in turn
+// and join their (m, l, o) in shared memory.  A segment that lies in one CTA is written at once; the
+// others leave (m, l, o) in the workspace, and the CTA that counts itself last joins them in the order
+// of their positions, so that the result does not depend on timing and no CTA waits for another.
+#include <algorithm>
+
 #include "device_common.cuh"
 #include "paged.cuh"
 
@@ -15,6 +24,12 @@ namespace {
 using namespace paged;
 
 constexpr int kAttnWarps = 4;
+constexpr int kAttnThreads = kAttnWarps * 32;
+constexpr int kBlock = 32;       // positions per block: one per lane for the page lookups
+constexpr int kMinBlocks = 4;    // a CTA's run is at least one block per warp
+constexpr int kMaxCtas = 1024;   // partial slots in the workspace
+constexpr int kMaxGroup = 16;    // query heads of a group
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnArgs {
   const void *k, *v;
@@ -29,83 +44,759 @@ struct AttnArgs {
   void* out;
   int64_t out_stride;
   float* lse;
+  uint32_t* counter;  // [n_seq][n_kv][groups]
+  float* part;        // [CTA][2][group][dim + 2]
+  int rep, group_size, groups;  // query heads per kv head, of a group, groups of a kv head
 };
 
-template <class A, class C>
-__global__ void __launch_bounds__(kAttnWarps * 32) paged_attn_kernel(const AttnArgs a) {
-  __shared__ float sm[kAttnWarps], sl[kAttnWarps], so[kAttnWarps][256];
-  __shared__ int bad;
-  const int s = blockIdx.y, h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = h / (a.n_heads / a.n_kv);
-  const A* q = static_cast<const A*>(a.q) + s * a.q_stride + (int64_t)h * a.dim;
-  const int len = max(a.len[s], 0);
-  if (threadIdx.x == 0) bad = (int64_t)len > (int64_t)a.table_stride * a.page_len;
-  __syncthreads();
-  const int n = bad ? 0 : len;
-  float qv[8], o[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    qv[i] = lane + 32 * i < a.dim ? to_f32(q[lane + 32 * i]) : 0.f;
-    o[i] = 0.f;
-  }
-  for (int p = warp; p < n; p += kAttnWarps) {
-    const int pg = p / a.page_len;
-    const int page = a.table[(int64_t)s * a.table_stride + pg];
-    if (page < 0 || page >= a.n_pages) {
-      bad = 1;
-      break;
-    }
-    const int64_t at = page * a.page_stride + hk * a.head_stride + (int64_t)(p - pg * a.page_len) * a.pos_stride;
-    const C* kr = static_cast<const C*>(a.k) + at;
-    const C* vr = static_cast<const C*>(a.v) + at;
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < a.dim) x = fmaf(qv[i], to_f32(kr[lane + 32 * i]), x);
-    x = warp_sum(x) * a.scale;
-    const float mn = fmaxf(m, x);
-    const float keep = mn == -INFINITY ? 1.f : expf(m - mn), e = mn == -INFINITY ? 0.f : expf(x - mn);
-    l = fmaf(l, keep, e);
-    m = mn;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < a.dim) o[i] = fmaf(o[i], keep, e * to_f32(vr[lane + 32 * i]));
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) so[warp][lane + 32 * i] = o[i];
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, sm[w]);
-  float f[kAttnWarps];
-  for (int w = 0; w < kAttnWarps; ++w) {
-    f[w] = sm[w] == -INFINITY ? 0.f : expf(sm[w] - top);
-    sum = fmaf(f[w], sl[w], sum);
-  }
-  const float nan = __int_as_float(0x7FC00000);
-  A* out = static_cast<A*>(a.out) + s * a.out_stride + (int64_t)h * a.dim;
-  for (int d = threadIdx.x; d < a.dim; d += kAttnWarps * 32) {
-    float r = 0.f;
-    for (int w = 0; w < kAttnWarps; ++w) r = fmaf(f[w], so[w][d], r);
-    out[d] = from_f32<A>(bad ? nan : (sum > 0.f ? r / sum : r));
-  }
-  if (a.lse && threadIdx.x == 0) a.lse[(int64_t)s * a.n_heads + h] = bad ? nan : top + logf(sum);
+// ---------------------------------------------------------------------------------------------
+// Loads of cached rows: each byte is used once, so it does not stay in L1.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint4 ld_row(const void* p) {
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_row_if(const void* p, bool ok) {
+  return ok ? ld_row(p) : make_uint4(0u, 0u, 0u, 0u);
 }
 
-template <class A, class C>
-void launch_attn(const AttnArgs& a, cudaStream_t st) {
-  paged_attn_kernel<A, C><<<dim3(a.n_heads, a.n_seq), kAttnWarps * 32, 0, st>>>(a);
+// 2^x for the softmax; x <= 0, or -inf.
+__device__ __forceinline__ float pow2(float x) { return exp2f(x); }
+
+// ---------------------------------------------------------------------------------------------
+// A CTA's run of blocks.
+// ---------------------------------------------------------------------------------------------
+struct Run {
+  int64_t q;          // blocks per CTA
+  int64_t u, end;     // next block, end of the run
+  int64_t before;     // blocks of the sequences before `seq`, per (kv head, group)
+  int seq;
+};
+
+__device__ __forceinline__ int blocks_of(const AttnArgs& a, int s) {
+  const int n = a.len[s];
+  return n <= 0 || (int64_t)n > (int64_t)a.table_stride * a.page_len ? 0 : (n - 1) / kBlock + 1;
+}
+
+__device__ __forceinline__ Run find_run(const AttnArgs& a) {
+  __shared__ int64_t wsum[kAttnWarps], s_before;
+  __shared__ int s_seq;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.n_seq + kAttnThreads - 1) / kAttnThreads;
+  const int s0 = min(tid * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
+  int64_t mine = 0;
+  for (int s = s0; s < s1; ++s) mine += blocks_of(a, s);
+  int64_t run = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == 31) wsum[warp] = run;
+  __syncthreads();
+  int64_t total = 0, lead = 0;
+#pragma unroll
+  for (int w = 0; w < kAttnWarps; ++w) {
+    if (w == warp) lead = total;
+    total += wsum[w];
+  }
+  const int64_t per_block = (int64_t)a.n_kv * a.groups;
+  const int64_t all = total * per_block;
+  Run r;
+  r.q = max((int64_t)kMinBlocks, (all + gridDim.x - 1) / gridDim.x);
+  r.u = blockIdx.x * r.q;
+  r.end = min(r.u + r.q, all);
+  r.seq = 0;
+  r.before = 0;
+  if (r.u >= all) return r;  // nothing (the same on every thread)
+  int64_t b = lead + run - mine;  // blocks before this thread's sequences
+  if (r.u >= b * per_block && r.u < (b + mine) * per_block) {
+    int s = s0;
+    for (;; ++s) {
+      const int n = blocks_of(a, s);
+      if (r.u < (b + n) * per_block) break;
+      b += n;
+    }
+    s_seq = s;
+    s_before = b;
+  }
+  __syncthreads();
+  r.seq = s_seq;
+  r.before = s_before;
+  return r;
+}
+
+// The part of a run that lies in one segment.
+struct Segment {
+  int seq, kv, group, len;
+  int b0, b1;          // blocks of the segment in this run
+  int nb;              // blocks of the segment
+  int64_t start;       // its first block in the batch's numbering
+  int heads;           // query heads of the group
+  int head0;           // the first of them
+};
+
+__device__ __forceinline__ bool next_segment(const AttnArgs& a, Run& r, Segment& g) {
+  if (r.u >= r.end) return false;
+  const int64_t per_block = (int64_t)a.n_kv * a.groups;
+  int nb = blocks_of(a, r.seq);
+  while (r.u >= (r.before + nb) * per_block) {
+    r.before += nb;
+    nb = blocks_of(a, ++r.seq);
+  }
+  const int64_t in = r.u - r.before * per_block;
+  const int j = (int)(in / nb);
+  g.seq = r.seq;
+  g.nb = nb;
+  g.len = a.len[r.seq];
+  g.kv = j / a.groups;
+  g.group = j - g.kv * a.groups;
+  g.b0 = (int)(in - (int64_t)j * nb);
+  g.b1 = (int)min((int64_t)nb, g.b0 + (r.end - r.u));
+  g.start = r.u - g.b0;
+  g.heads = min(a.rep - g.group * a.group_size, a.group_size);
+  g.head0 = g.kv * a.rep + g.group * a.group_size;
+  r.u += g.b1 - g.b0;
+  return true;
+}
+
+// Element offset of this lane's position of a block, -1 when it is past the length or its page is bad.
+__device__ __forceinline__ int64_t row_offset(const AttnArgs& a, const Segment& g, int block, int lane, int* bad) {
+  const int p = block * kBlock + lane;
+  if (block >= g.b1 || p >= g.len) return -1;
+  const int pg = p / a.page_len;
+  const int page = __ldg(a.table + (int64_t)g.seq * a.table_stride + pg);
+  if ((unsigned)page >= (unsigned)a.n_pages) {
+    *bad = 1;
+    return -1;
+  }
+  return page * a.page_stride + g.kv * a.head_stride + (int64_t)(p - pg * a.page_len) * a.pos_stride;
+}
+
+// What the warps of a CTA leave for the join of a segment: m (in units of log 2) and l, then o.
+struct Joint {
+  float *m, *l, *o;  // [warp][group], [warp][group], [warp][group][DP]
+};
+
+template <class A>
+__device__ __forceinline__ void write_out(const AttnArgs& a, const Segment& g, int h, int d, float o, float l) {
+  static_cast<A*>(a.out)[g.seq * a.out_stride + (int64_t)(g.head0 + h) * a.dim + d] = from_f32<A>(l == 0.f ? 0.f : o / l);
+}
+__device__ __forceinline__ void write_lse(const AttnArgs& a, const Segment& g, int h, float m, float l) {
+  if (a.lse) a.lse[(int64_t)g.seq * a.n_heads + g.head0 + h] = (m + log2f(l)) * (1.f / kLog2e);
+}
+
+// Joins the warps' (m, l, o); writes the segment's rows, or its part of them, and joins the parts when
+// this CTA is the last to leave one.
+template <class A, int DP>
+__device__ void finish(const AttnArgs& a, const Run& r, const Segment& g, const Joint& w, int bad) {
+  __shared__ int last;
+  const int tid = threadIdx.x;
+  const bool whole = g.b0 == 0 && g.b1 == g.nb;
+  const size_t slot = (size_t)a.group_size * (a.dim + 2);
+  float* part = a.part + ((size_t)blockIdx.x * 2 + (g.b0 == 0)) * slot;
+  for (int i = tid; i < g.heads * a.dim; i += kAttnThreads) {
+    const int h = i / a.dim, d = i - h * a.dim;
+    float m = -INFINITY, l = 0.f, o = 0.f;
+#pragma unroll
+    for (int k = 0; k < kAttnWarps; ++k) m = fmaxf(m, w.m[k * a.group_size + h]);
+#pragma unroll
+    for (int k = 0; k < kAttnWarps; ++k) {
+      const float mk = w.m[k * a.group_size + h];
+      const float f = mk == -INFINITY ? 0.f : pow2(mk - m);
+      l = fmaf(f, w.l[k * a.group_size + h], l);
+      o = fmaf(f, w.o[(k * a.group_size + h) * DP + d], o);
+    }
+    if (bad) l = __int_as_float(0x7FC00000);
+    if (whole) {
+      write_out<A>(a, g, h, d, o, l);
+      if (d == 0) write_lse(a, g, h, m, l);
+    } else {
+      part[i] = o;
+      if (d == 0) {
+        part[a.group_size * a.dim + 2 * h] = m;
+        part[a.group_size * a.dim + 2 * h + 1] = l;
+      }
+    }
+  }
+  if (whole) return;
+  const int first = (int)(g.start / r.q), parts = (int)((g.start + g.nb - 1) / r.q) - first + 1;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t* c = a.counter + ((int64_t)g.seq * a.n_kv + g.kv) * a.groups + g.group;
+    last = atomicAdd(c, 1u) == (uint32_t)parts - 1;
+    if (last) *c = 0;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int i = tid; i < g.heads * a.dim; i += kAttnThreads) {
+    const int h = i / a.dim;
+    float m = -INFINITY, l = 0.f, o = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+      const float* p = a.part + ((size_t)(first + k) * 2 + (k == 0)) * slot;
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + a.group_size * a.dim) + h);
+      const float ok = __ldcg(p + i), mn = fmaxf(m, ml.x);
+      const float f0 = m == -INFINITY ? 0.f : pow2(m - mn), f1 = ml.x == -INFINITY ? 0.f : pow2(ml.x - mn);
+      l = l * f0 + ml.y * f1;
+      o = o * f0 + ok * f1;
+      m = mn;
+    }
+    write_out<A>(a, g, h, i - h * a.dim, o, l);
+    if (i == h * a.dim) write_lse(a, g, h, m, l);
+  }
+}
+
+// Sequences without positions, and those whose length the table cannot hold.
+template <class A>
+__device__ void finish_empty(const AttnArgs& a) {
+  for (int s = blockIdx.x; s < a.n_seq; s += gridDim.x) {
+    if (blocks_of(a, s)) continue;
+    const float v = a.len[s] > 0 ? __int_as_float(0x7FC00000) : 0.f;
+    A* out = static_cast<A*>(a.out) + s * a.out_stride;
+    for (int i = threadIdx.x; i < a.n_heads * a.dim; i += kAttnThreads) out[i] = from_f32<A>(v);
+    if (a.lse)
+      for (int h = threadIdx.x; h < a.n_heads; h += kAttnThreads) a.lse[(int64_t)s * a.n_heads + h] = v == 0.f ? -INFINITY : v;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Caches of 16 bits: both products on the tensor cores, m16n8k16 with positions (then head_dim) as the
+// 16 rows and 8 query heads as the columns, so that a group of few heads wastes little.  The order of the
+// summed index is free as long as both operands share it, so every lane loads 16-byte pieces of cached
+// rows straight into the registers that are its operands: for the scores a lane's 8 neighbouring elements
+// of a key row serve two steps; for the output, pairs of value rows are woven by byte permutes.  Nothing
+// passes through shared memory but the queries.  The scores' accumulators, packed and transposed by
+// movmatrix, are the second product's operand.
+//
+// Queries of the cache's type are exact operands, and the weights are rounded to that type (their sum is
+// not), an error of the size of the output's own rounding.  f32 queries and weights are split into as
+// many 16-bit terms as f32 needs (3 in bf16, 2 in f16, where queries are first scaled by a power of two
+// to at most 1): the cached values are exact in either case.
+// ---------------------------------------------------------------------------------------------
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The terms of a pair: each is the rounding of what the ones before it left.
+template <class T, int TERMS>
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&w)[TERMS]) {
+#pragma unroll
+  for (int i = 0; i < TERMS; ++i) {
+    w[i] = pack2<T>(a, b);
+    if (i + 1 < TERMS) {
+      const T* e = reinterpret_cast<const T*>(&w[i]);
+      a -= to_f32(e[0]);
+      b -= to_f32(e[1]);
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(T) == 2 && __is_same(T, __half))
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+template <class T, class A>
+constexpr int terms_of() { return sizeof(A) == 2 ? 1 : (__is_same(T, __half) ? 2 : 3); }
+
+template <class T, class A, int DP, int NT>
+constexpr size_t mma_query_bytes() { return (size_t)(DP / 32) * terms_of<T, A>() * NT * 512; }
+
+// CTAs per SM that the register file is split for.
+template <int DP, int NT>
+constexpr int mma_ctas() { return DP == 64 ? 4 : (DP == 128 && NT == 1 ? 3 : 2); }
+
+template <class T, class A, int DP, int NT>
+__global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_kernel(const AttnArgs a) {
+  constexpr int C = DP / 32, V = DP / 64, J = DP == 64 ? 2 : 1, TERMS = terms_of<T, A>();
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float qscale[8 * NT];
+  __shared__ int bad;
+  uint4* const qs = reinterpret_cast<uint4*>(smem);  // [C][TERMS][NT][32]: each lane's operand words
+  Joint joint;
+  joint.m = reinterpret_cast<float*>(smem + mma_query_bytes<T, A, DP, NT>());
+  joint.l = joint.m + kAttnWarps * a.group_size;
+  joint.o = joint.l + kAttnWarps * a.group_size;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = lane >> 2, quad = lane & 3;
+  const T* const kp = static_cast<const T*>(a.k);
+  const T* const vp = static_cast<const T*>(a.v);
+
+  Run run = find_run(a);
+  Segment g;
+  while (next_segment(a, run, g)) {
+    // ---- the group's queries as operand words, every head's rows of 8 * NT columns (0 past the group)
+    __syncthreads();  // the last segment's queries and join are done with
+    if (tid == 0) bad = 0;
+    const A* const q = static_cast<const A*>(a.q) + g.seq * a.q_stride + (int64_t)g.head0 * a.dim;
+    if constexpr (TERMS == 2) {  // f32 queries as f16 terms: scaled to at most 1
+      for (int h = warp; h < 8 * NT; h += kAttnWarps) {
+        float m = 0.f;
+        for (int d = lane; h < g.heads && d < a.dim; d += 32) m = fmaxf(m, fabsf(to_f32(q[h * a.dim + d])));
+        m = warp_max(m);
+        int e = 0;
+        if (m > 0.f && m < INFINITY) (void)frexpf(m, &e);
+        if (lane == 0) qscale[h] = ldexpf(1.f, max(min(e, 126), -126));
+      }
+      __syncthreads();
+    }
+    for (int i = tid; i < C * NT * 32; i += kAttnThreads) {
+      const int l = i & 31, nt = (i >> 5) % NT, c = (i >> 5) / NT;
+      const int h = nt * 8 + (l >> 2), d = c * 32 + (l & 3) * 8;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = h < g.heads && d < a.dim ? to_f32(q[h * a.dim + d + e]) : 0.f;
+      if constexpr (TERMS == 2) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] /= qscale[h];
+      }
+      uint32_t w[4][TERMS];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split2<T, TERMS>(x[2 * e], x[2 * e + 1], w[e]);
+#pragma unroll
+      for (int s = 0; s < TERMS; ++s) qs[((c * TERMS + s) * NT + nt) * 32 + l] = make_uint4(w[0][s], w[1][s], w[2][s], w[3][s]);
+    }
+    __syncthreads();
+    float sc[NT][2];  // score factors of this lane's two columns, for base-2 exponents
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        sc[nt][e] = a.scale * kLog2e;
+        if constexpr (TERMS == 2) sc[nt][e] = a.scale * qscale[nt * 8 + quad * 2 + e] * kLog2e;
+      }
+
+    float m[NT][2], l[NT][2], o[V][4][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[v][i][nt][e] = 0.f;
+    }
+    int64_t off = row_offset(a, g, g.b0 + warp, lane, &bad);
+    for (int block = g.b0 + warp; block < g.b1; block += kAttnWarps) {
+      const int64_t off_next = row_offset(a, g, block + kAttnWarps, lane, &bad);
+#pragma unroll
+      for (int half = 0; half < 2; half += J) {
+        // ---- key and value rows of J x 16 positions
+        uint4 kf[J][C][2], vf[J][V][4];
+        bool live[J][2];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int64_t at = __shfl_sync(0xffffffffu, off, (half + j) * 16 + row + 8 * e);
+            live[j][e] = at >= 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const int d = c * 32 + quad * 8;
+              kf[j][c][e] = ld_row_if(kp + at + d, at >= 0 && d < a.dim);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t at = __shfl_sync(0xffffffffu, off, (half + j) * 16 + (e >> 1) * 8 + quad * 2 + (e & 1));
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+              const int d = v * 64 + row * 8;
+              vf[j][v][e] = ld_row_if(vp + at + d, at >= 0 && d < a.dim);
+            }
+          }
+        }
+        // ---- scores: positions x heads
+        float s[J][NT][4];
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][nt][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint4 b = qs[((c * TERMS + t) * NT + nt) * 32 + lane];
+#pragma unroll
+              for (int j = 0; j < J; ++j) {
+                mma<T>(s[j][nt], kf[j][c][0].x, kf[j][c][1].x, kf[j][c][0].y, kf[j][c][1].y, b.x, b.y);
+                mma<T>(s[j][nt], kf[j][c][0].z, kf[j][c][1].z, kf[j][c][0].w, kf[j][c][1].w, b.z, b.w);
+              }
+            }
+        if constexpr (TERMS > 1) {
+          // A key of +-inf times a later term of a query (of any sign, or 0) is NaN: there the first
+          // term alone gives the score that f32 products would.
+          bool odd = false;
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) odd |= s[j][nt][e] != s[j][nt][e];
+          if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                  const uint4 b = qs[(c * TERMS * NT + nt) * 32 + lane];
+                  mma<T>(f, kf[j][c][0].x, kf[j][c][1].x, kf[j][c][0].y, kf[j][c][1].y, b.x, b.y);
+                  mma<T>(f, kf[j][c][0].z, kf[j][c][1].z, kf[j][c][0].w, kf[j][c][1].w, b.z, b.w);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (s[j][nt][e] != s[j][nt][e]) s[j][nt][e] = f[e];
+              }
+          }
+        }
+        // ---- running maximum and sum of this lane's two heads, weights as the second operand
+        uint32_t p[J][NT][TERMS][2];
+        float keep[NT][2];
+        bool moved = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = m[nt][e];
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                float& x = s[j][nt][2 * k + e];
+                x = live[j][k] ? x * sc[nt][e] : -INFINITY;
+                top = fmaxf(top, x);
+              }
+#pragma unroll
+            for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+            moved |= top != m[nt][e];
+            const float base = top == -INFINITY ? 0.f : top;
+            keep[nt][e] = pow2(m[nt][e] - base);  // 0 while there was nothing
+            m[nt][e] = top;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                float& x = s[j][nt][2 * k + e];
+                x = pow2(x - base);
+                sum += x;
+              }
+            l[nt][e] = fmaf(l[nt][e], keep[nt][e], sum);
+          }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              uint32_t w[TERMS];
+              split2<T, TERMS>(s[j][nt][2 * k], s[j][nt][2 * k + 1], w);
+#pragma unroll
+              for (int t = 0; t < TERMS; ++t) p[j][nt][t][k] = transpose8x8(w[t]);
+            }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[v][i][nt][e] *= keep[nt][e & 1];
+        }
+        // ---- output: head_dim x heads; rows 8 v + ... of the values woven in pairs of positions
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x0 = word(vf[j][v][0], i), x1 = word(vf[j][v][1], i);
+              const uint32_t x2 = word(vf[j][v][2], i), x3 = word(vf[j][v][3], i);
+              const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
+              const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) mma<T>(o[v][i][nt], a0, a1, a2, a3, p[j][nt][t][0], p[j][nt][t][1]);
+            }
+      }
+      off = off_next;
+    }
+    // ---- leave (m, l, o) for the join
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], b);
+        const int h = nt * 8 + quad * 2 + e;
+        if (h < g.heads) {
+          if (row == 0) {
+            joint.m[warp * a.group_size + h] = m[nt][e];
+            joint.l[warp * a.group_size + h] = l[nt][e];
+          }
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<float2*>(joint.o + (warp * a.group_size + h) * DP + v * 64 + row * 8 + 2 * i) =
+                  make_float2(o[v][i][nt][e], o[v][i][nt][2 + e]);
+        }
+      }
+    __syncthreads();
+    finish<A, DP>(a, run, g, joint, bad);
+  }
+  finish_empty<A>(a);
+}
+
+// ---------------------------------------------------------------------------------------------
+// f32 caches: the products on the CUDA cores, at most 8 query heads for every cached element.  Four lanes
+// share a key row for the scores; for the output a row's elements are spread over the lanes in pieces of
+// four, the weights passing through shared memory.
+// ---------------------------------------------------------------------------------------------
+template <int DP, int G>
+constexpr size_t f32_query_bytes() { return (size_t)G * DP * 4 + (size_t)kAttnWarps * kBlock * G * 4; }
+
+template <int DP, int G>
+__global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 3 : 2) attn_f32_kernel(const AttnArgs a) {
+  constexpr int C = DP / 16, PER = DP / 4 < 32 ? DP / 4 : 32, ROWS = 32 / PER, V = DP / 4 / PER;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int bad;
+  float* const qs = reinterpret_cast<float*>(smem);       // [G][DP]
+  float* const ps = qs + G * DP;                          // [warp][position][G]
+  Joint joint;
+  joint.m = reinterpret_cast<float*>(smem + f32_query_bytes<DP, G>());
+  joint.l = joint.m + kAttnWarps * a.group_size;
+  joint.o = joint.l + kAttnWarps * a.group_size;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = lane >> 2, quad = lane & 3;
+  float* const pw = ps + warp * kBlock * G;
+  const float* const kp = static_cast<const float*>(a.k);
+  const float* const vp = static_cast<const float*>(a.v);
+  auto f4 = [](const uint4& u) {
+    return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+  };
+
+  Run run = find_run(a);
+  Segment g;
+  while (next_segment(a, run, g)) {
+    __syncthreads();
+    if (tid == 0) bad = 0;
+    const float* const q = static_cast<const float*>(a.q) + g.seq * a.q_stride + (int64_t)g.head0 * a.dim;
+    for (int i = tid; i < G * DP; i += kAttnThreads) {
+      const int h = i / DP, d = i - h * DP;
+      qs[i] = h < g.heads && d < a.dim ? q[h * a.dim + d] : 0.f;
+    }
+    __syncthreads();
+    float m[G], l[G];       // of every head, the same on every lane (l: this lane's positions)
+    float o[V][G][4];
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[v][h][e] = 0.f;
+    }
+    const float sc = a.scale * kLog2e;
+    int64_t off = row_offset(a, g, g.b0 + warp, lane, &bad);
+    for (int block = g.b0 + warp; block < g.b1; block += kAttnWarps) {
+      const int64_t off_next = row_offset(a, g, block + kAttnWarps, lane, &bad);
+      // ---- scores of rows row, row + 8, row + 16, row + 24
+      float s[4][G];
+      int64_t at[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        at[e] = __shfl_sync(0xffffffffu, off, row + 8 * e);
+#pragma unroll
+        for (int h = 0; h < G; ++h) s[e][h] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int d = c * 16 + quad * 4;
+        float4 k[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) k[e] = f4(ld_row_if(kp + at[e] + d, at[e] >= 0 && d < a.dim));
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          const float4 x = *reinterpret_cast<const float4*>(qs + h * DP + d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[e][h] = fmaf(k[e].x, x.x, fmaf(k[e].y, x.y, fmaf(k[e].z, x.z, fmaf(k[e].w, x.w, s[e][h]))));
+        }
+      }
+      bool moved = false;
+      float keep[G];
+      __syncwarp();  // the last block's weights are read
+#pragma unroll
+      for (int h = 0; h < G; ++h) {
+        float top = m[h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = s[e][h];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          s[e][h] = at[e] >= 0 ? x * sc : -INFINITY;
+          top = fmaxf(top, s[e][h]);
+        }
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+        moved |= top != m[h];
+        const float base = top == -INFINITY ? 0.f : top;
+        keep[h] = pow2(m[h] - base);
+        m[h] = top;
+        // lane quad e of a row holds the weight of row + 8 e
+        const float x = quad == 0 ? s[0][h] : quad == 1 ? s[1][h] : quad == 2 ? s[2][h] : s[3][h];
+        const float w = pow2(x - base);
+        l[h] = fmaf(l[h], keep[h], w);
+        pw[(row + 8 * quad) * G + h] = w;
+      }
+      __syncwarp();
+      if (moved) {  // the maxima are the same on every lane
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int h = 0; h < G; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[v][h][e] *= keep[h];
+      }
+      // ---- output: ROWS value rows at a time
+#pragma unroll 8
+      for (int p = 0; p < kBlock; p += ROWS) {
+        const int r = p + lane / PER;
+        const int64_t av = __shfl_sync(0xffffffffu, off, r);
+        float w[G];
+#pragma unroll
+        for (int h = 0; h < G; h += 4) *reinterpret_cast<float4*>(w + h) = *reinterpret_cast<const float4*>(pw + r * G + h);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int d = (v * PER + lane % PER) * 4;
+          const float4 x = f4(ld_row_if(vp + av + d, av >= 0 && d < a.dim));
+#pragma unroll
+          for (int h = 0; h < G; ++h) {
+            o[v][h][0] = fmaf(w[h], x.x, o[v][h][0]);
+            o[v][h][1] = fmaf(w[h], x.y, o[v][h][1]);
+            o[v][h][2] = fmaf(w[h], x.z, o[v][h][2]);
+            o[v][h][3] = fmaf(w[h], x.w, o[v][h][3]);
+          }
+        }
+      }
+      off = off_next;
+    }
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      l[h] = warp_sum(l[h]);
+      if (h < g.heads) {
+        if (lane == 0) {
+          joint.m[warp * a.group_size + h] = m[h];
+          joint.l[warp * a.group_size + h] = l[h];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int b = PER; b < 32; b <<= 1) o[v][h][e] += __shfl_xor_sync(0xffffffffu, o[v][h][e], b);
+          }
+          if (lane < PER)
+            *reinterpret_cast<float4*>(joint.o + (warp * a.group_size + h) * DP + (v * PER + lane) * 4) =
+                make_float4(o[v][h][0], o[v][h][1], o[v][h][2], o[v][h][3]);
+        }
+      }
+    }
+    __syncthreads();
+    finish<float, DP>(a, run, g, joint, bad);
+  }
+  finish_empty<float>(a);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------------------------
+size_t counter_bytes(int n_seq, int n_heads) { return (((size_t)n_seq * n_heads * 4 + 255) / 256) * 256; }
+
+template <class K>
+int launch(K kernel, const AttnArgs& a, int per_sm, size_t smem, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: no current CUDA device");
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: not enough shared memory");
+  // no more CTAs than runs of the shortest length over the whole table
+  const int64_t blocks = ((int64_t)a.table_stride * a.page_len + kBlock - 1) / kBlock;
+  const int64_t most = (blocks + kMinBlocks - 1) / kMinBlocks * a.n_seq * a.n_kv * a.groups;
+  const int grid = (int)std::min<int64_t>(most, std::min(kMaxCtas, sms * per_sm));
+  kernel<<<grid, kAttnThreads, smem, st>>>(a);
+  return launched("mllm_paged_attn: launch failed");
+}
+
+size_t joint_bytes(const AttnArgs& a, int dp) { return (size_t)kAttnWarps * a.group_size * (dp + 2) * 4; }
+
+template <class T, class A, int DP, int NT>
+int launch_mma(const AttnArgs& a, cudaStream_t st) {
+  return launch(attn_mma_kernel<T, A, DP, NT>, a, mma_ctas<DP, NT>(), mma_query_bytes<T, A, DP, NT>() + joint_bytes(a, DP), st);
+}
+template <class T, class A>
+int run_mma(AttnArgs& a, cudaStream_t st) {
+  a.group_size = std::min(a.rep, kMaxGroup);
+  a.groups = (a.rep + a.group_size - 1) / a.group_size;
+  const bool one = a.group_size <= 8;
+  if (a.dim <= 64) return one ? launch_mma<T, A, 64, 1>(a, st) : launch_mma<T, A, 64, 2>(a, st);
+  if (a.dim <= 128) return one ? launch_mma<T, A, 128, 1>(a, st) : launch_mma<T, A, 128, 2>(a, st);
+  return one ? launch_mma<T, A, 256, 1>(a, st) : launch_mma<T, A, 256, 2>(a, st);
+}
+template <int DP, int G>
+int launch_f32(const AttnArgs& a, cudaStream_t st) {
+  return launch(attn_f32_kernel<DP, G>, a, DP == 64 ? 3 : 2, f32_query_bytes<DP, G>() + joint_bytes(a, DP), st);
+}
+int run_f32(AttnArgs& a, cudaStream_t st) {
+  a.group_size = std::min(a.rep, 8);
+  a.groups = (a.rep + a.group_size - 1) / a.group_size;
+  const bool four = a.group_size <= 4;
+  if (a.dim <= 64) return four ? launch_f32<64, 4>(a, st) : launch_f32<64, 8>(a, st);
+  if (a.dim <= 128) return four ? launch_f32<128, 4>(a, st) : launch_f32<128, 8>(a, st);
+  return four ? launch_f32<256, 4>(a, st) : launch_f32<256, 8>(a, st);
 }
 
 }  // namespace
 }  // namespace mllm
 
 extern "C" size_t mllm_paged_attn_workspace(int n_seq, int n_heads, int head_dim) {
+  using namespace mllm;
   if (n_seq < 1 || n_heads < 1 || head_dim < 8 || head_dim > 256) return 0;
-  return 16;
+  return counter_bytes(n_seq, n_heads) + (size_t)kMaxCtas * 2 * std::min(n_heads, kMaxGroup) * (head_dim + 2) * 4;
 }
 
 extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d_q, int64_t q_stride, int n_seq,
@@ -130,19 +821,16 @@ extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d
   if (n_seq == 0) return MLLM_OK;
   if (!d_ws || ((uintptr_t)d_ws & 15) || ws_bytes < mllm_paged_attn_workspace(n_seq, n_heads, kv->head_dim))
     return refuse(MLLM_ERR_ARG, "mllm_paged_attn: workspace missing, misaligned or too small");
-  const AttnArgs a = {kv->k, kv->v, kv->page_stride, kv->head_stride, kv->pos_stride, kv->n_pages, kv->page_len,
-                      kv->n_kv_heads, kv->head_dim, d_q, q_stride, n_seq, n_heads, d_len, d_table, table_stride,
-                      scale, d_out, out_stride, d_lse};
+  AttnArgs a = {kv->k, kv->v, kv->page_stride, kv->head_stride, kv->pos_stride, kv->n_pages, kv->page_len,
+                kv->n_kv_heads, kv->head_dim, d_q, q_stride, n_seq, n_heads, d_len, d_table, table_stride,
+                scale, d_out, out_stride, d_lse};
+  a.rep = n_heads / kv->n_kv_heads;
+  a.counter = static_cast<uint32_t*>(d_ws);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + counter_bytes(n_seq, n_heads));
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == MLLM_DTYPE_F16)
-    launch_attn<__half, __half>(a, st);
-  else if (dtype == MLLM_DTYPE_BF16)
-    launch_attn<__nv_bfloat16, __nv_bfloat16>(a, st);
-  else if (kv->dtype == MLLM_DTYPE_F16)
-    launch_attn<float, __half>(a, st);
-  else if (kv->dtype == MLLM_DTYPE_BF16)
-    launch_attn<float, __nv_bfloat16>(a, st);
-  else
-    launch_attn<float, float>(a, st);
-  return launched("mllm_paged_attn: launch failed");
+  if (dtype == MLLM_DTYPE_F16) return run_mma<__half, __half>(a, st);
+  if (dtype == MLLM_DTYPE_BF16) return run_mma<__nv_bfloat16, __nv_bfloat16>(a, st);
+  if (kv->dtype == MLLM_DTYPE_F16) return run_mma<__half, float>(a, st);
+  if (kv->dtype == MLLM_DTYPE_BF16) return run_mma<__nv_bfloat16, float>(a, st);
+  return run_f32(a, st);
 }
