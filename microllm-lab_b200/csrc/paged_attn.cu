@@ -14,6 +14,7 @@
 // others leave (m, l, o) in the workspace, and the CTA that counts itself last joins them in the order
 // of their positions, so that the result does not depend on timing and no CTA waits for another.
 #include <algorithm>
+#include <atomic>
 
 #include "device_common.cuh"
 #include "paged.cuh"
@@ -50,16 +51,16 @@ struct AttnArgs {
 };
 
 // ---------------------------------------------------------------------------------------------
-// Loads of cached rows: each byte is used once, so it does not stay in L1.
+// Cached rows travel by asynchronous 16-byte copies into a ring in shared memory of which each lane reads
+// back only what it asked for itself: many more bytes are under way than registers could take, and no
+// barrier is needed, only the lane's own count of copies.
 // ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint4 ld_row(const void* p) {
-  uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+__device__ __forceinline__ void copy16(uint4* to, const void* from, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(ok ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ uint4 ld_row_if(const void* p, bool ok) {
-  return ok ? ld_row(p) : make_uint4(0u, 0u, 0u, 0u);
-}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // 2^x for the softmax; x <= 0, or -inf.
 __device__ __forceinline__ float pow2(float x) { return exp2f(x); }
@@ -174,9 +175,12 @@ __device__ __forceinline__ int64_t row_offset(const AttnArgs& a, const Segment& 
   return page * a.page_stride + g.kv * a.head_stride + (int64_t)(p - pg * a.page_len) * a.pos_stride;
 }
 
-// What the warps of a CTA leave for the join of a segment: m (in units of log 2) and l, then o.
+// What the warps of a CTA leave for the join of a segment: m (in units of log 2) and l, and o, each warp's
+// at the start of its ring.
 struct Joint {
-  float *m, *l, *o;  // [warp][group], [warp][group], [warp][group][DP]
+  float *m, *l;  // [warp][group]
+  float* o;      // [warp] rings, each beginning with [group][DP]
+  int ring;      // floats of a ring
 };
 
 template <class A>
@@ -206,7 +210,7 @@ __device__ void finish(const AttnArgs& a, const Run& r, const Segment& g, const 
       const float mk = w.m[k * a.group_size + h];
       const float f = mk == -INFINITY ? 0.f : pow2(mk - m);
       l = fmaf(f, w.l[k * a.group_size + h], l);
-      o = fmaf(f, w.o[(k * a.group_size + h) * DP + d], o);
+      o = fmaf(f, w.o[k * w.ring + h * DP + d], o);
     }
     if (bad) l = __int_as_float(0x7FC00000);
     if (whole) {
@@ -266,16 +270,15 @@ __device__ void finish_empty(const AttnArgs& a) {
 // ---------------------------------------------------------------------------------------------
 // Caches of 16 bits: both products on the tensor cores, m16n8k16 with positions (then head_dim) as the
 // 16 rows and 8 query heads as the columns, so that a group of few heads wastes little.  The order of the
-// summed index is free as long as both operands share it, so every lane loads 16-byte pieces of cached
-// rows straight into the registers that are its operands: for the scores a lane's 8 neighbouring elements
-// of a key row serve two steps; for the output, pairs of value rows are woven by byte permutes.  Nothing
-// passes through shared memory but the queries.  The scores' accumulators, packed and transposed by
-// movmatrix, are the second product's operand.
+// summed index is free as long as both operands share it, so the 16-byte pieces of cached rows that a lane
+// copies are its operands as they are: for the scores its 8 neighbouring elements of a key row serve two
+// steps; for the output, pairs of value rows are woven by byte permutes.  The scores' accumulators, packed
+// and transposed by movmatrix, are the second product's operand.
 //
-// Queries of the cache's type are exact operands, and the weights are rounded to that type (their sum is
-// not), an error of the size of the output's own rounding.  f32 queries and weights are split into as
-// many 16-bit terms as f32 needs (3 in bf16, 2 in f16, where queries are first scaled by a power of two
-// to at most 1): the cached values are exact in either case.
+// The cached values are exact operands, and so are queries of their type.  f32 queries and weights are
+// split into as many 16-bit terms as f32 needs (3 in bf16, 2 in f16, where queries are first scaled by a
+// power of two to at most 1).  With queries of 16 bits the weights get two terms: one alone would add an
+// error of the size of the output's own rounding (bf16 2.1e-3 of the result against 1.7e-3).
 // ---------------------------------------------------------------------------------------------
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -326,31 +329,78 @@ constexpr int terms_of() { return sizeof(A) == 2 ? 1 : (__is_same(T, __half) ? 2
 template <class T, class A, int DP, int NT>
 constexpr size_t mma_query_bytes() { return (size_t)(DP / 32) * terms_of<T, A>() * NT * 512; }
 
-// CTAs per SM that the register file is split for.
-template <int DP, int NT>
-constexpr int mma_ctas() { return DP == 64 ? 4 : (DP == 128 && NT == 1 ? 3 : 2); }
+// Ring stages of 16 positions, and CTAs per SM: about 190 KB of copies under way on each SM.
+template <int DP>
+constexpr int mma_stages() { return DP == 64 ? 4 : 3; }
+template <int DP>
+constexpr int mma_ctas() { return DP == 64 ? 3 : DP == 128 ? 2 : 1; }
+template <int DP>
+constexpr int mma_ring_bytes() { return mma_stages<DP>() * 16 * 2 * DP * 2; }  // of a warp
 
 template <class T, class A, int DP, int NT>
-__global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_kernel(const AttnArgs a) {
-  constexpr int C = DP / 32, V = DP / 64, J = DP == 64 ? 2 : 1, TERMS = terms_of<T, A>();
+__global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(const AttnArgs a) {
+  constexpr int C = DP / 32, V = DP / 64, S = mma_stages<DP>(), TERMS = terms_of<T, A>(), WT = TERMS == 1 ? 2 : TERMS;
+  constexpr int PIECES = 2 * C + 4 * V;  // 16-byte pieces of a stage per lane
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float qscale[8 * NT];
   __shared__ int bad;
-  uint4* const qs = reinterpret_cast<uint4*>(smem);  // [C][TERMS][NT][32]: each lane's operand words
-  Joint joint;
-  joint.m = reinterpret_cast<float*>(smem + mma_query_bytes<T, A, DP, NT>());
-  joint.l = joint.m + kAttnWarps * a.group_size;
-  joint.o = joint.l + kAttnWarps * a.group_size;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = lane >> 2, quad = lane & 3;
+  uint4* const ring = reinterpret_cast<uint4*>(smem + warp * mma_ring_bytes<DP>()) + lane;  // piece i of stage s: [(s PIECES + i) 32]
+  uint4* const qs = reinterpret_cast<uint4*>(smem + kAttnWarps * mma_ring_bytes<DP>());      // [C][TERMS][NT][32]: operand words
+  Joint joint;
+  joint.o = reinterpret_cast<float*>(smem);
+  joint.ring = mma_ring_bytes<DP>() / 4;
+  joint.m = reinterpret_cast<float*>(qs + C * TERMS * NT * 32);
+  joint.l = joint.m + kAttnWarps * a.group_size;
   const T* const kp = static_cast<const T*>(a.k);
   const T* const vp = static_cast<const T*>(a.v);
 
   Run run = find_run(a);
   Segment g;
   while (next_segment(a, run, g)) {
-    // ---- the group's queries as operand words, every head's rows of 8 * NT columns (0 past the group)
     __syncthreads();  // the last segment's queries and join are done with
     if (tid == 0) bad = 0;
+    __syncthreads();
+    // ---- this warp's stages: both halves of blocks b0 + warp, b0 + warp + 4, ...
+    const int mine = g.b1 - g.b0 > warp ? (g.b1 - g.b0 - warp - 1) / kAttnWarps + 1 : 0;
+    int n = 2 * mine;
+    if (n && (g.b0 + warp + (mine - 1) * kAttnWarps) * kBlock + 16 >= g.len) --n;  // the last half is past the length
+    int64_t off = row_offset(a, g, g.b0 + warp, lane, &bad);
+    int64_t off_next = row_offset(a, g, g.b0 + warp + kAttnWarps, lane, &bad);
+    auto issue = [&](int i) {
+      if (i < n) {
+        uint4* const to = ring + (i % S) * PIECES * 32;
+        const int half = (i & 1) * 16;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // key rows row, row + 8
+          const int64_t at = __shfl_sync(0xffffffffu, off, half + row + 8 * e);
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const int d = c * 32 + quad * 8;
+            const bool ok = at >= 0 && d < a.dim;
+            copy16(to + (2 * c + e) * 32, kp + (ok ? at + d : 0), ok);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // value rows 2 quad, 2 quad + 1, 2 quad + 8, 2 quad + 9
+          const int64_t at = __shfl_sync(0xffffffffu, off, half + (e >> 1) * 8 + quad * 2 + (e & 1));
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const int d = v * 64 + row * 8;
+            const bool ok = at >= 0 && d < a.dim;
+            copy16(to + (2 * C + 4 * v + e) * 32, vp + (ok ? at + d : 0), ok);
+          }
+        }
+        if (i & 1) {
+          off = off_next;
+          off_next = row_offset(a, g, g.b0 + warp + ((i >> 1) + 2) * kAttnWarps, lane, &bad);
+        }
+      }
+      copies_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(i);
+    // ---- the group's queries as operand words, every head's rows of 8 * NT columns (0 past the group)
     const A* const q = static_cast<const A*>(a.q) + g.seq * a.q_stride + (int64_t)g.head0 * a.dim;
     if constexpr (TERMS == 2) {  // f32 queries as f16 terms: scaled to at most 1
       for (int h = warp; h < 8 * NT; h += kAttnWarps) {
@@ -401,160 +451,112 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[v][i][nt][e] = 0.f;
     }
-    int64_t off = row_offset(a, g, g.b0 + warp, lane, &bad);
-    for (int block = g.b0 + warp; block < g.b1; block += kAttnWarps) {
-      const int64_t off_next = row_offset(a, g, block + kAttnWarps, lane, &bad);
+    for (int i = 0; i < n; ++i) {
+      copies_wait<S - 2>();
+      issue(i + S - 1);  // into the stage that the last round read
+      const uint4* const st = ring + (i % S) * PIECES * 32;
+      const int p0 = (g.b0 + warp + (i >> 1) * kAttnWarps) * kBlock + (i & 1) * 16 + row;
+      // ---- scores: 16 positions x heads
+      float s[NT][4];
 #pragma unroll
-      for (int half = 0; half < 2; half += J) {
-        // ---- key and value rows of J x 16 positions
-        uint4 kf[J][C][2], vf[J][V][4];
-        bool live[J][2];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
+        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+      auto score = [&](float (&f)[4], const uint4& k0, const uint4& k1, const uint4& b) {
+        mma<T>(f, k0.x, k1.x, k0.y, k1.y, b.x, b.y);
+        mma<T>(f, k0.z, k1.z, k0.w, k1.w, b.z, b.w);
+      };
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int64_t at = __shfl_sync(0xffffffffu, off, (half + j) * 16 + row + 8 * e);
-            live[j][e] = at >= 0;
+      for (int c = 0; c < C; ++c) {
+        const uint4 k0 = st[(2 * c) * 32], k1 = st[(2 * c + 1) * 32];
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-              const int d = c * 32 + quad * 8;
-              kf[j][c][e] = ld_row_if(kp + at + d, at >= 0 && d < a.dim);
-            }
-          }
+        for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int64_t at = __shfl_sync(0xffffffffu, off, (half + j) * 16 + (e >> 1) * 8 + quad * 2 + (e & 1));
+          for (int nt = 0; nt < NT; ++nt) score(s[nt], k0, k1, qs[((c * TERMS + t) * NT + nt) * 32 + lane]);
+      }
+      if constexpr (TERMS > 1) {
+        // A key of +-inf times a later term of a query (of any sign, or 0) is NaN: there the first
+        // term alone gives the score that f32 products would.
+        bool odd = false;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-              const int d = v * 64 + row * 8;
-              vf[j][v][e] = ld_row_if(vp + at + d, at >= 0 && d < a.dim);
-            }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd |= s[nt][e] != s[nt][e];
+        if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < C; ++c) score(f, st[(2 * c) * 32], st[(2 * c + 1) * 32], qs[(c * TERMS * NT + nt) * 32 + lane]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (s[nt][e] != s[nt][e]) s[nt][e] = f[e];
           }
         }
-        // ---- scores: positions x heads
-        float s[J][NT][4];
+      }
+      // ---- running maximum and sum of this lane's two heads, weights as the second operand
+      uint32_t p[NT][WT][2];
+      float keep[NT][2];
+      bool moved = false;
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 2; ++e) {
+          float x0 = p0 < g.len ? s[nt][e] * sc[nt][e] : -INFINITY;
+          float x1 = p0 + 8 < g.len ? s[nt][2 + e] * sc[nt][e] : -INFINITY;
+          float top = fmaxf(m[nt][e], fmaxf(x0, x1));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][nt][e] = 0.f;
+          for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+          moved |= top != m[nt][e];
+          const float base = top == -INFINITY ? 0.f : top;
+          keep[nt][e] = pow2(m[nt][e] - base);  // 0 while there was nothing
+          m[nt][e] = top;
+          x0 = pow2(x0 - base);
+          x1 = pow2(x1 - base);
+          l[nt][e] = fmaf(l[nt][e], keep[nt][e], x0 + x1);
+          s[nt][e] = x0;
+          s[nt][2 + e] = x1;
+        }
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int t = 0; t < TERMS; ++t)
+        for (int k = 0; k < 2; ++k) {
+          uint32_t w[WT];
+          split2<T, WT>(s[nt][2 * k], s[nt][2 * k + 1], w);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint4 b = qs[((c * TERMS + t) * NT + nt) * 32 + lane];
+          for (int t = 0; t < WT; ++t) p[nt][t][k] = transpose8x8(w[t]);
+        }
+      if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-              for (int j = 0; j < J; ++j) {
-                mma<T>(s[j][nt], kf[j][c][0].x, kf[j][c][1].x, kf[j][c][0].y, kf[j][c][1].y, b.x, b.y);
-                mma<T>(s[j][nt], kf[j][c][0].z, kf[j][c][1].z, kf[j][c][0].w, kf[j][c][1].w, b.z, b.w);
-              }
-            }
-        if constexpr (TERMS > 1) {
-          // A key of +-inf times a later term of a query (of any sign, or 0) is NaN: there the first
-          // term alone gives the score that f32 products would.
-          bool odd = false;
+        for (int v = 0; v < V; ++v)
 #pragma unroll
-          for (int j = 0; j < J; ++j)
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) odd |= s[j][nt][e] != s[j][nt][e];
-          if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float f[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                  const uint4 b = qs[(c * TERMS * NT + nt) * 32 + lane];
-                  mma<T>(f, kf[j][c][0].x, kf[j][c][1].x, kf[j][c][0].y, kf[j][c][1].y, b.x, b.y);
-                  mma<T>(f, kf[j][c][0].z, kf[j][c][1].z, kf[j][c][0].w, kf[j][c][1].w, b.z, b.w);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (s[j][nt][e] != s[j][nt][e]) s[j][nt][e] = f[e];
-              }
-          }
-        }
-        // ---- running maximum and sum of this lane's two heads, weights as the second operand
-        uint32_t p[J][NT][TERMS][2];
-        float keep[NT][2];
-        bool moved = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = m[nt][e];
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                float& x = s[j][nt][2 * k + e];
-                x = live[j][k] ? x * sc[nt][e] : -INFINITY;
-                top = fmaxf(top, x);
-              }
-#pragma unroll
-            for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
-            moved |= top != m[nt][e];
-            const float base = top == -INFINITY ? 0.f : top;
-            keep[nt][e] = pow2(m[nt][e] - base);  // 0 while there was nothing
-            m[nt][e] = top;
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                float& x = s[j][nt][2 * k + e];
-                x = pow2(x - base);
-                sum += x;
-              }
-            l[nt][e] = fmaf(l[nt][e], keep[nt][e], sum);
-          }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < J; ++j)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              uint32_t w[TERMS];
-              split2<T, TERMS>(s[j][nt][2 * k], s[j][nt][2 * k + 1], w);
-#pragma unroll
-              for (int t = 0; t < TERMS; ++t) p[j][nt][t][k] = transpose8x8(w[t]);
-            }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[v][i][nt][e] *= keep[nt][e & 1];
-        }
-        // ---- output: head_dim x heads; rows 8 v + ... of the values woven in pairs of positions
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-          for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t x0 = word(vf[j][v][0], i), x1 = word(vf[j][v][1], i);
-              const uint32_t x2 = word(vf[j][v][2], i), x3 = word(vf[j][v][3], i);
-              const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
-              const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int t = 0; t < TERMS; ++t) mma<T>(o[v][i][nt], a0, a1, a2, a3, p[j][nt][t][0], p[j][nt][t][1]);
-            }
+              for (int e = 0; e < 4; ++e) o[v][k][nt][e] *= keep[nt][e & 1];
       }
-      off = off_next;
+      // ---- output: head_dim x heads, the value rows woven in pairs of positions
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        uint4 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = st[(2 * C + 4 * v + e) * 32];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a0 = __byte_perm(word(x[0], k), word(x[1], k), 0x5410), a1 = __byte_perm(word(x[0], k), word(x[1], k), 0x7632);
+          const uint32_t a2 = __byte_perm(word(x[2], k), word(x[3], k), 0x5410), a3 = __byte_perm(word(x[2], k), word(x[3], k), 0x7632);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int t = 0; t < WT; ++t) mma<T>(o[v][k][nt], a0, a1, a2, a3, p[nt][t][0], p[nt][t][1]);
+        }
+      }
     }
+    copies_wait<0>();
     // ---- leave (m, l, o) for the join
+    float* const jo = joint.o + warp * joint.ring;
+    __syncwarp();  // every lane has read the ring
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -570,9 +572,8 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
 #pragma unroll
           for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<float2*>(joint.o + (warp * a.group_size + h) * DP + v * 64 + row * 8 + 2 * i) =
-                  make_float2(o[v][i][nt][e], o[v][i][nt][2 + e]);
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<float2*>(jo + h * DP + v * 64 + row * 8 + 2 * k) = make_float2(o[v][k][nt][e], o[v][k][nt][2 + e]);
         }
       }
     __syncthreads();
@@ -586,40 +587,89 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
 // share a key row for the scores; for the output a row's elements are spread over the lanes in pieces of
 // four, the weights passing through shared memory.
 // ---------------------------------------------------------------------------------------------
+// Key rows of a stage that a lane shares (stages of 8 R positions), ring stages, CTAs per SM.
+template <int DP>
+constexpr int f32_rows() { return DP == 256 ? 1 : 2; }
+template <int DP>
+constexpr int f32_stages() { return DP == 64 ? 3 : 2; }
+template <int DP>
+constexpr int f32_ctas() { return DP == 64 ? 2 : 1; }
+template <int DP>
+constexpr int f32_ring_bytes() { return f32_stages<DP>() * 8 * f32_rows<DP>() * 2 * DP * 4; }  // of a warp
 template <int DP, int G>
-constexpr size_t f32_query_bytes() { return (size_t)G * DP * 4 + (size_t)kAttnWarps * kBlock * G * 4; }
+constexpr size_t f32_query_bytes() { return (size_t)G * DP * 4 + (size_t)kAttnWarps * 8 * f32_rows<DP>() * G * 4; }
 
 template <int DP, int G>
-__global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 3 : 2) attn_f32_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(const AttnArgs a) {
+  constexpr int R = f32_rows<DP>(), P = 8 * R, S = f32_stages<DP>(), PARTS = kBlock / P;  // stages of a block
   constexpr int C = DP / 16, PER = DP / 4 < 32 ? DP / 4 : 32, ROWS = 32 / PER, V = DP / 4 / PER;
+  constexpr int PIECES = R * C + P / ROWS * V;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int bad;
-  float* const qs = reinterpret_cast<float*>(smem);       // [G][DP]
-  float* const ps = qs + G * DP;                          // [warp][position][G]
-  Joint joint;
-  joint.m = reinterpret_cast<float*>(smem + f32_query_bytes<DP, G>());
-  joint.l = joint.m + kAttnWarps * a.group_size;
-  joint.o = joint.l + kAttnWarps * a.group_size;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = lane >> 2, quad = lane & 3;
-  float* const pw = ps + warp * kBlock * G;
+  uint4* const ring = reinterpret_cast<uint4*>(smem + warp * f32_ring_bytes<DP>()) + lane;
+  float* const qs = reinterpret_cast<float*>(smem + kAttnWarps * f32_ring_bytes<DP>());  // [G][DP]
+  float* const pw = qs + G * DP + warp * P * G;                                            // [position][G]
+  Joint joint;
+  joint.o = reinterpret_cast<float*>(smem);
+  joint.ring = f32_ring_bytes<DP>() / 4;
+  joint.m = qs + G * DP + kAttnWarps * P * G;
+  joint.l = joint.m + kAttnWarps * a.group_size;
   const float* const kp = static_cast<const float*>(a.k);
   const float* const vp = static_cast<const float*>(a.v);
-  auto f4 = [](const uint4& u) {
-    return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
-  };
+  const float sc = a.scale * kLog2e;
 
   Run run = find_run(a);
   Segment g;
   while (next_segment(a, run, g)) {
     __syncthreads();
     if (tid == 0) bad = 0;
+    __syncthreads();
+    const int mine = g.b1 - g.b0 > warp ? (g.b1 - g.b0 - warp - 1) / kAttnWarps + 1 : 0;
+    int n = PARTS * mine;
+    while (n && (g.b0 + warp + (mine - 1) * kAttnWarps) * kBlock + ((n - 1) % PARTS) * P >= g.len) --n;
+    int64_t off = row_offset(a, g, g.b0 + warp, lane, &bad);
+    int64_t off_next = row_offset(a, g, g.b0 + warp + kAttnWarps, lane, &bad);
+    auto issue = [&](int i) {
+      if (i < n) {
+        uint4* const to = ring + (i % S) * PIECES * 32;
+        const int part = (i % PARTS) * P;
+#pragma unroll
+        for (int e = 0; e < R; ++e) {
+          const int64_t at = __shfl_sync(0xffffffffu, off, part + row + 8 * e);
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const int d = c * 16 + quad * 4;
+            const bool ok = at >= 0 && d < a.dim;
+            copy16(to + (c * R + e) * 32, kp + (ok ? at + d : 0), ok);
+          }
+        }
+#pragma unroll
+        for (int p = 0; p < P / ROWS; ++p) {
+          const int64_t at = __shfl_sync(0xffffffffu, off, part + p * ROWS + lane / PER);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const int d = (v * PER + lane % PER) * 4;
+            const bool ok = at >= 0 && d < a.dim;
+            copy16(to + (R * C + p * V + v) * 32, vp + (ok ? at + d : 0), ok);
+          }
+        }
+        if (i % PARTS == PARTS - 1) {
+          off = off_next;
+          off_next = row_offset(a, g, g.b0 + warp + (i / PARTS + 2) * kAttnWarps, lane, &bad);
+        }
+      }
+      copies_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(i);
     const float* const q = static_cast<const float*>(a.q) + g.seq * a.q_stride + (int64_t)g.head0 * a.dim;
     for (int i = tid; i < G * DP; i += kAttnThreads) {
       const int h = i / DP, d = i - h * DP;
       qs[i] = h < g.heads && d < a.dim ? q[h * a.dim + d] : 0.f;
     }
     __syncthreads();
-    float m[G], l[G];       // of every head, the same on every lane (l: this lane's positions)
+    float m[G], l[G];  // of every head: m the same on every lane, l of this lane's positions
     float o[V][G][4];
 #pragma unroll
     for (int h = 0; h < G; ++h) {
@@ -630,45 +680,42 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 3 : 2) attn_f32_kerne
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[v][h][e] = 0.f;
     }
-    const float sc = a.scale * kLog2e;
-    int64_t off = row_offset(a, g, g.b0 + warp, lane, &bad);
-    for (int block = g.b0 + warp; block < g.b1; block += kAttnWarps) {
-      const int64_t off_next = row_offset(a, g, block + kAttnWarps, lane, &bad);
-      // ---- scores of rows row, row + 8, row + 16, row + 24
-      float s[4][G];
-      int64_t at[4];
+    for (int i = 0; i < n; ++i) {
+      copies_wait<S - 2>();
+      issue(i + S - 1);
+      const float4* const st = reinterpret_cast<const float4*>(ring + (i % S) * PIECES * 32);
+      const int p0 = (g.b0 + warp + (i / PARTS) * kAttnWarps) * kBlock + (i % PARTS) * P + row;
+      // ---- scores of rows row, row + 8, ...
+      float s[R][G];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        at[e] = __shfl_sync(0xffffffffu, off, row + 8 * e);
+      for (int e = 0; e < R; ++e)
 #pragma unroll
         for (int h = 0; h < G; ++h) s[e][h] = 0.f;
-      }
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int d = c * 16 + quad * 4;
-        float4 k[4];
+        float4 k[R];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) k[e] = f4(ld_row_if(kp + at[e] + d, at[e] >= 0 && d < a.dim));
+        for (int e = 0; e < R; ++e) k[e] = st[(c * R + e) * 32];
 #pragma unroll
         for (int h = 0; h < G; ++h) {
-          const float4 x = *reinterpret_cast<const float4*>(qs + h * DP + d);
+          const float4 x = *reinterpret_cast<const float4*>(qs + h * DP + c * 16 + quad * 4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < R; ++e)
             s[e][h] = fmaf(k[e].x, x.x, fmaf(k[e].y, x.y, fmaf(k[e].z, x.z, fmaf(k[e].w, x.w, s[e][h]))));
         }
       }
       bool moved = false;
       float keep[G];
-      __syncwarp();  // the last block's weights are read
+      __syncwarp();  // the last round's weights are read
 #pragma unroll
       for (int h = 0; h < G; ++h) {
         float top = m[h];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < R; ++e) {
           float x = s[e][h];
           x += __shfl_xor_sync(0xffffffffu, x, 1);
           x += __shfl_xor_sync(0xffffffffu, x, 2);
-          s[e][h] = at[e] >= 0 ? x * sc : -INFINITY;
+          s[e][h] = p0 + 8 * e < g.len ? x * sc : -INFINITY;
           top = fmaxf(top, s[e][h]);
         }
 #pragma unroll
@@ -677,11 +724,12 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 3 : 2) attn_f32_kerne
         const float base = top == -INFINITY ? 0.f : top;
         keep[h] = pow2(m[h] - base);
         m[h] = top;
-        // lane quad e of a row holds the weight of row + 8 e
-        const float x = quad == 0 ? s[0][h] : quad == 1 ? s[1][h] : quad == 2 ? s[2][h] : s[3][h];
-        const float w = pow2(x - base);
-        l[h] = fmaf(l[h], keep[h], w);
-        pw[(row + 8 * quad) * G + h] = w;
+        l[h] *= keep[h];
+        if (quad < R) {  // lane e of a row's four holds the weight of row + 8 e
+          const float w = pow2((R == 1 || quad == 0 ? s[0][h] : s[R - 1][h]) - base);
+          l[h] += w;
+          pw[(row + 8 * quad) * G + h] = w;
+        }
       }
       __syncwarp();
       if (moved) {  // the maxima are the same on every lane
@@ -693,17 +741,15 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 3 : 2) attn_f32_kerne
             for (int e = 0; e < 4; ++e) o[v][h][e] *= keep[h];
       }
       // ---- output: ROWS value rows at a time
-#pragma unroll 8
-      for (int p = 0; p < kBlock; p += ROWS) {
-        const int r = p + lane / PER;
-        const int64_t av = __shfl_sync(0xffffffffu, off, r);
+#pragma unroll
+      for (int p = 0; p < P / ROWS; ++p) {
         float w[G];
 #pragma unroll
-        for (int h = 0; h < G; h += 4) *reinterpret_cast<float4*>(w + h) = *reinterpret_cast<const float4*>(pw + r * G + h);
+        for (int h = 0; h < G; h += 4)
+          *reinterpret_cast<float4*>(w + h) = *reinterpret_cast<const float4*>(pw + (p * ROWS + lane / PER) * G + h);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const int d = (v * PER + lane % PER) * 4;
-          const float4 x = f4(ld_row_if(vp + av + d, av >= 0 && d < a.dim));
+          const float4 x = st[(R * C + p * V + v) * 32];
 #pragma unroll
           for (int h = 0; h < G; ++h) {
             o[v][h][0] = fmaf(w[h], x.x, o[v][h][0]);
@@ -713,8 +759,10 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 3 : 2) attn_f32_kerne
           }
         }
       }
-      off = off_next;
     }
+    copies_wait<0>();
+    float* const jo = joint.o + warp * joint.ring;
+    __syncwarp();  // every lane has read the ring
 #pragma unroll
     for (int h = 0; h < G; ++h) {
       l[h] = warp_sum(l[h]);
@@ -731,8 +779,7 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 3 : 2) attn_f32_kerne
             for (int b = PER; b < 32; b <<= 1) o[v][h][e] += __shfl_xor_sync(0xffffffffu, o[v][h][e], b);
           }
           if (lane < PER)
-            *reinterpret_cast<float4*>(joint.o + (warp * a.group_size + h) * DP + (v * PER + lane) * 4) =
-                make_float4(o[v][h][0], o[v][h][1], o[v][h][2], o[v][h][3]);
+            *reinterpret_cast<float4*>(jo + h * DP + (v * PER + lane) * 4) = make_float4(o[v][h][0], o[v][h][1], o[v][h][2], o[v][h][3]);
         }
       }
     }
@@ -747,26 +794,34 @@ __global__ void __launch_bounds__(kAttnThreads, DP == 64 ? 3 : 2) attn_f32_kerne
 // ---------------------------------------------------------------------------------------------
 size_t counter_bytes(int n_seq, int n_heads) { return (((size_t)n_seq * n_heads * 4 + 255) / 256) * 256; }
 
-template <class K>
-int launch(K kernel, const AttnArgs& a, int per_sm, size_t smem, cudaStream_t st) {
+// Opt in to more than 48 KB of shared memory, once per kernel and device.
+template <auto KERNEL>
+bool allow_smem(int dev, size_t smem) {
+  static std::atomic<uint64_t> done{0};
+  if (smem <= 48 * 1024 || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return true;
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess) return false;
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return true;
+}
+
+template <auto KERNEL>
+int launch(const AttnArgs& a, int per_sm, size_t smem, cudaStream_t st) {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: no current CUDA device");
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: not enough shared memory");
+  smem += (size_t)2 * kAttnWarps * a.group_size * 4;  // m and l of the join
+  if (!allow_smem<KERNEL>(dev, smem)) return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: not enough shared memory");
   // no more CTAs than runs of the shortest length over the whole table
   const int64_t blocks = ((int64_t)a.table_stride * a.page_len + kBlock - 1) / kBlock;
   const int64_t most = (blocks + kMinBlocks - 1) / kMinBlocks * a.n_seq * a.n_kv * a.groups;
   const int grid = (int)std::min<int64_t>(most, std::min(kMaxCtas, sms * per_sm));
-  kernel<<<grid, kAttnThreads, smem, st>>>(a);
+  KERNEL<<<grid, kAttnThreads, smem, st>>>(a);
   return launched("mllm_paged_attn: launch failed");
 }
 
-size_t joint_bytes(const AttnArgs& a, int dp) { return (size_t)kAttnWarps * a.group_size * (dp + 2) * 4; }
-
 template <class T, class A, int DP, int NT>
 int launch_mma(const AttnArgs& a, cudaStream_t st) {
-  return launch(attn_mma_kernel<T, A, DP, NT>, a, mma_ctas<DP, NT>(), mma_query_bytes<T, A, DP, NT>() + joint_bytes(a, DP), st);
+  return launch<attn_mma_kernel<T, A, DP, NT>>(a, mma_ctas<DP>(), kAttnWarps * mma_ring_bytes<DP>() + mma_query_bytes<T, A, DP, NT>(), st);
 }
 template <class T, class A>
 int run_mma(AttnArgs& a, cudaStream_t st) {
@@ -779,7 +834,7 @@ int run_mma(AttnArgs& a, cudaStream_t st) {
 }
 template <int DP, int G>
 int launch_f32(const AttnArgs& a, cudaStream_t st) {
-  return launch(attn_f32_kernel<DP, G>, a, DP == 64 ? 3 : 2, f32_query_bytes<DP, G>() + joint_bytes(a, DP), st);
+  return launch<attn_f32_kernel<DP, G>>(a, f32_ctas<DP>(), kAttnWarps * f32_ring_bytes<DP>() + f32_query_bytes<DP, G>(), st);
 }
 int run_f32(AttnArgs& a, cudaStream_t st) {
   a.group_size = std::min(a.rep, 8);
