@@ -6,13 +6,15 @@
 // (m, l, o) into (M, l e^(m - M) + sum e^(s - M), o e^(m - M) + sum e^(s - M) v), M = max(m, m').  Two
 // multiply-adds per cached element and query head of its group: bound by the bytes of the cache.
 //
-// Work is cut into blocks of 32 positions of one (sequence, kv head, group of query heads), numbered in
-// that order over the whole batch.  Every CTA takes an equal run of them, whatever the lengths: it sums
-// the lengths itself, so that they may live on the device and the grid does not depend on them.  A run
-// covers parts of a segment (a sequence's kv head) or several; the warps of a CTA take its blocks in turn
-// and join their (m, l, o) in shared memory.  A segment that lies in one CTA is written at once; the
-// others leave (m, l, o) in the workspace, and the CTA that counts itself last joins them in the order
-// of their positions, so that the result does not depend on timing and no CTA waits for another.
+// Work is cut into blocks of 32 positions of one segment (a sequence's kv head and group of query heads),
+// numbered segment by segment over the whole batch.  Every CTA takes an equal run of blocks, whatever the
+// lengths, and so does every warp within it: a warp walks its run on its own, through the ends of segments.
+// The CTAs sum the lengths themselves, so that these may live on the device and the grid does not depend
+// on them.  A segment that lies in one warp's run is written at once; the parts of the others are joined
+// by the CTA in shared memory, and what spans CTAs through the workspace by the CTA that counts itself
+// last, always in the order of positions: the result does not depend on timing, and no CTA waits for
+// another.  Where every segment is short and can have a CTA of its own, it gets one, which saves the
+// second join.
 #include <algorithm>
 #include <atomic>
 
@@ -28,6 +30,8 @@ constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kBlock = 32;       // positions per block: one per lane for the page lookups
 constexpr int kMinBlocks = 4;    // a CTA's run is at least one block per warp
+constexpr int kWholeBlocks = 16; // segments up to this long get a CTA of their own where there are enough CTAs
+constexpr int kMaxParts = 64;    // CTAs that one segment is spread over: one CTA reads all their parts
 constexpr int kMaxCtas = 1024;   // partial slots in the workspace
 constexpr int kMaxGroup = 16;    // query heads of a group
 constexpr float kLog2e = 1.4426950408889634f;
@@ -46,7 +50,7 @@ struct AttnArgs {
   int64_t out_stride;
   float* lse;
   uint32_t* counter;  // [n_seq][n_kv][groups]
-  float* part;        // [CTA][2][group][dim + 2]
+  float* part;        // [CTA][2]: o [group][dim], (m, l) [group]
   int rep, group_size, groups;  // query heads per kv head, of a group, groups of a kv head
 };
 
@@ -66,191 +70,302 @@ __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_grou
 __device__ __forceinline__ float pow2(float x) { return exp2f(x); }
 
 // ---------------------------------------------------------------------------------------------
-// A CTA's run of blocks.
+// Runs of blocks.
 // ---------------------------------------------------------------------------------------------
-struct Run {
-  int64_t q;          // blocks per CTA
-  int64_t u, end;     // next block, end of the run
-  int64_t before;     // blocks of the sequences before `seq`, per (kv head, group)
-  int seq;
-};
-
 __device__ __forceinline__ int blocks_of(const AttnArgs& a, int s) {
-  const int n = a.len[s];
+  const int n = __ldg(a.len + s);
   return n <= 0 || (int64_t)n > (int64_t)a.table_stride * a.page_len ? 0 : (n - 1) / kBlock + 1;
 }
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {  // a >= 0, b > 0; nearly always of 32 bits
+  return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
+// A place in the batch: block b of segment (seq, j), j = kv head * groups + group.
+struct Place {
+  int seq, j, b, nb, len;
+  __device__ __forceinline__ void at_seq(const AttnArgs& a, int s) {
+    seq = s;
+    nb = blocks_of(a, s);
+    len = __ldg(a.len + s);
+  }
+  // To the next block; only called while more blocks follow.
+  __device__ __forceinline__ void next(const AttnArgs& a) {
+    if (++b < nb) return;
+    b = 0;
+    if (++j < a.n_kv * a.groups) return;
+    j = 0;
+    do at_seq(a, seq + 1);
+    while (!nb);
+  }
+};
+
+// What a CTA knows of the partition, and this warp's run.
+struct Run {
+  int64_t q;      // blocks of a CTA's run
+  int64_t u, n;   // first block of this warp's run, blocks in it (0: none)
+  bool whole;     // every CTA has one whole segment (numbered as if all were equally long)
+  Place from;
+};
 
 __device__ __forceinline__ Run find_run(const AttnArgs& a) {
-  __shared__ int64_t wsum[kAttnWarps], s_before;
-  __shared__ int s_seq;
+  __shared__ int64_t wsum[kAttnWarps], s_before[kAttnWarps];
+  __shared__ int wused[kAttnWarps], wlong[kAttnWarps], s_seq[kAttnWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.n_seq + kAttnThreads - 1) / kAttnThreads;
   const int s0 = min(tid * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
-  int64_t mine = 0;
-  for (int s = s0; s < s1; ++s) mine += blocks_of(a, s);
-  int64_t run = mine;
+  int64_t mine = 0;          // blocks of this thread's sequences
+  int used = 0, longest = 0;  // those that have any, the longest
+  for (int s = s0; s < s1; ++s) {
+    const int nb = blocks_of(a, s);
+    mine += nb;
+    used += nb > 0;
+    longest = max(longest, nb);
+  }
+  int64_t sum = mine;
+  int count = used;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += up;
+    const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+    const int uc = __shfl_up_sync(0xffffffffu, count, o);
+    if (lane >= o) {
+      sum += up;
+      count += uc;
+    }
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
   }
-  if (lane == 31) wsum[warp] = run;
+  if (lane == 31) {
+    wsum[warp] = sum;
+    wused[warp] = count;
+    wlong[warp] = longest;
+  }
   __syncthreads();
   int64_t total = 0, lead = 0;
+  int all_used = 0, lead_used = 0;
 #pragma unroll
   for (int w = 0; w < kAttnWarps; ++w) {
-    if (w == warp) lead = total;
-    total += wsum[w];
-  }
-  const int64_t per_block = (int64_t)a.n_kv * a.groups;
-  const int64_t all = total * per_block;
-  Run r;
-  r.q = max((int64_t)kMinBlocks, (all + gridDim.x - 1) / gridDim.x);
-  r.u = blockIdx.x * r.q;
-  r.end = min(r.u + r.q, all);
-  r.seq = 0;
-  r.before = 0;
-  if (r.u >= all) return r;  // nothing (the same on every thread)
-  int64_t b = lead + run - mine;  // blocks before this thread's sequences
-  if (r.u >= b * per_block && r.u < (b + mine) * per_block) {
-    int s = s0;
-    for (;; ++s) {
-      const int n = blocks_of(a, s);
-      if (r.u < (b + n) * per_block) break;
-      b += n;
+    if (w == warp) {
+      lead = total;
+      lead_used = all_used;
     }
-    s_seq = s;
-    s_before = b;
+    total += wsum[w];
+    all_used += wused[w];
+    longest = max(longest, wlong[w]);
+  }
+  const int per_block = a.n_kv * a.groups;
+  Run r;
+  r.whole = longest <= kWholeBlocks && (int64_t)all_used * per_block <= gridDim.x;
+  int64_t all, before;  // of this thread's sequences
+  if (r.whole) {
+    all = (int64_t)all_used * longest;
+    before = (int64_t)(lead_used + count - used) * longest;
+    r.q = longest;
+  } else {
+    all = total;
+    before = lead + sum - mine;
+    r.q = max(max(divide(all * per_block + gridDim.x - 1, gridDim.x), (int64_t)kMinBlocks), (int64_t)(longest + kMaxParts - 1) / kMaxParts);
+  }
+  // the sequences in which the warps' runs begin
+  const int64_t u0 = blockIdx.x * r.q, end = min(u0 + r.q, all * per_block);
+  r.n = 0;
+  if (u0 >= end) return r;
+  const int64_t each = r.whole ? 0 : (end - u0 + kAttnWarps - 1) / kAttnWarps;
+#pragma unroll
+  for (int w = 0; w < kAttnWarps; ++w) {
+    const int64_t u = u0 + w * each, mine_all = r.whole ? (int64_t)used * longest : mine;
+    if (u >= before * per_block && u < (before + mine_all) * per_block) {
+      int64_t b = before;
+      int s = s0;
+      for (;; ++s) {
+        const int nb = blocks_of(a, s), n = r.whole && nb ? longest : nb;
+        if (u < (b + n) * per_block) break;
+        b += n;
+      }
+      s_seq[w] = s;
+      s_before[w] = b;
+    }
   }
   __syncthreads();
-  r.seq = s_seq;
-  r.before = s_before;
+  r.u = u0 + warp * each;
+  r.n = min(each, end - r.u);
+  if (!r.whole && r.n <= 0) {
+    r.n = 0;
+    return r;
+  }
+  r.from.at_seq(a, s_seq[warp]);
+  const int64_t in = r.u - s_before[warp] * per_block;
+  const int n = r.whole ? longest : r.from.nb;
+  r.from.j = (int)divide(in, n);
+  r.from.b = (int)(in - (int64_t)r.from.j * n);
+  if (r.whole) {  // the warps share the blocks of the one segment
+    const int share = (r.from.nb + kAttnWarps - 1) / kAttnWarps;
+    r.from.b = warp * share;
+    r.u += r.from.b;
+    r.n = max(min(share, r.from.nb - r.from.b), 0);
+  }
   return r;
 }
 
-// The part of a run that lies in one segment.
-struct Segment {
-  int seq, kv, group, len;
-  int b0, b1;          // blocks of the segment in this run
-  int nb;              // blocks of the segment
-  int64_t start;       // its first block in the batch's numbering
-  int heads;           // query heads of the group
-  int head0;           // the first of them
-};
-
-__device__ __forceinline__ bool next_segment(const AttnArgs& a, Run& r, Segment& g) {
-  if (r.u >= r.end) return false;
-  const int64_t per_block = (int64_t)a.n_kv * a.groups;
-  int nb = blocks_of(a, r.seq);
-  while (r.u >= (r.before + nb) * per_block) {
-    r.before += nb;
-    nb = blocks_of(a, ++r.seq);
-  }
-  const int64_t in = r.u - r.before * per_block;
-  const int j = (int)(in / nb);
-  g.seq = r.seq;
-  g.nb = nb;
-  g.len = a.len[r.seq];
-  g.kv = j / a.groups;
-  g.group = j - g.kv * a.groups;
-  g.b0 = (int)(in - (int64_t)j * nb);
-  g.b1 = (int)min((int64_t)nb, g.b0 + (r.end - r.u));
-  g.start = r.u - g.b0;
-  g.heads = min(a.rep - g.group * a.group_size, a.group_size);
-  g.head0 = g.kv * a.rep + g.group * a.group_size;
-  r.u += g.b1 - g.b0;
-  return true;
-}
-
-// Element offset of this lane's position of a block, -1 when it is past the length or its page is bad.
-__device__ __forceinline__ int64_t row_offset(const AttnArgs& a, const Segment& g, int block, int lane, int* bad) {
-  const int p = block * kBlock + lane;
-  if (block >= g.b1 || p >= g.len) return -1;
+// Element offset of this lane's position of a block, -1 when it is past the length or its page is bad
+// (noted in bit ord of `bad`).
+__device__ __forceinline__ int64_t row_offset(const AttnArgs& a, const Place& c, int lane, uint32_t& bad, int ord) {
+  const int p = c.b * kBlock + lane;
+  if (p >= c.len) return -1;
   const int pg = p / a.page_len;
-  const int page = __ldg(a.table + (int64_t)g.seq * a.table_stride + pg);
+  const int page = __ldg(a.table + (int64_t)c.seq * a.table_stride + pg);
   if ((unsigned)page >= (unsigned)a.n_pages) {
-    *bad = 1;
+    bad |= 1u << (ord & 31);
     return -1;
   }
-  return page * a.page_stride + g.kv * a.head_stride + (int64_t)(p - pg * a.page_len) * a.pos_stride;
+  return page * a.page_stride + c.j / a.groups * a.head_stride + (int64_t)(p - pg * a.page_len) * a.pos_stride;
+}
+__device__ __forceinline__ int first_head(const AttnArgs& a, int j) {
+  return j / a.groups * a.rep + j % a.groups * a.group_size;
+}
+__device__ __forceinline__ int heads_of(const AttnArgs& a, int j) {
+  return min(a.rep - j % a.groups * a.group_size, a.group_size);
 }
 
-// What the warps of a CTA leave for the join of a segment: m (in units of log 2) and l, and o, each warp's
-// at the start of its ring.
+// A part of a segment: what one run holds of it.
+struct Part {
+  int seq, j, b0, blocks, nb;  // blocks 0: none
+};
+// The parts that a CTA's warps leave for the join: of a run's first segment (slot 0) and of its last (slot
+// 1).  m is in units of log 2.  A page id outside the pool makes l, and with it the result, NaN.
 struct Joint {
-  float *m, *l;  // [warp][group]
-  float* o;      // [warp] rings, each beginning with [group][DP]
-  int ring;      // floats of a ring
+  Part* part;           // [warp][2]
+  float *m, *l;         // [warp][2][group]
+  float *first, *ring;  // o [group][DP]: slot 0 in `first`, slot 1 at the start of the warp's ring
+  int ring_floats;
+  template <int DP>
+  __device__ __forceinline__ float* o(const AttnArgs& a, int warp, int slot) const {
+    return slot ? ring + warp * ring_floats : first + warp * a.group_size * DP;
+  }
 };
 
-template <class A>
-__device__ __forceinline__ void write_out(const AttnArgs& a, const Segment& g, int h, int d, float o, float l) {
-  static_cast<A*>(a.out)[g.seq * a.out_stride + (int64_t)(g.head0 + h) * a.dim + d] = from_f32<A>(l == 0.f ? 0.f : o / l);
+__device__ __forceinline__ float4 rows4(const float4& v, float f) { return make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
+__device__ __forceinline__ float4 fma4(float f, const float4& x, const float4& y) {
+  return make_float4(fmaf(f, x.x, y.x), fmaf(f, x.y, y.y), fmaf(f, x.z, y.z), fmaf(f, x.w, y.w));
 }
-__device__ __forceinline__ void write_lse(const AttnArgs& a, const Segment& g, int h, float m, float l) {
-  if (a.lse) a.lse[(int64_t)g.seq * a.n_heads + g.head0 + h] = (m + log2f(l)) * (1.f / kLog2e);
+template <class A>
+__device__ __forceinline__ void store4(A* p, const float4& v) {  // p on a 4-element boundary
+  if constexpr (sizeof(A) == 4) {
+    *reinterpret_cast<float4*>(p) = v;
+  } else {
+    A e[4] = {from_f32<A>(v.x), from_f32<A>(v.y), from_f32<A>(v.z), from_f32<A>(v.w)};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(e);
+  }
+}
+// Four elements of a finished row of head h of the group; l == 0: no position had a weight.
+template <class A>
+__device__ __forceinline__ void write_out(const AttnArgs& a, int seq, int j, int h, int d, const float4& o, float l) {
+  A* out = static_cast<A*>(a.out) + seq * a.out_stride + (int64_t)(first_head(a, j) + h) * a.dim + d;
+  store4(out, l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x / l, o.y / l, o.z / l, o.w / l));
+}
+__device__ __forceinline__ void write_lse(const AttnArgs& a, int seq, int j, int h, float m, float l) {
+  if (a.lse) a.lse[(int64_t)seq * a.n_heads + first_head(a, j) + h] = (m + log2f(l)) * (1.f / kLog2e);
 }
 
-// Joins the warps' (m, l, o); writes the segment's rows, or its part of them, and joins the parts when
-// this CTA is the last to leave one.
+// Joins the parts that the warps left, and those of other CTAs where this is the last CTA of a segment.
 template <class A, int DP>
-__device__ void finish(const AttnArgs& a, const Run& r, const Segment& g, const Joint& w, int bad) {
-  __shared__ int last;
-  const int tid = threadIdx.x;
-  const bool whole = g.b0 == 0 && g.b1 == g.nb;
-  const size_t slot = (size_t)a.group_size * (a.dim + 2);
-  float* part = a.part + ((size_t)blockIdx.x * 2 + (g.b0 == 0)) * slot;
-  for (int i = tid; i < g.heads * a.dim; i += kAttnThreads) {
-    const int h = i / a.dim, d = i - h * a.dim;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-#pragma unroll
-    for (int k = 0; k < kAttnWarps; ++k) m = fmaxf(m, w.m[k * a.group_size + h]);
-#pragma unroll
-    for (int k = 0; k < kAttnWarps; ++k) {
-      const float mk = w.m[k * a.group_size + h];
-      const float f = mk == -INFINITY ? 0.f : pow2(mk - m);
-      l = fmaf(f, w.l[k * a.group_size + h], l);
-      o = fmaf(f, w.o[k * w.ring + h * DP + d], o);
+__device__ void join(const AttnArgs& a, const Run& r, const Joint& w) {
+  __shared__ int s_last[2];
+  const int tid = threadIdx.x, quads = a.dim / 4;
+  const size_t slot = (size_t)a.group_size * (a.dim + 4);  // o, then m and l; 16-byte aligned for any group
+  Part open[2];  // the segments that go on in other CTAs: begun before this CTA, or in it
+  open[0].blocks = open[1].blocks = 0;
+  __syncthreads();
+  for (int i = 0; i < 2 * kAttnWarps;) {
+    const Part p = w.part[i];
+    if (!p.blocks) {
+      ++i;
+      continue;
     }
-    if (bad) l = __int_as_float(0x7FC00000);
-    if (whole) {
-      write_out<A>(a, g, h, d, o, l);
-      if (d == 0) write_lse(a, g, h, m, l);
-    } else {
-      part[i] = o;
-      if (d == 0) {
-        part[a.group_size * a.dim + 2 * h] = m;
-        part[a.group_size * a.dim + 2 * h + 1] = l;
+    int have = 0, end = i;  // parts i .. end - 1 are of this segment
+    for (; end < 2 * kAttnWarps; ++end) {
+      const Part& q = w.part[end];
+      if (!q.blocks) continue;
+      if (q.seq != p.seq || q.j != p.j) break;
+      have += q.blocks;
+    }
+    const bool done = have == p.nb;
+    const int side = p.b0 == 0;
+    float* const out = a.part + ((size_t)blockIdx.x * 2 + side) * slot;
+    const int heads = heads_of(a, p.j);
+    for (int x = tid; x < heads * quads; x += kAttnThreads) {
+      const int h = x / quads, d = (x - h * quads) * 4;
+      float m = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = i; k < end; ++k)
+        if (w.part[k].blocks) m = fmaxf(m, w.m[k * a.group_size + h]);
+      for (int k = i; k < end; ++k) {
+        if (!w.part[k].blocks) continue;
+        const float mk = w.m[k * a.group_size + h], f = mk == -INFINITY ? 0.f : pow2(mk - m);
+        l = fmaf(f, w.l[k * a.group_size + h], l);
+        o = fma4(f, *reinterpret_cast<const float4*>(w.o<DP>(a, k >> 1, k & 1) + h * DP + d), o);
+      }
+      if (done) {
+        write_out<A>(a, p.seq, p.j, h, d, o, l);
+        if (d == 0) write_lse(a, p.seq, p.j, h, m, l);
+      } else {
+        *reinterpret_cast<float4*>(out + h * a.dim + d) = o;
+        if (d == 0) *reinterpret_cast<float2*>(out + a.group_size * a.dim + 2 * h) = make_float2(m, l);
       }
     }
-  }
-  if (whole) return;
-  const int first = (int)(g.start / r.q), parts = (int)((g.start + g.nb - 1) / r.q) - first + 1;
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    uint32_t* c = a.counter + ((int64_t)g.seq * a.n_kv + g.kv) * a.groups + g.group;
-    last = atomicAdd(c, 1u) == (uint32_t)parts - 1;
-    if (last) *c = 0;
-  }
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  for (int i = tid; i < g.heads * a.dim; i += kAttnThreads) {
-    const int h = i / a.dim;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-      const float* p = a.part + ((size_t)(first + k) * 2 + (k == 0)) * slot;
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + a.group_size * a.dim) + h);
-      const float ok = __ldcg(p + i), mn = fmaxf(m, ml.x);
-      const float f0 = m == -INFINITY ? 0.f : pow2(m - mn), f1 = ml.x == -INFINITY ? 0.f : pow2(ml.x - mn);
-      l = l * f0 + ml.y * f1;
-      o = o * f0 + ok * f1;
-      m = mn;
+    if (!done && side == 0) {
+      open[0] = p;
+      open[0].blocks = have;
+    } else if (!done) {
+      open[1] = p;
+      open[1].blocks = have;
     }
-    write_out<A>(a, g, h, i - h * a.dim, o, l);
-    if (i == h * a.dim) write_lse(a, g, h, m, l);
+    i = end;
+  }
+  if (!open[0].blocks && !open[1].blocks) return;
+  // which CTAs have a part, from the segment's first block in the batch: one that begins in this CTA's run
+  // goes on to its end
+  const int64_t u0 = blockIdx.x * r.q;
+  int first[2], parts[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t start = i == 0 ? u0 - open[0].b0 : u0 + r.q - open[1].blocks;
+    first[i] = open[i].blocks ? (int)divide(start, r.q) : 0;
+    parts[i] = open[i].blocks ? (int)divide(start + open[i].nb - 1, r.q) - first[i] + 1 : 0;
+  }
+  __threadfence();
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (tid == 32 * i && open[i].blocks) {
+      uint32_t* c = a.counter + (int64_t)open[i].seq * a.n_kv * a.groups + open[i].j;
+      s_last[i] = atomicAdd(c, 1u) == (uint32_t)parts[i] - 1;
+      if (s_last[i]) *c = 0;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (!open[i].blocks || !s_last[i]) continue;
+    __threadfence();
+    const Part& p = open[i];
+    const int heads = heads_of(a, p.j);
+    for (int x = tid; x < heads * quads; x += kAttnThreads) {
+      const int h = x / quads, d = (x - h * quads) * 4;
+      float m = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int k = 0; k < parts[i]; ++k) {
+        const float* q = a.part + ((size_t)(first[i] + k) * 2 + (k == 0)) * slot;
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + a.group_size * a.dim) + h);
+        const float4 ok = __ldcg(reinterpret_cast<const float4*>(q + h * a.dim + d));
+        const float top = fmaxf(m, ml.x);
+        const float f0 = m == -INFINITY ? 0.f : pow2(m - top), f1 = ml.x == -INFINITY ? 0.f : pow2(ml.x - top);
+        l = l * f0 + ml.y * f1;
+        o = fma4(f1, ok, rows4(o, f0));
+        m = top;
+      }
+      write_out<A>(a, p.seq, p.j, h, d, o, l);
+      if (d == 0) write_lse(a, p.seq, p.j, h, m, l);
+    }
   }
 }
 
@@ -326,59 +441,70 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 template <class T, class A>
 constexpr int terms_of() { return sizeof(A) == 2 ? 1 : (__is_same(T, __half) ? 2 : 3); }
 
-template <class T, class A, int DP, int NT>
-constexpr size_t mma_query_bytes() { return (size_t)(DP / 32) * terms_of<T, A>() * NT * 512; }
-
-// Ring stages of 16 positions, and CTAs per SM: about 190 KB of copies under way on each SM.
+// Ring stages of 16 positions, and CTAs per SM: 130 to 190 KB of copies under way on each SM.
 template <int DP>
-constexpr int mma_stages() { return DP == 64 ? 4 : 3; }
+constexpr int mma_stages() { return DP == 64 ? 4 : DP == 128 ? 3 : 2; }
 template <int DP>
 constexpr int mma_ctas() { return DP == 64 ? 3 : DP == 128 ? 2 : 1; }
 template <int DP>
 constexpr int mma_ring_bytes() { return mma_stages<DP>() * 16 * 2 * DP * 2; }  // of a warp
+// Operand words of the queries of a warp's segment: in registers where they are few.
+template <class T, class A, int DP, int NT>
+constexpr int mma_query_words() { return (DP / 32) * terms_of<T, A>() * NT; }  // uint4 of a lane
+template <class T, class A, int DP, int NT>
+constexpr bool mma_query_regs() { return mma_query_words<T, A, DP, NT>() <= 6; }
+template <class T, class A, int DP, int NT>
+constexpr int mma_query_bytes() { return mma_query_regs<T, A, DP, NT>() ? 0 : mma_query_words<T, A, DP, NT>() * 512; }  // of a warp
 
 template <class T, class A, int DP, int NT>
 __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(const AttnArgs a) {
   constexpr int C = DP / 32, V = DP / 64, S = mma_stages<DP>(), TERMS = terms_of<T, A>(), WT = TERMS == 1 ? 2 : TERMS;
   constexpr int PIECES = 2 * C + 4 * V;  // 16-byte pieces of a stage per lane
+  constexpr bool QREG = mma_query_regs<T, A, DP, NT>();
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float qscale[8 * NT];
-  __shared__ int bad;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = lane >> 2, quad = lane & 3;
+  __shared__ Part parts[2 * kAttnWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, quad = lane & 3;
   uint4* const ring = reinterpret_cast<uint4*>(smem + warp * mma_ring_bytes<DP>()) + lane;  // piece i of stage s: [(s PIECES + i) 32]
-  uint4* const qs = reinterpret_cast<uint4*>(smem + kAttnWarps * mma_ring_bytes<DP>());      // [C][TERMS][NT][32]: operand words
+  uint4* const qs = reinterpret_cast<uint4*>(smem + kAttnWarps * mma_ring_bytes<DP>() + warp * mma_query_bytes<T, A, DP, NT>()) + lane;
   Joint joint;
-  joint.o = reinterpret_cast<float*>(smem);
-  joint.ring = mma_ring_bytes<DP>() / 4;
-  joint.m = reinterpret_cast<float*>(qs + C * TERMS * NT * 32);
-  joint.l = joint.m + kAttnWarps * a.group_size;
+  joint.part = parts;
+  joint.ring = reinterpret_cast<float*>(smem);
+  joint.ring_floats = mma_ring_bytes<DP>() / 4;
+  joint.first = reinterpret_cast<float*>(smem + kAttnWarps * (mma_ring_bytes<DP>() + mma_query_bytes<T, A, DP, NT>()));
+  joint.m = joint.first + kAttnWarps * a.group_size * DP;
+  joint.l = joint.m + 2 * kAttnWarps * a.group_size;
   const T* const kp = static_cast<const T*>(a.k);
   const T* const vp = static_cast<const T*>(a.v);
 
-  Run run = find_run(a);
-  Segment g;
-  while (next_segment(a, run, g)) {
-    __syncthreads();  // the last segment's queries and join are done with
-    if (tid == 0) bad = 0;
-    __syncthreads();
-    // ---- this warp's stages: both halves of blocks b0 + warp, b0 + warp + 4, ...
-    const int mine = g.b1 - g.b0 > warp ? (g.b1 - g.b0 - warp - 1) / kAttnWarps + 1 : 0;
-    int n = 2 * mine;
-    if (n && (g.b0 + warp + (mine - 1) * kAttnWarps) * kBlock + 16 >= g.len) --n;  // the last half is past the length
-    int64_t off = row_offset(a, g, g.b0 + warp, lane, &bad);
-    int64_t off_next = row_offset(a, g, g.b0 + warp + kAttnWarps, lane, &bad);
+  const Run run = find_run(a);
+  if (lane == 0) parts[2 * warp].blocks = parts[2 * warp + 1].blocks = 0;
+  const int n = (int)run.n;  // blocks; two stages each
+  if (n) {
+    Place ahead = run.from, c = run.from;
+    uint32_t bad = 0;  // by segment, numbered along the run: this lane has met a page outside the pool
+    int ahead_ord = 0, ord = 0;
+    int64_t off = row_offset(a, ahead, lane, bad, ahead_ord), off_next = -1;
+    auto look = [&](int k) {  // the rows of block k of the run
+      if (k < n) {
+        const int j = ahead.j, seq = ahead.seq;
+        ahead.next(a);
+        ahead_ord += ahead.j != j || ahead.seq != seq;
+        off_next = row_offset(a, ahead, lane, bad, ahead_ord);
+      }
+    };
+    look(1);
     auto issue = [&](int i) {
-      if (i < n) {
+      if (i < 2 * n) {
         uint4* const to = ring + (i % S) * PIECES * 32;
         const int half = (i & 1) * 16;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {  // key rows row, row + 8
           const int64_t at = __shfl_sync(0xffffffffu, off, half + row + 8 * e);
 #pragma unroll
-          for (int c = 0; c < C; ++c) {
-            const int d = c * 32 + quad * 8;
+          for (int x = 0; x < C; ++x) {
+            const int d = x * 32 + quad * 8;
             const bool ok = at >= 0 && d < a.dim;
-            copy16(to + (2 * c + e) * 32, kp + (ok ? at + d : 0), ok);
+            copy16(to + (2 * x + e) * 32, kp + (ok ? at + d : 0), ok);
           }
         }
 #pragma unroll
@@ -393,192 +519,254 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
         }
         if (i & 1) {
           off = off_next;
-          off_next = row_offset(a, g, g.b0 + warp + ((i >> 1) + 2) * kAttnWarps, lane, &bad);
+          look((i >> 1) + 2);
         }
       }
       copies_commit();
     };
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) issue(i);
-    // ---- the group's queries as operand words, every head's rows of 8 * NT columns (0 past the group)
-    const A* const q = static_cast<const A*>(a.q) + g.seq * a.q_stride + (int64_t)g.head0 * a.dim;
-    if constexpr (TERMS == 2) {  // f32 queries as f16 terms: scaled to at most 1
-      for (int h = warp; h < 8 * NT; h += kAttnWarps) {
-        float m = 0.f;
-        for (int d = lane; h < g.heads && d < a.dim; d += 32) m = fmaxf(m, fabsf(to_f32(q[h * a.dim + d])));
-        m = warp_max(m);
-        int e = 0;
-        if (m > 0.f && m < INFINITY) (void)frexpf(m, &e);
-        if (lane == 0) qscale[h] = ldexpf(1.f, max(min(e, 126), -126));
-      }
-      __syncthreads();
-    }
-    for (int i = tid; i < C * NT * 32; i += kAttnThreads) {
-      const int l = i & 31, nt = (i >> 5) % NT, c = (i >> 5) / NT;
-      const int h = nt * 8 + (l >> 2), d = c * 32 + (l & 3) * 8;
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = h < g.heads && d < a.dim ? to_f32(q[h * a.dim + d + e]) : 0.f;
-      if constexpr (TERMS == 2) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] /= qscale[h];
-      }
-      uint32_t w[4][TERMS];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) split2<T, TERMS>(x[2 * e], x[2 * e + 1], w[e]);
-#pragma unroll
-      for (int s = 0; s < TERMS; ++s) qs[((c * TERMS + s) * NT + nt) * 32 + l] = make_uint4(w[0][s], w[1][s], w[2][s], w[3][s]);
-    }
-    __syncthreads();
-    float sc[NT][2];  // score factors of this lane's two columns, for base-2 exponents
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        sc[nt][e] = a.scale * kLog2e;
-        if constexpr (TERMS == 2) sc[nt][e] = a.scale * qscale[nt * 8 + quad * 2 + e] * kLog2e;
-      }
 
+    uint4 qr[QREG ? C : 1][QREG ? TERMS : 1][QREG ? NT : 1] = {};
+    auto query = [&](int x, int t, int nt) -> uint4 {
+      if constexpr (QREG)
+        return qr[x][t][nt];
+      else
+        return qs[((x * TERMS + t) * NT + nt) * 32];
+    };
+    float sc[NT][2];  // score factors of this lane's two heads, for base-2 exponents
     float m[NT][2], l[NT][2], o[V][4][NT][4];
+    int b0 = 0;
+    for (int k = 0; k < n; ++k) {
+      if (k == 0 || c.b == 0) {  // a segment begins: its queries, every head's row of 8 * NT (0 past the group)
+        b0 = c.b;
+        const int heads = heads_of(a, c.j);
+        const A* const q = static_cast<const A*>(a.q) + c.seq * a.q_stride + (int64_t)first_head(a, c.j) * a.dim;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+          const int h = nt * 8 + row;
+          if constexpr (TERMS == 1) {
 #pragma unroll
-      for (int v = 0; v < V; ++v)
+            for (int x = 0; x < C; ++x) {
+              const int d = x * 32 + quad * 8;
+              uint4 w = make_uint4(0u, 0u, 0u, 0u);
+              if (h < heads && d < a.dim) w = __ldg(reinterpret_cast<const uint4*>(q + h * a.dim + d));
+              if constexpr (QREG)
+                qr[x][0][nt] = w;
+              else
+                qs[(x * NT + nt) * 32] = w;
+            }
+            sc[nt][0] = sc[nt][1] = a.scale * kLog2e;
+          } else {
+            float f[C][8], top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int x = 0; x < C; ++x) {
+              const int d = x * 32 + quad * 8;
+              float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+              if (h < heads && d < a.dim) {
+                u = __ldg(reinterpret_cast<const float4*>(q + h * a.dim + d));
+                v = __ldg(reinterpret_cast<const float4*>(q + h * a.dim + d) + 1);
+              }
+              f[x][0] = u.x, f[x][1] = u.y, f[x][2] = u.z, f[x][3] = u.w;
+              f[x][4] = v.x, f[x][5] = v.y, f[x][6] = v.z, f[x][7] = v.w;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[v][i][nt][e] = 0.f;
-    }
-    for (int i = 0; i < n; ++i) {
-      copies_wait<S - 2>();
-      issue(i + S - 1);  // into the stage that the last round read
-      const uint4* const st = ring + (i % S) * PIECES * 32;
-      const int p0 = (g.b0 + warp + (i >> 1) * kAttnWarps) * kBlock + (i & 1) * 16 + row;
-      // ---- scores: 16 positions x heads
-      float s[NT][4];
+              for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[x][e]));
+            }
+            float up = 1.f, down = 1.f;
+            if constexpr (TERMS == 2) {  // f16 terms: scaled to at most 1
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+              int e = 0;
+              if (top > 0.f && top < INFINITY) (void)frexpf(top, &e);
+              e = max(min(e, 126), -126);
+              up = ldexpf(1.f, e);
+              down = ldexpf(1.f, -e);
+            }
+            sc[nt][0] = a.scale * __shfl_sync(0xffffffffu, up, quad * 8) * kLog2e;
+            sc[nt][1] = a.scale * __shfl_sync(0xffffffffu, up, quad * 8 + 4) * kLog2e;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+            for (int x = 0; x < C; ++x) {
+              uint32_t w[4][TERMS];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-      auto score = [&](float (&f)[4], const uint4& k0, const uint4& k1, const uint4& b) {
-        mma<T>(f, k0.x, k1.x, k0.y, k1.y, b.x, b.y);
-        mma<T>(f, k0.z, k1.z, k0.w, k1.w, b.z, b.w);
-      };
+              for (int e = 0; e < 4; ++e) split2<T, TERMS>(f[x][2 * e] * down, f[x][2 * e + 1] * down, w[e]);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const uint4 k0 = st[(2 * c) * 32], k1 = st[(2 * c + 1) * 32];
-#pragma unroll
-        for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) score(s[nt], k0, k1, qs[((c * TERMS + t) * NT + nt) * 32 + lane]);
-      }
-      if constexpr (TERMS > 1) {
-        // A key of +-inf times a later term of a query (of any sign, or 0) is NaN: there the first
-        // term alone gives the score that f32 products would.
-        bool odd = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= s[nt][e] != s[nt][e];
-        if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float f[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < C; ++c) score(f, st[(2 * c) * 32], st[(2 * c + 1) * 32], qs[(c * TERMS * NT + nt) * 32 + lane]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (s[nt][e] != s[nt][e]) s[nt][e] = f[e];
+              for (int t = 0; t < TERMS; ++t) {
+                const uint4 v = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
+                if constexpr (QREG)
+                  qr[x][t][nt] = v;
+                else
+                  qs[((x * TERMS + t) * NT + nt) * 32] = v;
+              }
+            }
           }
-        }
-      }
-      // ---- running maximum and sum of this lane's two heads, weights as the second operand
-      uint32_t p[NT][WT][2];
-      float keep[NT][2];
-      bool moved = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x0 = p0 < g.len ? s[nt][e] * sc[nt][e] : -INFINITY;
-          float x1 = p0 + 8 < g.len ? s[nt][2 + e] * sc[nt][e] : -INFINITY;
-          float top = fmaxf(m[nt][e], fmaxf(x0, x1));
-#pragma unroll
-          for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
-          moved |= top != m[nt][e];
-          const float base = top == -INFINITY ? 0.f : top;
-          keep[nt][e] = pow2(m[nt][e] - base);  // 0 while there was nothing
-          m[nt][e] = top;
-          x0 = pow2(x0 - base);
-          x1 = pow2(x1 - base);
-          l[nt][e] = fmaf(l[nt][e], keep[nt][e], x0 + x1);
-          s[nt][e] = x0;
-          s[nt][2 + e] = x1;
-        }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t w[WT];
-          split2<T, WT>(s[nt][2 * k], s[nt][2 * k + 1], w);
-#pragma unroll
-          for (int t = 0; t < WT; ++t) p[nt][t][k] = transpose8x8(w[t]);
-        }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[v][k][nt][e] *= keep[nt][e & 1];
-      }
-      // ---- output: head_dim x heads, the value rows woven in pairs of positions
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        uint4 x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = st[(2 * C + 4 * v + e) * 32];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t a0 = __byte_perm(word(x[0], k), word(x[1], k), 0x5410), a1 = __byte_perm(word(x[0], k), word(x[1], k), 0x7632);
-          const uint32_t a2 = __byte_perm(word(x[2], k), word(x[3], k), 0x5410), a3 = __byte_perm(word(x[2], k), word(x[3], k), 0x7632);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int t = 0; t < WT; ++t) mma<T>(o[v][k][nt], a0, a1, a2, a3, p[nt][t][0], p[nt][t][1]);
-        }
-      }
-    }
-    copies_wait<0>();
-    // ---- leave (m, l, o) for the join
-    float* const jo = joint.o + warp * joint.ring;
-    __syncwarp();  // every lane has read the ring
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int b = 4; b < 32; b <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], b);
-        const int h = nt * 8 + quad * 2 + e;
-        if (h < g.heads) {
-          if (row == 0) {
-            joint.m[warp * a.group_size + h] = m[nt][e];
-            joint.l[warp * a.group_size + h] = l[nt][e];
-          }
+          m[nt][0] = m[nt][1] = -INFINITY;
+          l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
           for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<float2*>(jo + h * DP + v * 64 + row * 8 + 2 * k) = make_float2(o[v][k][nt][e], o[v][k][nt][2 + e]);
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[v][x][nt][e] = 0.f;
         }
       }
-    __syncthreads();
-    finish<A, DP>(a, run, g, joint, bad);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int i = 2 * k + half;
+        copies_wait<S - 2>();
+        issue(i + S - 1);  // into the stage that the last round read
+        if (c.b * kBlock + half * 16 >= c.len) continue;
+        const uint4* const st = ring + (i % S) * PIECES * 32;
+        const int p0 = c.b * kBlock + half * 16 + row;
+        // ---- scores: 16 positions x heads
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+        auto score = [&](float (&f)[4], const uint4& k0, const uint4& k1, const uint4& b) {
+          mma<T>(f, k0.x, k1.x, k0.y, k1.y, b.x, b.y);
+          mma<T>(f, k0.z, k1.z, k0.w, k1.w, b.z, b.w);
+        };
+#pragma unroll
+        for (int x = 0; x < C; ++x) {
+          const uint4 k0 = st[(2 * x) * 32], k1 = st[(2 * x + 1) * 32];
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) score(s[nt], k0, k1, query(x, t, nt));
+        }
+        if constexpr (TERMS > 1) {
+          // A key of +-inf times a later term of a query (of any sign, or 0) is NaN: there the first
+          // term alone gives the score that f32 products would.
+          bool odd = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= s[nt][e] != s[nt][e];
+          if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int x = 0; x < C; ++x) score(f, st[(2 * x) * 32], st[(2 * x + 1) * 32], query(x, 0, nt));
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (s[nt][e] != s[nt][e]) s[nt][e] = f[e];
+            }
+          }
+        }
+        // ---- running maximum and sum of this lane's two heads, weights as the second operand
+        uint32_t p[NT][WT][2];
+        float keep[NT][2];
+        bool moved = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x0 = p0 < c.len ? s[nt][e] * sc[nt][e] : -INFINITY;
+            float x1 = p0 + 8 < c.len ? s[nt][2 + e] * sc[nt][e] : -INFINITY;
+            float top = fmaxf(m[nt][e], fmaxf(x0, x1));
+#pragma unroll
+            for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+            moved |= top != m[nt][e];
+            const float base = top == -INFINITY ? 0.f : top;
+            keep[nt][e] = pow2(m[nt][e] - base);  // 0 while there was nothing
+            m[nt][e] = top;
+            x0 = pow2(x0 - base);
+            x1 = pow2(x1 - base);
+            l[nt][e] = fmaf(l[nt][e], keep[nt][e], x0 + x1);
+            s[nt][e] = x0;
+            s[nt][2 + e] = x1;
+          }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t w[WT];
+            split2<T, WT>(s[nt][2 * x], s[nt][2 * x + 1], w);
+#pragma unroll
+            for (int t = 0; t < WT; ++t) p[nt][t][x] = transpose8x8(w[t]);
+          }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[v][x][nt][e] *= keep[nt][e & 1];
+        }
+        // ---- output: head_dim x heads, the value rows woven in pairs of positions
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          uint4 x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = st[(2 * C + 4 * v + e) * 32];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint32_t a0 = __byte_perm(word(x[0], y), word(x[1], y), 0x5410), a1 = __byte_perm(word(x[0], y), word(x[1], y), 0x7632);
+            const uint32_t a2 = __byte_perm(word(x[2], y), word(x[3], y), 0x5410), a3 = __byte_perm(word(x[2], y), word(x[3], y), 0x7632);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int t = 0; t < WT; ++t) mma<T>(o[v][y][nt], a0, a1, a2, a3, p[nt][t][0], p[nt][t][1]);
+          }
+        }
+      }
+      const bool ends = c.b + 1 == c.nb;
+      if (ends || k + 1 == n) {  // all that this run has of the segment
+        const bool done = ends && b0 == 0;
+        const int slot = k + 1 - (c.b + 1 - b0) == 0 ? 0 : 1;
+        const int heads = heads_of(a, c.j);
+        const bool nan = __any_sync(0xffffffffu, bad >> (ord & 31) & 1u);
+        bad &= ~(1u << (ord & 31));
+        if (slot == 1 && !done) {  // the run's end: the ring is free
+          copies_wait<0>();
+          __syncwarp();
+        }
+        float* const jo = joint.o<DP>(a, warp, slot);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float sum = l[nt][e];
+#pragma unroll
+            for (int b = 4; b < 32; b <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, b);
+            if (nan) sum = __int_as_float(0x7FC00000);
+            const int h = nt * 8 + quad * 2 + e;
+            if (h >= heads) continue;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+              const int d = v * 64 + row * 8;
+              if (d >= a.dim) continue;
+              const float4 lo = make_float4(o[v][0][nt][e], o[v][0][nt][2 + e], o[v][1][nt][e], o[v][1][nt][2 + e]);
+              const float4 hi = make_float4(o[v][2][nt][e], o[v][2][nt][2 + e], o[v][3][nt][e], o[v][3][nt][2 + e]);
+              if (done) {
+                write_out<A>(a, c.seq, c.j, h, d, lo, sum);
+                write_out<A>(a, c.seq, c.j, h, d + 4, hi, sum);
+              } else {
+                *reinterpret_cast<float4*>(jo + h * DP + d) = lo;
+                *reinterpret_cast<float4*>(jo + h * DP + d + 4) = hi;
+              }
+            }
+            if (row == 0) {
+              if (done) {
+                write_lse(a, c.seq, c.j, h, m[nt][e], sum);
+              } else {
+                joint.m[(2 * warp + slot) * a.group_size + h] = m[nt][e];
+                joint.l[(2 * warp + slot) * a.group_size + h] = sum;
+              }
+            }
+          }
+        if (!done && lane == 0) parts[2 * warp + slot] = Part{c.seq, c.j, b0, c.b + 1 - b0, c.nb};
+        ++ord;
+      }
+      if (k + 1 < n) c.next(a);
+    }
+    copies_wait<0>();
   }
+  join<A, DP>(a, run, joint);
   finish_empty<A>(a);
 }
 
@@ -597,7 +785,7 @@ constexpr int f32_ctas() { return DP == 64 ? 2 : 1; }
 template <int DP>
 constexpr int f32_ring_bytes() { return f32_stages<DP>() * 8 * f32_rows<DP>() * 2 * DP * 4; }  // of a warp
 template <int DP, int G>
-constexpr size_t f32_query_bytes() { return (size_t)G * DP * 4 + (size_t)kAttnWarps * 8 * f32_rows<DP>() * G * 4; }
+constexpr int f32_query_bytes() { return G * DP * 4 + 8 * f32_rows<DP>() * G * 4; }  // of a warp: queries and weights
 
 template <int DP, int G>
 __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(const AttnArgs a) {
@@ -605,43 +793,51 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
   constexpr int C = DP / 16, PER = DP / 4 < 32 ? DP / 4 : 32, ROWS = 32 / PER, V = DP / 4 / PER;
   constexpr int PIECES = R * C + P / ROWS * V;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int bad;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = lane >> 2, quad = lane & 3;
+  __shared__ Part parts[2 * kAttnWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, quad = lane & 3;
   uint4* const ring = reinterpret_cast<uint4*>(smem + warp * f32_ring_bytes<DP>()) + lane;
-  float* const qs = reinterpret_cast<float*>(smem + kAttnWarps * f32_ring_bytes<DP>());  // [G][DP]
-  float* const pw = qs + G * DP + warp * P * G;                                            // [position][G]
+  float* const qs = reinterpret_cast<float*>(smem + kAttnWarps * f32_ring_bytes<DP>() + warp * f32_query_bytes<DP, G>());  // [G][DP]
+  float* const pw = qs + G * DP;                                                                                            // [position][G]
   Joint joint;
-  joint.o = reinterpret_cast<float*>(smem);
-  joint.ring = f32_ring_bytes<DP>() / 4;
-  joint.m = qs + G * DP + kAttnWarps * P * G;
-  joint.l = joint.m + kAttnWarps * a.group_size;
+  joint.part = parts;
+  joint.ring = reinterpret_cast<float*>(smem);
+  joint.ring_floats = f32_ring_bytes<DP>() / 4;
+  joint.first = reinterpret_cast<float*>(smem + kAttnWarps * (f32_ring_bytes<DP>() + f32_query_bytes<DP, G>()));
+  joint.m = joint.first + kAttnWarps * a.group_size * DP;
+  joint.l = joint.m + 2 * kAttnWarps * a.group_size;
   const float* const kp = static_cast<const float*>(a.k);
   const float* const vp = static_cast<const float*>(a.v);
   const float sc = a.scale * kLog2e;
 
-  Run run = find_run(a);
-  Segment g;
-  while (next_segment(a, run, g)) {
-    __syncthreads();
-    if (tid == 0) bad = 0;
-    __syncthreads();
-    const int mine = g.b1 - g.b0 > warp ? (g.b1 - g.b0 - warp - 1) / kAttnWarps + 1 : 0;
-    int n = PARTS * mine;
-    while (n && (g.b0 + warp + (mine - 1) * kAttnWarps) * kBlock + ((n - 1) % PARTS) * P >= g.len) --n;
-    int64_t off = row_offset(a, g, g.b0 + warp, lane, &bad);
-    int64_t off_next = row_offset(a, g, g.b0 + warp + kAttnWarps, lane, &bad);
+  const Run run = find_run(a);
+  if (lane == 0) parts[2 * warp].blocks = parts[2 * warp + 1].blocks = 0;
+  const int n = (int)run.n;  // blocks
+  if (n) {
+    Place ahead = run.from, c = run.from;
+    uint32_t bad = 0;
+    int ahead_ord = 0, ord = 0;
+    int64_t off = row_offset(a, ahead, lane, bad, ahead_ord), off_next = -1;
+    auto look = [&](int k) {
+      if (k < n) {
+        const int j = ahead.j, seq = ahead.seq;
+        ahead.next(a);
+        ahead_ord += ahead.j != j || ahead.seq != seq;
+        off_next = row_offset(a, ahead, lane, bad, ahead_ord);
+      }
+    };
+    look(1);
     auto issue = [&](int i) {
-      if (i < n) {
+      if (i < PARTS * n) {
         uint4* const to = ring + (i % S) * PIECES * 32;
         const int part = (i % PARTS) * P;
 #pragma unroll
-        for (int e = 0; e < R; ++e) {
+        for (int e = 0; e < R; ++e) {  // key rows row, row + 8, ...
           const int64_t at = __shfl_sync(0xffffffffu, off, part + row + 8 * e);
 #pragma unroll
-          for (int c = 0; c < C; ++c) {
-            const int d = c * 16 + quad * 4;
+          for (int x = 0; x < C; ++x) {
+            const int d = x * 16 + quad * 4;
             const bool ok = at >= 0 && d < a.dim;
-            copy16(to + (c * R + e) * 32, kp + (ok ? at + d : 0), ok);
+            copy16(to + (x * R + e) * 32, kp + (ok ? at + d : 0), ok);
           }
         }
 #pragma unroll
@@ -656,136 +852,172 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
         }
         if (i % PARTS == PARTS - 1) {
           off = off_next;
-          off_next = row_offset(a, g, g.b0 + warp + (i / PARTS + 2) * kAttnWarps, lane, &bad);
+          look(i / PARTS + 2);
         }
       }
       copies_commit();
     };
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) issue(i);
-    const float* const q = static_cast<const float*>(a.q) + g.seq * a.q_stride + (int64_t)g.head0 * a.dim;
-    for (int i = tid; i < G * DP; i += kAttnThreads) {
-      const int h = i / DP, d = i - h * DP;
-      qs[i] = h < g.heads && d < a.dim ? q[h * a.dim + d] : 0.f;
-    }
-    __syncthreads();
     float m[G], l[G];  // of every head: m the same on every lane, l of this lane's positions
     float o[V][G][4];
+    int b0 = 0;
+    for (int k = 0; k < n; ++k) {
+      if (k == 0 || c.b == 0) {
+        b0 = c.b;
+        const int heads = heads_of(a, c.j);
+        const float* const q = static_cast<const float*>(a.q) + c.seq * a.q_stride + (int64_t)first_head(a, c.j) * a.dim;
+        __syncwarp();  // the last segment's queries are read
 #pragma unroll
-    for (int h = 0; h < G; ++h) {
-      m[h] = -INFINITY;
-      l[h] = 0.f;
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[v][h][e] = 0.f;
-    }
-    for (int i = 0; i < n; ++i) {
-      copies_wait<S - 2>();
-      issue(i + S - 1);
-      const float4* const st = reinterpret_cast<const float4*>(ring + (i % S) * PIECES * 32);
-      const int p0 = (g.b0 + warp + (i / PARTS) * kAttnWarps) * kBlock + (i % PARTS) * P + row;
-      // ---- scores of rows row, row + 8, ...
-      float s[R][G];
-#pragma unroll
-      for (int e = 0; e < R; ++e)
-#pragma unroll
-        for (int h = 0; h < G; ++h) s[e][h] = 0.f;
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        float4 k[R];
-#pragma unroll
-        for (int e = 0; e < R; ++e) k[e] = st[(c * R + e) * 32];
+        for (int x = 0; x < G * DP / 128; ++x) {
+          const int e = (x * 32 + lane) * 4, h = e / DP, d = e % DP;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (h < heads && d < a.dim) v = __ldg(reinterpret_cast<const float4*>(q + h * a.dim + d));
+          *reinterpret_cast<float4*>(qs + e) = v;
+        }
+        __syncwarp();
 #pragma unroll
         for (int h = 0; h < G; ++h) {
-          const float4 x = *reinterpret_cast<const float4*>(qs + h * DP + c * 16 + quad * 4);
+          m[h] = -INFINITY;
+          l[h] = 0.f;
 #pragma unroll
-          for (int e = 0; e < R; ++e)
-            s[e][h] = fmaf(k[e].x, x.x, fmaf(k[e].y, x.y, fmaf(k[e].z, x.z, fmaf(k[e].w, x.w, s[e][h]))));
+          for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[v][h][e] = 0.f;
         }
       }
-      bool moved = false;
-      float keep[G];
-      __syncwarp();  // the last round's weights are read
+#pragma unroll 1
+      for (int part = 0; part < PARTS; ++part) {
+        const int i = PARTS * k + part;
+        copies_wait<S - 2>();
+        issue(i + S - 1);
+        if (c.b * kBlock + part * P >= c.len) continue;
+        const float4* const st = reinterpret_cast<const float4*>(ring + (i % S) * PIECES * 32);
+        const int p0 = c.b * kBlock + part * P + row;
+        // ---- scores of rows row, row + 8, ...
+        float s[R][G];
 #pragma unroll
-      for (int h = 0; h < G; ++h) {
-        float top = m[h];
+        for (int e = 0; e < R; ++e)
 #pragma unroll
-        for (int e = 0; e < R; ++e) {
-          float x = s[e][h];
-          x += __shfl_xor_sync(0xffffffffu, x, 1);
-          x += __shfl_xor_sync(0xffffffffu, x, 2);
-          s[e][h] = p0 + 8 * e < g.len ? x * sc : -INFINITY;
-          top = fmaxf(top, s[e][h]);
-        }
+          for (int h = 0; h < G; ++h) s[e][h] = 0.f;
 #pragma unroll
-        for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
-        moved |= top != m[h];
-        const float base = top == -INFINITY ? 0.f : top;
-        keep[h] = pow2(m[h] - base);
-        m[h] = top;
-        l[h] *= keep[h];
-        if (quad < R) {  // lane e of a row's four holds the weight of row + 8 e
-          const float w = pow2((R == 1 || quad == 0 ? s[0][h] : s[R - 1][h]) - base);
-          l[h] += w;
-          pw[(row + 8 * quad) * G + h] = w;
-        }
-      }
-      __syncwarp();
-      if (moved) {  // the maxima are the same on every lane
+        for (int x = 0; x < C; ++x) {
+          float4 key[R];
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-          for (int h = 0; h < G; ++h)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[v][h][e] *= keep[h];
-      }
-      // ---- output: ROWS value rows at a time
-#pragma unroll
-      for (int p = 0; p < P / ROWS; ++p) {
-        float w[G];
-#pragma unroll
-        for (int h = 0; h < G; h += 4)
-          *reinterpret_cast<float4*>(w + h) = *reinterpret_cast<const float4*>(pw + (p * ROWS + lane / PER) * G + h);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float4 x = st[(R * C + p * V + v) * 32];
+          for (int e = 0; e < R; ++e) key[e] = st[(x * R + e) * 32];
 #pragma unroll
           for (int h = 0; h < G; ++h) {
-            o[v][h][0] = fmaf(w[h], x.x, o[v][h][0]);
-            o[v][h][1] = fmaf(w[h], x.y, o[v][h][1]);
-            o[v][h][2] = fmaf(w[h], x.z, o[v][h][2]);
-            o[v][h][3] = fmaf(w[h], x.w, o[v][h][3]);
+            const float4 q = *reinterpret_cast<const float4*>(qs + h * DP + x * 16 + quad * 4);
+#pragma unroll
+            for (int e = 0; e < R; ++e)
+              s[e][h] = fmaf(key[e].x, q.x, fmaf(key[e].y, q.y, fmaf(key[e].z, q.z, fmaf(key[e].w, q.w, s[e][h]))));
+          }
+        }
+        bool moved = false;
+        float keep[G];
+        __syncwarp();  // the last round's weights are read
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          float top = m[h];
+#pragma unroll
+          for (int e = 0; e < R; ++e) {
+            float x = s[e][h];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+            s[e][h] = p0 + 8 * e < c.len ? x * sc : -INFINITY;
+            top = fmaxf(top, s[e][h]);
+          }
+#pragma unroll
+          for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+          moved |= top != m[h];
+          const float base = top == -INFINITY ? 0.f : top;
+          keep[h] = pow2(m[h] - base);
+          m[h] = top;
+          l[h] *= keep[h];
+          if (quad < R) {  // lane e of a row's four holds the weight of row + 8 e
+            const float w = pow2((R == 1 || quad == 0 ? s[0][h] : s[R - 1][h]) - base);
+            l[h] += w;
+            pw[(row + 8 * quad) * G + h] = w;
+          }
+        }
+        __syncwarp();
+        if (moved) {  // the maxima are the same on every lane
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int h = 0; h < G; ++h)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[v][h][e] *= keep[h];
+        }
+        // ---- output: ROWS value rows at a time
+#pragma unroll
+        for (int p = 0; p < P / ROWS; ++p) {
+          float w[G];
+#pragma unroll
+          for (int h = 0; h < G; h += 4)
+            *reinterpret_cast<float4*>(w + h) = *reinterpret_cast<const float4*>(pw + (p * ROWS + lane / PER) * G + h);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float4 x = st[(R * C + p * V + v) * 32];
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+              o[v][h][0] = fmaf(w[h], x.x, o[v][h][0]);
+              o[v][h][1] = fmaf(w[h], x.y, o[v][h][1]);
+              o[v][h][2] = fmaf(w[h], x.z, o[v][h][2]);
+              o[v][h][3] = fmaf(w[h], x.w, o[v][h][3]);
+            }
           }
         }
       }
+      const bool ends = c.b + 1 == c.nb;
+      if (ends || k + 1 == n) {  // all that this run has of the segment
+        const bool done = ends && b0 == 0;
+        const int slot = k + 1 - (c.b + 1 - b0) == 0 ? 0 : 1;
+        const int heads = heads_of(a, c.j);
+        const bool nan = __any_sync(0xffffffffu, bad >> (ord & 31) & 1u);
+        bad &= ~(1u << (ord & 31));
+        if (slot == 1 && !done) {  // the run's end: the ring is free
+          copies_wait<0>();
+          __syncwarp();
+        }
+        float* const jo = joint.o<DP>(a, warp, slot);
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          float sum = warp_sum(l[h]);
+          if (nan) sum = __int_as_float(0x7FC00000);
+          if (h >= heads) continue;
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+              for (int b = PER; b < 32; b <<= 1) o[v][h][e] += __shfl_xor_sync(0xffffffffu, o[v][h][e], b);
+            }
+            const int d = (v * PER + lane) * 4;
+            if (lane >= PER || d >= a.dim) continue;
+            const float4 x = make_float4(o[v][h][0], o[v][h][1], o[v][h][2], o[v][h][3]);
+            if (done)
+              write_out<float>(a, c.seq, c.j, h, d, x, sum);
+            else
+              *reinterpret_cast<float4*>(jo + h * DP + d) = x;
+          }
+          if (lane == 0) {
+            if (done) {
+              write_lse(a, c.seq, c.j, h, m[h], sum);
+            } else {
+              joint.m[(2 * warp + slot) * a.group_size + h] = m[h];
+              joint.l[(2 * warp + slot) * a.group_size + h] = sum;
+            }
+          }
+        }
+        if (!done && lane == 0) parts[2 * warp + slot] = Part{c.seq, c.j, b0, c.b + 1 - b0, c.nb};
+        ++ord;
+      }
+      if (k + 1 < n) c.next(a);
     }
     copies_wait<0>();
-    float* const jo = joint.o + warp * joint.ring;
-    __syncwarp();  // every lane has read the ring
-#pragma unroll
-    for (int h = 0; h < G; ++h) {
-      l[h] = warp_sum(l[h]);
-      if (h < g.heads) {
-        if (lane == 0) {
-          joint.m[warp * a.group_size + h] = m[h];
-          joint.l[warp * a.group_size + h] = l[h];
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-#pragma unroll
-            for (int b = PER; b < 32; b <<= 1) o[v][h][e] += __shfl_xor_sync(0xffffffffu, o[v][h][e], b);
-          }
-          if (lane < PER)
-            *reinterpret_cast<float4*>(jo + h * DP + (v * PER + lane) * 4) = make_float4(o[v][h][0], o[v][h][1], o[v][h][2], o[v][h][3]);
-        }
-      }
-    }
-    __syncthreads();
-    finish<float, DP>(a, run, g, joint, bad);
   }
+  join<float, DP>(a, run, joint);
   finish_empty<float>(a);
 }
 
@@ -804,13 +1036,15 @@ bool allow_smem(int dev, size_t smem) {
   return true;
 }
 
+// `smem`: what the warps need; the parts of the join come on top.
 template <auto KERNEL>
-int launch(const AttnArgs& a, int per_sm, size_t smem, cudaStream_t st) {
+int launch(const AttnArgs& a, int dp, int per_sm, size_t smem, cudaStream_t st) {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: no current CUDA device");
-  smem += (size_t)2 * kAttnWarps * a.group_size * 4;  // m and l of the join
+  smem += (size_t)kAttnWarps * a.group_size * (dp + 4) * 4;
   if (!allow_smem<KERNEL>(dev, smem)) return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: not enough shared memory");
+  per_sm = std::min(per_sm, (int)(228 * 1024 / (smem + 1024 + 512)));
   // no more CTAs than runs of the shortest length over the whole table
   const int64_t blocks = ((int64_t)a.table_stride * a.page_len + kBlock - 1) / kBlock;
   const int64_t most = (blocks + kMinBlocks - 1) / kMinBlocks * a.n_seq * a.n_kv * a.groups;
@@ -821,20 +1055,20 @@ int launch(const AttnArgs& a, int per_sm, size_t smem, cudaStream_t st) {
 
 template <class T, class A, int DP, int NT>
 int launch_mma(const AttnArgs& a, cudaStream_t st) {
-  return launch<attn_mma_kernel<T, A, DP, NT>>(a, mma_ctas<DP>(), kAttnWarps * mma_ring_bytes<DP>() + mma_query_bytes<T, A, DP, NT>(), st);
+  return launch<attn_mma_kernel<T, A, DP, NT>>(a, DP, mma_ctas<DP>(), kAttnWarps * (mma_ring_bytes<DP>() + mma_query_bytes<T, A, DP, NT>()), st);
 }
 template <class T, class A>
 int run_mma(AttnArgs& a, cudaStream_t st) {
-  a.group_size = std::min(a.rep, kMaxGroup);
+  a.group_size = std::min(a.rep, a.dim <= 128 ? kMaxGroup : 8);
   a.groups = (a.rep + a.group_size - 1) / a.group_size;
   const bool one = a.group_size <= 8;
   if (a.dim <= 64) return one ? launch_mma<T, A, 64, 1>(a, st) : launch_mma<T, A, 64, 2>(a, st);
   if (a.dim <= 128) return one ? launch_mma<T, A, 128, 1>(a, st) : launch_mma<T, A, 128, 2>(a, st);
-  return one ? launch_mma<T, A, 256, 1>(a, st) : launch_mma<T, A, 256, 2>(a, st);
+  return launch_mma<T, A, 256, 1>(a, st);
 }
 template <int DP, int G>
 int launch_f32(const AttnArgs& a, cudaStream_t st) {
-  return launch<attn_f32_kernel<DP, G>>(a, f32_ctas<DP>(), kAttnWarps * f32_ring_bytes<DP>() + f32_query_bytes<DP, G>(), st);
+  return launch<attn_f32_kernel<DP, G>>(a, DP, f32_ctas<DP>(), kAttnWarps * (f32_ring_bytes<DP>() + f32_query_bytes<DP, G>()), st);
 }
 int run_f32(AttnArgs& a, cudaStream_t st) {
   a.group_size = std::min(a.rep, 8);
@@ -851,7 +1085,7 @@ int run_f32(AttnArgs& a, cudaStream_t st) {
 extern "C" size_t mllm_paged_attn_workspace(int n_seq, int n_heads, int head_dim) {
   using namespace mllm;
   if (n_seq < 1 || n_heads < 1 || head_dim < 8 || head_dim > 256) return 0;
-  return counter_bytes(n_seq, n_heads) + (size_t)kMaxCtas * 2 * std::min(n_heads, kMaxGroup) * (head_dim + 2) * 4;
+  return counter_bytes(n_seq, n_heads) + (size_t)kMaxCtas * 2 * std::min(n_heads, kMaxGroup) * (head_dim + 4) * 4;
 }
 
 extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d_q, int64_t q_stride, int n_seq,
