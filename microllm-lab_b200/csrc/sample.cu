@@ -11,11 +11,13 @@
 //
 // A row is read once, into the shared memory of one CTA, or of a cluster's CTAs, each of which has a
 // contiguous part, where rows are fewer than SMs or do not fit.  The edge is found without sorting the row:
-//   - top_k up to 512: the k-th largest of the threads' own maxima bounds the k-th token from below, so the
-//     few tokens at or above it are gathered, and everything else happens in that list;
-//   - otherwise by a histogram of tokens or weight over x in two levels of 512 steps (of 1/16, then 1/8192
-//     of a unit of (x - m) r), then among the tokens of one step;
-//   - and by halving, one pass per bit, where a list would not fit (thousands of tokens of one value).
+//   - top_k up to 512: the step of 1/16 of a unit of (x - m) r in which the k-th largest of the threads' own
+//     maxima lies bounds the k-th token from below, so the few tokens down to that step are gathered, and
+//     everything else happens in that list;
+//   - otherwise by a histogram of tokens or weight over 512 such steps, then among the tokens of one step,
+//     or of a 512th of it where they are too many for a list;
+//   - and by halving, one pass per bit, where those are too many as well (thousands of tokens of one value).
+// A list is sorted and summed by one warp when it is short, by the CTA otherwise.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -32,38 +34,22 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleList = 2048;   // tokens of a list
+constexpr int kWarpList = 128;      // tokens of a list that one warp handles
 constexpr int kSampleMaxK = 512;    // top_k that starts from the threads' maxima
-constexpr int kSampleSteps = 512;   // steps of a histogram level
+constexpr int kSteps = 512;         // steps of a histogram level
 constexpr int kMaxCluster = 16;
 constexpr float kOne = 1099511627776.f;  // 2^40
-constexpr uint32_t kKeyNone = 0x007FFFFFu;  // key of -inf
+constexpr float kFar = -31.9998779296875f;  // 1/8192 short of -32: nothing at or below weighs anything (2^-40 is 27.7 down)
 
-// Order-preserving key: a < b as floats iff key(a) < key(b); -0 counts as +0, NaN as -inf.
+// Order-preserving key: a < b as floats iff key(a) < key(b); -0 counts as +0.  Not for NaN.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  x = x != x ? -INFINITY : x + 0.f;
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
-__device__ __forceinline__ uint64_t order_of(uint32_t key, uint32_t i) { return (uint64_t)key << 32 | (uint32_t)~i; }
-
-// Scale of a row: its maximum and 1 / T.
-struct Scale {
-  uint32_t top;
-  float m, r;
-  // (x - m) / T; the top itself may be infinite
-  __device__ __forceinline__ float gap(uint32_t k) const { return k == top ? 0.f : __fmul_rn(__fsub_rn(of_key(k), m), r); }
-  __device__ __forceinline__ uint64_t weight(uint32_t k) const {
-    const float e = expf(gap(k));
-    return k != kKeyNone && e > 0.f ? (uint64_t)__fmul_rn(e, kOne) : 0;  // not for NaN: an infinite gap times 1 / T = 0
-  }
-  // Step of 1/8192 below the maximum; the last one holds all that weighs nothing (beyond 40 ln 2 = 27.7).
-  __device__ __forceinline__ uint32_t step(uint32_t k) const {
-    const float d = gap(k) * -8192.f;
-    return d < (float)(kSampleSteps * kSampleSteps - 1) ? (uint32_t)d : kSampleSteps * kSampleSteps - 1;
-  }
-};
-constexpr uint32_t kLastStep = kSampleSteps * kSampleSteps - 1;
+__device__ __forceinline__ uint64_t order_of(float x, int i) { return (uint64_t)key_of(x) << 32 | (uint32_t)~i; }
+__device__ __forceinline__ float value_of(uint64_t o) { return of_key((uint32_t)(o >> 32)); }
+__device__ __forceinline__ int index_of(uint64_t o) { return (int)~(uint32_t)o; }
 
 struct SampleArgs {
   const void* x;
@@ -81,42 +67,93 @@ struct SampleArgs {
 // What a CTA's threads share, beside their part of the row.
 struct SampleShared {
   uint64_t list[kSampleList];
-  uint32_t lo[kSampleSteps], hi[kSampleSteps];  // a histogram of 64-bit sums
-  uint64_t slot[2][kMaxCluster];                // one word from every CTA of the cluster
-  uint64_t wsum[kSampleWarps], wbase[kSampleWarps];
+  uint32_t lo[kSteps], hi[kSteps];  // a histogram of 64-bit sums
+  uint64_t slot[2][kMaxCluster];    // one word from every CTA of the cluster
+  uint64_t wsum[kSampleWarps], wbase[kSampleWarps], all;
   uint64_t word[2];  // what the first CTA has decided
-  uint32_t pick;
+  uint32_t pick, count;
 };
+
+static_assert(sizeof(SampleShared) % 16 == 0, "the row follows it");
 
 template <class T>
 struct Sampler {
+  static constexpr int E = 16 / sizeof(T);  // tokens of a 16-byte piece
   SampleShared& sh;
-  const T* x;        // this CTA's part of the row
-  int n, base, ranks, rank;
-  int flip = 0;      // slot in use
-  Scale sc;
+  T* x;              // this CTA's part of the row, at the row's own alignment within 16 bytes; -inf around it
+  int pieces;        // 16-byte pieces of it
+  int base;          // index of x[0]; below the part's first token when that is not at a 16-byte boundary
+  int ranks, rank;
+  int flip;          // slot in use
+  float m, r;        // the row's maximum, 1 / T
+  uint64_t k;        // top_k
+  float p;           // top_p
+  uint64_t total;    // of the last histogram
+  double want, least;  // weight before which a token is still taken by top_p; weight that min_p asks for
+  float xe;          // the edge: tokens above xe, and those equal to it up to index ie
+  int ie;
 
-  __device__ __forceinline__ uint32_t key(int i) const { return key_of(to_f32(x[i])); }
+  // (x - m) / T; the maximum itself may be infinite.
+  __device__ __forceinline__ float gap(float v) const { return v == m ? 0.f : __fmul_rn(__fsub_rn(v, m), r); }
+  __device__ __forceinline__ uint64_t weigh(float g) const {  // g = NaN (an infinite gap times 1 / T = 0): nothing
+    const float e = expf(g);
+    return e > 0.f ? (uint64_t)__fmul_rn(e, kOne) : 0;
+  }
+  __device__ __forceinline__ uint64_t weight(float v) const { return weigh(gap(v)); }
+  __device__ __forceinline__ bool above_edge(float v, int i) const { return v > xe || (v == xe && i <= ie); }
+  __device__ __forceinline__ void set_edge(uint64_t o) {
+    xe = value_of(o);
+    ie = index_of(o);
+  }
+  template <bool MASS>
+  __device__ __forceinline__ bool taken(uint64_t b) const {  // whether a token before which b lies is taken
+    return MASS ? b == 0 || (double)b < want : b < k;
+  }
+
   __device__ __forceinline__ void sync() const {
     if (ranks > 1)
       cg::this_cluster().sync();
     else
       __syncthreads();
   }
-  // One word of every CTA, on every thread, combined in the order of the CTAs.
+  // f(value, index) of this thread's tokens: each warp has a contiguous run of pieces, lanes interleaved.
+  __device__ __forceinline__ void share(int& b, int& e) const {
+    const int each = (pieces + kSampleWarps - 1) / kSampleWarps;
+    b = min((int)(threadIdx.x >> 5) * each, pieces);
+    e = min(b + each, pieces);
+  }
+  __device__ __forceinline__ void piece(int c, float (&v)[E]) const {
+    const uint4 u = reinterpret_cast<const uint4*>(x)[c];
+    const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = to_f32(t[e]);
+  }
   template <class F>
-  __device__ __forceinline__ uint64_t combine(uint64_t v, F f) {  // v: of thread 0
+  __device__ __forceinline__ void each(F f) const {
+    int b, e;
+    share(b, e);
+#pragma unroll 2
+    for (int c = b + (threadIdx.x & 31); c < e; c += 32) {
+      float v[E];
+      piece(c, v);
+#pragma unroll
+      for (int j = 0; j < E; ++j) f(v[j], base + c * E + j);
+    }
+  }
+
+  // One word of every CTA (its thread 0's), on every thread, combined in the order of the CTAs.
+  template <class F>
+  __device__ __forceinline__ uint64_t combine(uint64_t v, F f) {
     flip ^= 1;
-    if (threadIdx.x == 0) {
-      if (ranks == 1) {
-        sh.slot[flip][0] = v;
-      } else {
-        for (int k = 0; k < ranks; ++k) *cg::this_cluster().map_shared_rank(&sh.slot[flip][rank], k) = v;
-      }
+    if (ranks == 1) {
+      if (threadIdx.x == 0) sh.slot[flip][0] = v;
+    } else if (threadIdx.x < 32) {
+      v = __shfl_sync(0xffffffffu, v, 0);
+      if (threadIdx.x < ranks) *cg::this_cluster().map_shared_rank(&sh.slot[flip][rank], threadIdx.x) = v;
     }
     sync();
     v = sh.slot[flip][0];
-    for (int k = 1; k < ranks; ++k) v = f(v, sh.slot[flip][k]);
+    for (int c = 1; c < ranks; ++c) v = f(v, sh.slot[flip][c]);
     return v;
   }
   template <class F>
@@ -139,7 +176,17 @@ struct Sampler {
   __device__ __forceinline__ uint64_t largest(uint64_t v) {
     return reduce(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
   }
-  // Sum of what lies before this thread in the CTA (threads in order); `all`: of the whole CTA.
+
+  // ---- teams: the first warp, or the CTA
+  template <bool WARP>
+  __device__ __forceinline__ static void team_sync() {
+    if (WARP)
+      __syncwarp();
+    else
+      __syncthreads();
+  }
+  // Sum of what lies before this thread in the team; `all`: of the whole team.
+  template <bool WARP>
   __device__ __forceinline__ uint64_t before(uint64_t v, uint64_t& all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint64_t run = v;
@@ -147,6 +194,10 @@ struct Sampler {
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t up = __shfl_up_sync(0xffffffffu, run, o);
       if (lane >= o) run += up;
+    }
+    if (WARP) {
+      all = __shfl_sync(0xffffffffu, run, 31);
+      return run - v;
     }
     __syncthreads();
     if (lane == 31) sh.wsum[warp] = run;
@@ -159,117 +210,137 @@ struct Sampler {
         if (lane >= o) t += up;
       }
       sh.wbase[lane] = t - w;
-      if (lane == 31) sh.word[1] = t;
+      if (lane == 31) sh.all = t;
     }
     __syncthreads();
-    all = sh.word[1];
+    all = sh.all;
     return sh.wbase[warp] + run - v;
   }
-  // The words that the first CTA wrote into sh.word, on every CTA.
-  __device__ __forceinline__ uint64_t decided() {
-    sync();
-    const uint64_t w = ranks == 1 ? sh.word[0] : *cg::this_cluster().map_shared_rank(&sh.word[0], 0);
-    sync();
-    return w;
-  }
-
-  // Warp w's contiguous share of the part.
-  __device__ __forceinline__ void share(int& b, int& e) const {
-    const int len = ((n + kSampleWarps - 1) / kSampleWarps + 31) / 32 * 32;
-    b = min((int)(threadIdx.x >> 5) * len, n);
-    e = min(b + len, n);
-  }
-  // Gathers (key, ~index) of the tokens with f(key, index) into the first CTA's list, in index order.
-  // Returns their number; nothing is written when the list cannot hold them.
-  template <class F>
-  __device__ __forceinline__ int gather(F f) {
-    const int lane = threadIdx.x & 31;
-    int b, e, count = 0;
-    share(b, e);
-    for (int i = b; i < e; i += 32) {
-      const int at = i + lane;
-      bool in = false;
-      if (at < e) in = f(key(at), base + at);
-      count += __popc(__ballot_sync(0xffffffffu, in));
-    }
-    uint64_t mine;
-    int place = (int)before(lane == 0 ? count : 0, mine);
-    place = __shfl_sync(0xffffffffu, place, 0);
-    const uint64_t all = combine(mine, [](uint64_t a, uint64_t c) { return a + c; });
-    for (int k = 0; k < rank; ++k) place += (int)sh.slot[flip][k];
-    if (all <= kSampleList) {
-      uint64_t* list = ranks == 1 ? sh.list : cg::this_cluster().map_shared_rank(sh.list, 0);
-      for (int i = b; i < e; i += 32) {
-        const int at = i + lane;
-        uint32_t k = 0;
-        bool in = false;
-        if (at < e) {
-          k = key(at);
-          in = f(k, base + at);
-        }
-        const uint32_t who = __ballot_sync(0xffffffffu, in);
-        if (in) list[place + __popc(who & ((1u << lane) - 1))] = order_of(k, base + at);
-        place += __popc(who);
-      }
-    }
-    sync();
-    return (int)min(all, (uint64_t)0x7FFFFFFF);
-  }
-  // Sorts list[0 .. m) of this CTA to falling order.
-  __device__ void sort_list(int m) {
+  // Sorts list[0 .. n) to falling order.
+  template <bool WARP>
+  __device__ __noinline__ static void sort(uint64_t* list, int n) {
+    const int me = threadIdx.x;
+    constexpr int team = WARP ? 32 : kSampleThreads;
     int size = 32;
-    while (size < m) size <<= 1;
-    for (int i = m + threadIdx.x; i < size; i += kSampleThreads) sh.list[i] = 0;
-    __syncthreads();
-    for (int k = 2; k <= size; k <<= 1) {
-      for (int j = k >> 1; j >= 32; j >>= 1) {
-        for (int t = threadIdx.x; t < size / 2; t += kSampleThreads) {
+    while (size < n) size <<= 1;
+    for (int i = n + me; i < size; i += team) list[i] = 0;
+    team_sync<WARP>();
+    for (int h = 2; h <= size; h <<= 1) {
+      for (int j = h >> 1; j >= 32; j >>= 1) {
+        for (int t = me; t < size / 2; t += team) {
           const int a = 2 * t - (t & (j - 1)), b = a + j;
-          const uint64_t u = sh.list[a], v = sh.list[b];
-          if ((u < v) == ((a & k) == 0)) {
-            sh.list[a] = v;
-            sh.list[b] = u;
+          const uint64_t u = list[a], v = list[b];
+          if ((u < v) == ((a & h) == 0)) {
+            list[a] = v;
+            list[b] = u;
           }
         }
-        __syncthreads();
+        team_sync<WARP>();
       }
-      for (int t = threadIdx.x; t < size; t += kSampleThreads) {  // strides within a warp
-        uint64_t v = sh.list[t];
-        for (int j = min(k >> 1, 16); j > 0; j >>= 1) {
+      for (int t = me; t < size; t += team) {  // strides within a warp
+        uint64_t v = list[t];
+        for (int j = min(h >> 1, 16); j > 0; j >>= 1) {
           const uint64_t u = __shfl_xor_sync(0xffffffffu, v, j);
-          const bool big = ((t & j) == 0) == ((t & k) == 0);  // this place takes the larger
+          const bool big = ((t & j) == 0) == ((t & h) == 0);  // this place takes the larger
           v = (u > v) == big ? u : v;
         }
-        sh.list[t] = v;
+        list[t] = v;
       }
-      __syncthreads();
+      if (h >= 32) team_sync<WARP>();  // smaller ones stay within a warp's 32 places
     }
+    team_sync<WARP>();
   }
-  // For a falling list of m tokens: how many are taken, where taken(b) says whether one with measure b
-  // before it is (it holds for none before, and never again once it does not).
-  template <bool MASS, class Taken>
-  __device__ int taken_of_list(int m, uint64_t above, Taken taken) {
-    constexpr int kEach = kSampleList / kSampleThreads;
-    const int i0 = threadIdx.x * kEach;
-    uint64_t w[kEach], mine = 0, all;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      w[e] = i0 + e < m ? (MASS ? sc.weight((uint32_t)(sh.list[i0 + e] >> 32)) : 1) : 0;
-      mine += w[e];
+  // For a falling list of n tokens, `above` before them: how many are taken.
+  template <bool WARP, bool MASS>
+  __device__ __forceinline__ int taken_of_list(int n, uint64_t above) {
+    const int per = (n + (WARP ? 32 : kSampleThreads) - 1) / (WARP ? 32 : kSampleThreads), i0 = threadIdx.x * per;
+    uint64_t mine = 0, all;
+    for (int i = i0; i < min(i0 + per, n); ++i) mine += MASS ? weight(value_of(sh.list[i])) : 1;
+    uint64_t b = above + before<WARP>(mine, all);
+    uint32_t yes = 0;
+    for (int i = i0; i < min(i0 + per, n); ++i) {
+      yes += taken<MASS>(b);
+      b += MASS ? weight(value_of(sh.list[i])) : 1;
     }
-    uint64_t b = above + before(mine, all);
-    int yes = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      yes += i0 + e < m && taken(b);
-      b += w[e];
-    }
-    return count_of(yes);
-  }
-  __device__ __forceinline__ int count_of(int v) {
-    uint64_t all;
-    (void)before((uint64_t)v, all);
+    (void)before<WARP>(yes, all);
     return (int)all;
+  }
+  __device__ __forceinline__ uint64_t aim(float u, uint64_t z) const {
+    return u > 0.f ? min((uint64_t)((double)u * (double)z), z - 1) : 0;
+  }
+  __device__ __forceinline__ void answer(const SampleArgs& a, int rw, int id, float v, uint64_t z, uint64_t kept) const {
+    a.id[rw] = id;
+    if (a.kept) a.kept[rw] = (int32_t)kept;
+    if (a.logprob) a.logprob[rw] = gap(v) - logf(__fdiv_rn((float)(double)z, kOne));
+  }
+  // Everything from a list that holds the top k tokens: the edge of top_p, the kept weight and the id.
+  template <bool WARP>
+  __device__ __forceinline__ void finish_list(const SampleArgs& a, int rw, int n) {
+    constexpr int team = WARP ? 32 : kSampleThreads;
+    const int me = threadIdx.x;
+    sort<WARP>(sh.list, n);
+    int c = (int)min((uint64_t)n, k);
+    if (!(p >= 1.f)) {
+      uint64_t total = 0, all;
+      for (int i = me; i < c; i += team) total += weight(value_of(sh.list[i]));
+      (void)before<WARP>(total, all);
+      want = (double)p * (double)all;
+      c = taken_of_list<WARP, true>(c, 0);
+    }
+    if (me == 0) sh.word[0] = sh.list[c - 1];
+    // the kept ones by rising index: sorted by (~index, key)
+    team_sync<WARP>();
+    for (int i = me; i < c; i += team) {
+      const uint64_t v = sh.list[i];
+      sh.list[i] = v << 32 | v >> 32;
+    }
+    team_sync<WARP>();
+    sort<WARP>(sh.list, c);
+    const int per = (c + team - 1) / team, i0 = me * per, i1 = min(i0 + per, c);
+    uint64_t mass = 0, some = 0, z, kept;
+    for (int i = i0; i < i1; ++i) {
+      const uint64_t w = weight(of_key((uint32_t)sh.list[i]));
+      if (w == 0 || (double)w < least) continue;
+      mass += w;
+      ++some;
+    }
+    (void)before<WARP>(some, kept);
+    uint64_t b = before<WARP>(mass, z);
+    const uint64_t at = aim(a.u[rw], z);
+    if (b <= at && at < b + mass) {
+      for (int i = i0; i < i1; ++i) {
+        const uint64_t v = sh.list[i], w = weight(of_key((uint32_t)v));
+        if (w == 0 || (double)w < least) continue;
+        if (at < b + w) {
+          answer(a, rw, index_of(v >> 32), of_key((uint32_t)v), z, kept);
+          break;
+        }
+        b += w;
+      }
+    }
+    if (me == 0) sh.word[1] = z;
+  }
+
+  // Gathers the tokens with f(value, index) into the first CTA's list, in no order.  Returns their number;
+  // the list is cut off at its length.  sh.count of the first CTA is 0 before.
+  template <class F>
+  __device__ __forceinline__ int gather(F f) {
+    uint64_t* list = sh.list;
+    uint32_t* count = &sh.count;
+    if (ranks > 1) {
+      list = cg::this_cluster().map_shared_rank(list, 0);
+      count = cg::this_cluster().map_shared_rank(count, 0);
+    }
+    each([&](float v, int i) {
+      if (!f(v, i)) return;
+      const uint32_t at = atomicAdd(count, 1u);
+      if (at < kSampleList) list[at] = order_of(v, i);
+    });
+    sync();
+    const int n = (int)*(volatile uint32_t*)count;
+    sync();
+    if (rank == 0 && threadIdx.x == 0) sh.count = 0;
+    return n;
   }
 
   // Histogram step: adds v to the 64-bit sum of step s.  The carry out of the low word is seen by the one
@@ -280,285 +351,312 @@ struct Sampler {
     const uint32_t h = (uint32_t)(v >> 32) + (was + l < l);
     if (h) atomicAdd(&sh.hi[s], h);
   }
-  // One level: the last step, counted from the top, before which little enough lies, of the tokens with
-  // f(key, index, step) (which also gives the token's step of this level).  `above`: what lies before it.
-  template <bool MASS, class F, class Taken>
-  __device__ uint32_t level(uint64_t& above, F f, Taken taken) {
+  __device__ __forceinline__ void clear() {
     __syncthreads();
-    for (int i = threadIdx.x; i < kSampleSteps; i += kSampleThreads) sh.lo[i] = sh.hi[i] = 0;
+    for (int i = threadIdx.x; i < kSteps; i += kSampleThreads) sh.lo[i] = sh.hi[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kSampleThreads) {
-      const uint32_t k = key(i);
-      uint32_t s;
-      if (!f(k, base + i, s)) continue;
-      if (MASS) {
-        const uint64_t w = sc.weight(k);
-        if (w) add(s, w);
-      } else {
-        atomicAdd(&sh.lo[s], 1u);
-      }
-    }
+  }
+  // Of the cluster's histogram: the last step, counted from the top, whose first token is taken.  `above`:
+  // what lies before it, at first what lies before step 0.  TOTAL: top_p's limit is of this histogram's sum.
+  template <bool MASS, bool TOTAL>
+  __device__ __forceinline__ uint32_t pick(uint64_t& above) {
     sync();
     uint64_t v = 0, all;
-    if (threadIdx.x < kSampleSteps) {
+    if (threadIdx.x < kSteps) {
       for (int c = 0; c < ranks; ++c) {  // every CTA sums all: none has to tell the others
         const SampleShared* o = ranks == 1 ? &sh : cg::this_cluster().map_shared_rank(&sh, c);
         v += (uint64_t)o->hi[threadIdx.x] << 32 | o->lo[threadIdx.x];
       }
     }
     if (threadIdx.x == 0) sh.pick = 0;
-    const uint64_t b = above + before(v, all);
-    if (v && taken(b)) atomicMax(&sh.pick, threadIdx.x);
+    const uint64_t b = above + before<false>(v, all);
+    total = all;
+    if (TOTAL) want = (double)p * (double)all;
+    if (v && taken<MASS>(b)) atomicMax(&sh.pick, threadIdx.x);
     __syncthreads();
     const uint32_t s = sh.pick;
-    if (threadIdx.x == s) sh.word[0] = b;
+    if (threadIdx.x == s) sh.word[1] = b;
     sync();  // also: the other CTAs have read this one's sums
-    above = sh.word[0];
+    above = sh.word[1];
     return s;
   }
-  // The edge among the tokens at or above `edge`: see taken_of_list.
-  template <bool MASS, class Taken>
-  __device__ uint64_t find_edge(uint64_t edge, Taken taken) {
+  // The edge of top_k (by tokens) or top_p (by weight) among the tokens above the present one.
+  template <bool MASS>
+  __device__ __forceinline__ void find_edge() {
     uint64_t above = 0;
-    const uint32_t s1 = level<MASS>(above, [&](uint32_t k, int i, uint32_t& s) {
-      const uint32_t t = sc.step(k);
-      s = t / kSampleSteps;
-      return t != kLastStep && order_of(k, i) >= edge;
-    }, taken);
-    const uint32_t s2 = level<MASS>(above, [&](uint32_t k, int i, uint32_t& s) {
-      const uint32_t t = sc.step(k);
-      s = t % kSampleSteps;
-      return t / kSampleSteps == s1 && t != kLastStep && order_of(k, i) >= edge;
-    }, taken);
-    const uint32_t want = s1 * kSampleSteps + s2;
-    auto in = [&](uint32_t k, int i) { return sc.step(k) == want && order_of(k, i) >= edge; };
-    const int m = gather(in);
-    if (m <= kSampleList) {
-      if (rank == 0) {
-        sort_list(m);
-        const int c = taken_of_list<MASS>(m, above, taken);
+    clear();
+    each([&](float v, int i) {
+      const float g = gap(v);
+      if (!(g > kFar) || !above_edge(v, i)) return;
+      const uint32_t s = (uint32_t)(g * -16.f);
+      if (MASS) {
+        const uint64_t w = weigh(g);
+        if (w) add(s, w);
+      } else {
+        atomicAdd(&sh.lo[s], 1u);
+      }
+    });
+    const uint32_t s1 = pick<MASS, MASS>(above);
+    const float from = -0.0625f * (float)s1, to = from - 0.0625f;
+    auto in1 = [&](float v, int i) {
+      const float g = gap(v);
+      return g <= from && g > to && g > kFar && above_edge(v, i);
+    };
+    int n = gather(in1);
+    if (n > kSampleList) {
+      clear();
+      each([&](float v, int i) {
+        if (!in1(v, i)) return;
+        const float g = gap(v);
+        const uint32_t s = (uint32_t)(g * -8192.f) % kSteps;
+        if (MASS) {
+          const uint64_t w = weigh(g);
+          if (w) add(s, w);
+        } else {
+          atomicAdd(&sh.lo[s], 1u);
+        }
+      });
+      const uint32_t s2 = s1 * kSteps + pick<MASS, false>(above);
+      auto in2 = [&](float v, int i) { return in1(v, i) && (uint32_t)(gap(v) * -8192.f) == s2; };
+      n = gather(in2);
+      if (n > kSampleList) return halve<MASS>(above, in2);
+    }
+    if (rank == 0) {
+      if (n <= kWarpList) {
+        if (threadIdx.x < 32) {
+          sort<true>(sh.list, n);
+          const int c = taken_of_list<true, MASS>(n, above);
+          if (threadIdx.x == 0) sh.word[0] = sh.list[max(c, 1) - 1];
+        }
+      } else {
+        sort<false>(sh.list, n);
+        const int c = taken_of_list<false, MASS>(n, above);
         if (threadIdx.x == 0) sh.word[0] = sh.list[max(c, 1) - 1];
       }
-      return decided();
     }
-    // halving: the lowest number above which little enough lies
-    uint64_t low = ~0ull, high = 0;  // of the tokens of this step
-    for (int i = threadIdx.x; i < n; i += kSampleThreads) {
-      const uint32_t k = key(i);
-      if (!in(k, base + i)) continue;
-      low = min(low, order_of(k, base + i));
-      high = max(high, order_of(k, base + i));
-    }
+    sync();
+    set_edge(ranks == 1 ? sh.word[0] : *cg::this_cluster().map_shared_rank(&sh.word[0], 0));
+    sync();
+  }
+  // The lowest number above which little enough lies, among the tokens of `in`.
+  template <bool MASS, class F>
+  __device__ __forceinline__ void halve(uint64_t above, F in) {
+    uint64_t low = ~0ull, high = 0;
+    each([&](float v, int i) {
+      if (!in(v, i)) return;
+      low = min(low, order_of(v, i));
+      high = max(high, order_of(v, i));
+    });
     low = ~largest(~low);
     high = largest(high);
     while (low < high) {
       const uint64_t mid = low + (high - low) / 2;
-      uint64_t v = 0;
-      for (int i = threadIdx.x; i < n; i += kSampleThreads) {
-        const uint32_t k = key(i);
-        if (order_of(k, base + i) > mid && in(k, base + i)) v += MASS ? sc.weight(k) : 1;
-      }
-      if (taken(above + sum(v)))
+      uint64_t b = 0;
+      each([&](float v, int i) {
+        if (in(v, i) && order_of(v, i) > mid) b += MASS ? weight(v) : 1;
+      });
+      if (taken<MASS>(above + sum(b)))
         high = mid;
       else
         low = mid + 1;
     }
-    return low;
+    set_edge(low);
   }
 };
 
 template <class T>
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
+  using S = Sampler<T>;
+  constexpr int E = S::E;
   SampleShared& sh = *reinterpret_cast<SampleShared*>(smem);
-  T* const x = reinterpret_cast<T*>(smem + sizeof(SampleShared));
-  const int ranks = gridDim.x, rank = blockIdx.x, rw = blockIdx.y;
-  const int tid = threadIdx.x, lane = tid & 31;
-  Sampler<T> s{sh, x, 0, 0, ranks, rank};
-  s.base = min(rank * a.part, a.vocab);
-  s.n = min(a.part, a.vocab - s.base);
-  const int n = s.n;
-  float* const probs = a.probs ? a.probs + (int64_t)rw * a.vocab + s.base : nullptr;
+  const int rw = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  S s{sh, reinterpret_cast<T*>(smem + sizeof(SampleShared))};
+  s.ranks = gridDim.x;
+  s.rank = blockIdx.x;
+  s.flip = 0;
+  const int first = min(s.rank * a.part, a.vocab), n = min(a.part, a.vocab - first);  // this CTA's tokens
+  const T* const row = static_cast<const T*>(a.x) + (int64_t)rw * a.row_stride + first;
+  const int lead = (int)((uintptr_t)row & 15) / (int)sizeof(T);
+  s.base = first - lead;
+  s.pieces = (lead + n + E - 1) / E;
+  float* const probs = a.probs ? a.probs + (int64_t)rw * a.vocab : nullptr;
+  if (tid == 0) sh.count = 0;
+  for (int i = tid; i < kSteps; i += kSampleThreads) sh.lo[i] = sh.hi[i] = 0;
   // ---- the row, and every thread's maximum
-  const T* const row = static_cast<const T*>(a.x) + (int64_t)rw * a.row_stride + s.base;
-  uint32_t mine = 0;
-#pragma unroll 8
-  for (int i = tid; i < n; i += kSampleThreads) {
-    const T v = row[i];
-    x[i] = v;
-    mine = max(mine, key_of(to_f32(v)));
+  float mine = -INFINITY;
+  {
+    const uint4* const from = reinterpret_cast<const uint4*>(row - lead);
+    int b, e;
+    s.share(b, e);
+#pragma unroll 4
+    for (int c = b + lane; c < e; c += 32) {
+      uint4 u;
+      if (c * E >= lead && (c + 1) * E <= lead + n) {
+        u = __ldcs(from + c);
+      } else {  // the row ends within this piece: token by token
+        T v[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const int i = c * E + j - lead;
+          v[j] = i >= 0 && i < n ? row[i] : from_f32<T>(-INFINITY);
+        }
+        u = *reinterpret_cast<const uint4*>(v);
+      }
+      reinterpret_cast<uint4*>(s.x)[c] = u;
+      const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int j = 0; j < E; ++j) mine = fmaxf(mine, to_f32(t[j]));  // not NaN's
+    }
   }
-  if (ranks > 1) s.sync();  // every CTA of the cluster runs before its memory is written
-  s.sc.top = (uint32_t)s.largest(mine);
-  s.sc.m = of_key(s.sc.top);
-  s.sc.r = 1.f;
-  auto none = [&] {  // no token to draw
-    if (rank == 0 && tid == 0) {
+  if (s.ranks > 1) s.sync();  // every CTA of the cluster runs before its memory is written
+  s.m = of_key((uint32_t)s.largest(key_of(mine)));
+  const float min_p = a.min_p ? a.min_p[rw] : 0.f, t = a.temperature ? a.temperature[rw] : 1.f;
+  s.least = (double)min_p * (double)kOne;
+  if (s.m == -INFINITY || min_p > 1.f) {  // no token to draw
+    if (s.rank == 0 && tid == 0) {
       a.id[rw] = -1;
       if (a.logprob) a.logprob[rw] = -INFINITY;
       if (a.kept) a.kept[rw] = 0;
     }
     if (probs)
-      for (int i = tid; i < n; i += kSampleThreads) probs[i] = 0.f;
-  };
-  const double least = (double)(a.min_p ? a.min_p[rw] : 0.f) * (double)kOne;
-  if (s.sc.top <= kKeyNone || least > (double)kOne) {
-    none();
-    if (ranks > 1) s.sync();  // no CTA leaves while another may still write its words
+      for (int i = tid; i < n; i += kSampleThreads) probs[first + i] = 0.f;
+    if (s.ranks > 1) s.sync();  // no CTA leaves while another may still write its words
     return;
   }
-  const float t = a.temperature ? a.temperature[rw] : 1.f;
   const bool greedy = !(t > 0.f);
-  if (!greedy) s.sc.r = __fdiv_rn(1.f, t);
+  s.r = greedy ? 1.f : __fdiv_rn(1.f, t);
   int k = greedy ? 1 : (a.top_k ? a.top_k[rw] : 0);
   if (k <= 0 || k > a.vocab) k = a.vocab;
-  const float p = a.top_p ? a.top_p[rw] : 1.f;
-  const float u = a.u[rw];
+  s.k = k;
+  s.p = a.top_p ? a.top_p[rw] : 1.f;
+  s.xe = -INFINITY;  // every token that weighs anything
+  s.ie = -1;
 
   // ---- the edge: tokens at or above it are kept
-  uint64_t edge = 0;
-  bool listed = false;  // the first CTA's list holds all kept tokens
-  int kept_list = 0;
+  bool listed = false;  // the first CTA's list holds the top k
   if (k < a.vocab && k <= kSampleMaxK) {
-    // the k-th largest of this CTA's thread maxima, to 16 bits: at least k tokens are as large
-    uint32_t low = 0;
+    // the step in which the k-th largest of the threads' maxima lies, and all that is above it
+    float to = 0.f;
     if (k == 1) {
-      low = s.sc.top;
+      to = -1e-30f;
     } else {
-      for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
-        if (__syncthreads_count(mine >= (low | bit)) >= k) low |= bit;
-      if (ranks > 1) low = (uint32_t)s.combine(low, [](uint64_t b, uint64_t c) { return b > c ? b : c; });
+      const float g = s.gap(mine);
+      if (g > kFar) atomicAdd(&sh.lo[(uint32_t)(g * -16.f)], 1u);
+      uint64_t above = 0;
+      to = -0.0625f * (float)(s.template pick<false, false>(above) + 1);
+      if (s.total < s.k) to = kFar;  // fewer threads than k hold a token of weight
     }
-    low = max(low, kKeyNone + 1);
-    const int m = s.gather([&](uint32_t key, int) { return key >= low; });
-    if (m <= kSampleList) {
+    const int c = s.gather([&](float v, int) {
+      const float g = s.gap(v);
+      return g > to && g > kFar;
+    });
+    if (c <= kSampleList) {
       listed = true;
-      if (rank == 0) {
-        s.sort_list(m);
-        int c = min(m, k);
-        if (!(p >= 1.f)) {
-          uint64_t total = 0, all;
-          for (int i = tid; i < c; i += kSampleThreads) total += s.sc.weight((uint32_t)(sh.list[i] >> 32));
-          (void)s.before(total, all);
-          const double want = (double)p * (double)all;
-          c = max(1, s.template taken_of_list<true>(c, 0, [&](uint64_t b) { return b == 0 || (double)b < want; }));
-        }
-        kept_list = c;
+      if (s.rank == 0) {
+        if (c > kWarpList)
+          s.template finish_list<false>(a, rw, c);
+        else if (tid < 32)
+          s.template finish_list<true>(a, rw, c);
       }
     }
   }
-  if (!listed) {
-    if (k < a.vocab) edge = s.template find_edge<false>(0, [&](uint64_t b) { return b < (uint64_t)k; });
-    if (!(p >= 1.f)) {
-      uint64_t v = 0;
-      for (int i = tid; i < n; i += kSampleThreads) {
-        const uint32_t key = s.key(i);
-        if (order_of(key, s.base + i) >= edge) v += s.sc.weight(key);
-      }
-      const double want = (double)p * (double)s.sum(v);
-      edge = s.template find_edge<true>(edge, [&](uint64_t b) { return b == 0 || (double)b < want; });
-    }
-  }
-  auto kept_weight = [&](uint32_t key, int i) -> uint64_t {
-    if (order_of(key, i) < edge) return 0;
-    const uint64_t w = s.sc.weight(key);
-    return (double)w >= least ? w : 0;
-  };
-  auto aim_of = [&](uint64_t z) { return u > 0.f ? min((uint64_t)((double)u * (double)z), z - 1) : 0; };
-  auto answer = [&](int id, uint32_t key, uint64_t z, uint64_t kept) {
-    a.id[rw] = id;
-    if (a.kept) a.kept[rw] = (int32_t)kept;
-    if (a.logprob) a.logprob[rw] = s.sc.gap(key) - logf(__fdiv_rn((float)(double)z, kOne));
-  };
-  // ---- the kept weight Z, and the token in index order where the running weight passes floor(u Z)
   uint64_t z = 0;
   if (listed) {
-    if (rank == 0) {
-      edge = sh.list[kept_list - 1];
-      __syncthreads();
-      for (int i = tid; i < kept_list; i += kSampleThreads) {  // to rising index: sorted by (~index, key)
-        const uint64_t v = sh.list[i];
-        sh.list[i] = v << 32 | v >> 32;
-      }
-      __syncthreads();
-      s.sort_list(kept_list);
-      constexpr int kEach = kSampleList / kSampleThreads;
-      uint64_t w[kEach], mass = 0;
-      int some = 0;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int i = tid * kEach + e;
-        w[e] = i < kept_list ? s.sc.weight((uint32_t)sh.list[i]) : 0;
-        if ((double)w[e] < least) w[e] = 0;
-        mass += w[e];
-        some += w[e] > 0;
-      }
-      const uint64_t kept = s.count_of(some);
-      uint64_t b = s.before(mass, z);
-      const uint64_t aim = aim_of(z);
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        if (w[e] && b <= aim && aim < b + w[e]) {
-          const uint64_t v = sh.list[tid * kEach + e];
-          answer((int)~(uint32_t)(v >> 32), (uint32_t)v, z, kept);
-        }
-        b += w[e];
-      }
-      if (tid == 0) {
-        sh.word[0] = edge;
-        sh.word[1] = z;
-      }
-    }
     if (probs) {
       s.sync();
-      const uint64_t* word = ranks == 1 ? sh.word : cg::this_cluster().map_shared_rank(sh.word, 0);
-      edge = word[0];
+      const uint64_t* word = s.ranks == 1 ? sh.word : cg::this_cluster().map_shared_rank(sh.word, 0);
+      s.set_edge(word[0]);
       z = word[1];
     }
   } else {
+    if (k < a.vocab) s.template find_edge<false>();
+    if (!(s.p >= 1.f)) s.template find_edge<true>();
+    // ---- the kept weight Z, and the token in index order where the running weight passes floor(u Z).  Few
+    // tokens are kept as a rule: a thread marks its own first, then weighs those.
+    auto kept_weight = [&](float v, int i) -> uint64_t {
+      if (!s.above_edge(v, i)) return 0;
+      const uint64_t w = s.weight(v);
+      return (double)w >= s.least ? w : 0;
+    };
     int b, e;
     s.share(b, e);
-    uint64_t v = 0;
-    int some = 0;
-    for (int i = b + lane; i < e; i += 32) {
-      const uint64_t w = kept_weight(s.key(i), s.base + i);
-      v += w;
-      some += w > 0;
+    uint64_t v = 0, some = 0;
+    constexpr int kMark = 32 / E;  // pieces of a mask
+    for (int c0 = b + lane; c0 < e; c0 += 32 * kMark) {
+      uint32_t mask = 0;
+#pragma unroll
+      for (int q = 0; q < kMark; ++q) {
+        const int c = c0 + 32 * q;
+        if (c >= e) break;
+        float f[E];
+        s.piece(c, f);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (s.above_edge(f[j], s.base + c * E + j)) mask |= 1u << (q * E + j);
+      }
+      while (mask) {
+        const int bit = __ffs((int)mask) - 1;
+        mask &= mask - 1;
+        const uint64_t w = s.weight(to_f32(s.x[(c0 + 32 * (bit / E)) * E + bit % E]));
+        if ((double)w < s.least) continue;
+        v += w;
+        some += w > 0;
+      }
     }
     const uint64_t kept = s.sum(some);
     uint64_t all;
-    uint64_t lead = s.before(v, all);  // this warp's, then the CTA's
-    z = s.combine(all, [](uint64_t c, uint64_t d) { return c + d; });
-    uint64_t aim = aim_of(z);
-    for (int c = 0; c < rank; ++c) lead += sh.slot[s.flip][c];
-    const uint64_t first = __shfl_sync(0xffffffffu, lead, 0);
+    uint64_t ahead = s.template before<false>(v, all);
+    z = s.combine(all, [](uint64_t x, uint64_t y) { return x + y; });
+    for (int c = 0; c < s.rank; ++c) ahead += sh.slot[s.flip][c];
+    ahead = __shfl_sync(0xffffffffu, ahead, 0);  // before this warp's share
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (first <= aim && aim < first + v) {  // one warp of one CTA: the place in its share
-      aim -= first;
-      for (int i = b; i < e; i += 32) {
-        const uint32_t key = i + lane < e ? s.key(i + lane) : kKeyNone;
-        const uint64_t w = i + lane < e ? kept_weight(key, s.base + i + lane) : 0;
-        uint64_t run = w;
+    uint64_t aim = s.aim(a.u[rw], z);
+    if (ahead <= aim && aim < ahead + v) {  // one warp of one CTA: the place in its share
+      aim -= ahead;
+      for (int c = b; c < e; c += 32) {
+        float f[E];
+        uint64_t w[E], own = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint64_t up = __shfl_up_sync(0xffffffffu, run, o);
-          if (lane >= o) run += up;
+        for (int j = 0; j < E; ++j) w[j] = 0;
+        if (c + lane < e) {
+          s.piece(c + lane, f);
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            w[j] = kept_weight(f[j], s.base + (c + lane) * E + j);
+            own += w[j];
+          }
         }
-        const uint64_t past = __ballot_sync(0xffffffffu, run > aim);
-        if (past) {
-          if (lane == __ffs((int)past) - 1) answer(s.base + i + lane, key, z, kept);
+        uint64_t sum;
+        uint64_t before = s.template before<true>(own, sum);
+        if (aim < sum) {
+          if (before <= aim && aim < before + own) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+              if (before <= aim && aim < before + w[j]) s.answer(a, rw, s.base + (c + lane) * E + j, f[j], z, kept);
+              before += w[j];
+            }
+          }
           break;
         }
-        aim -= __shfl_sync(0xffffffffu, run, 31);
+        aim -= sum;
       }
     }
   }
   if (probs) {
     const float zf = (float)z;
-    for (int i = tid; i < n; i += kSampleThreads) probs[i] = __fdiv_rn((float)kept_weight(s.key(i), s.base + i), zf);
+    for (int i = tid; i < n; i += kSampleThreads) {
+      const float v = to_f32(s.x[lead + i]);
+      float q = 0.f;
+      if (s.above_edge(v, first + i)) {
+        const uint64_t w = s.weight(v);
+        if ((double)w >= s.least) q = __fdiv_rn((float)w, zf);
+      }
+      probs[first + i] = q;
+    }
   }
-  if (ranks > 1) s.sync();  // no CTA leaves while another may still read or write its words
+  if (s.ranks > 1) s.sync();  // no CTA leaves while another may still read or write its words
 }
 
 // Opt in to the shared memory, and to clusters of 16, once per kernel and device.
@@ -580,7 +678,7 @@ int launch_sample(SampleArgs a, int rows, cudaStream_t st) {
       !allow_sample<T>(dev))
     return refuse(MLLM_ERR_CUDA, "mllm_sample: no current CUDA device, or too little shared memory");
   // CTAs per row: as many as its tokens need room for, and more while SMs are left and each keeps 4,096 tokens
-  const int64_t room = (227 * 1024 - (int64_t)sizeof(SampleShared)) / sizeof(T) / 32 * 32;
+  const int64_t room = (227 * 1024 - 32 - (int64_t)sizeof(SampleShared)) / sizeof(T) / 32 * 32;
   int ranks = 1;
   while (ranks < kMaxCluster && ((int64_t)ranks * room < a.vocab || ((int64_t)rows * ranks * 2 <= sms && a.vocab / (2 * ranks) >= 4096)))
     ranks *= 2;
@@ -588,7 +686,7 @@ int launch_sample(SampleArgs a, int rows, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ranks, rows);
   cfg.blockDim = dim3(kSampleThreads);
-  cfg.dynamicSmemBytes = sizeof(SampleShared) + (size_t)a.part * sizeof(T);
+  cfg.dynamicSmemBytes = sizeof(SampleShared) + (size_t)a.part * sizeof(T) + 32;  // a piece at either end
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
