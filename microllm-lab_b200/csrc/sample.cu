@@ -17,10 +17,19 @@
 //   - otherwise by a histogram of tokens or weight over 512 such steps, then among the tokens of one step,
 //     or of a 512th of it where they are too many for a list;
 //   - and by halving, one pass per bit, where those are too many as well (thousands of tokens of one value).
-// A list is sorted and summed by one warp when it is short, by the CTA otherwise.
+// A short list is not sorted either: several threads per token count, and weigh, what precedes it.
+// Every CTA of a cluster keeps its own copy of a list and comes to the same edge, so that they meet at a
+// barrier only to exchange a maximum, a histogram, a list or a sum.
+//
+// Of a few microseconds per row much goes into fetching instructions, so the code is kept small: what runs
+// once is called, not inlined, and the passes over the row either test 16 bytes at a time and do the rest
+// for the few that pass, or take a token at a time.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+#include <cstdlib>
 #include <atomic>
+#include <climits>
 
 #include "device_common.cuh"
 #include "paged.cuh"
@@ -34,7 +43,7 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleList = 2048;   // tokens of a list
-constexpr int kWarpList = 128;      // tokens of a list that one warp handles
+constexpr int kShortList = 256;     // tokens of a list that is counted instead of sorted
 constexpr int kSampleMaxK = 512;    // top_k that starts from the threads' maxima
 constexpr int kSteps = 512;         // steps of a histogram level
 constexpr int kMaxCluster = 16;
@@ -64,17 +73,136 @@ struct SampleArgs {
   float* probs;
 };
 
-// What a CTA's threads share, beside their part of the row.
-struct SampleShared {
+// What a CTA's threads share, beside their part of the row.  What other CTAs write or read is there twice, used
+// in turn: a CTA cannot be two exchanges ahead of another.
+struct alignas(16) SampleShared {
   uint64_t list[kSampleList];
-  uint32_t lo[kSteps], hi[kSteps];  // a histogram of 64-bit sums
-  uint64_t slot[2][kMaxCluster];    // one word from every CTA of the cluster
-  uint64_t wsum[kSampleWarps], wbase[kSampleWarps], all;
-  uint64_t word[2];  // what the first CTA has decided
-  uint32_t pick, count;
+  uint32_t lo[2][kSteps], hi[2][kSteps];  // a histogram of 64-bit sums
+  uint64_t slot[2][kMaxCluster][2];       // two words from every CTA of the cluster
+  uint64_t weights[kShortList];
+  uint64_t wsum[kSampleWarps];
+  uint64_t word;
+  uint32_t pick, count[2];
 };
 
-static_assert(sizeof(SampleShared) % 16 == 0, "the row follows it");
+// ---- over a CTA's threads
+// Sum over a warp, in three parts whose sums 32 bits hold.
+__device__ __forceinline__ uint64_t warp_add(uint64_t v) {
+  const uint32_t a = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0x7FFFFFFu);
+  const uint32_t b = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 27) & 0x7FFFFFFu);
+  const uint32_t c = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 54));
+  return ((uint64_t)c << 54) + ((uint64_t)b << 27) + a;
+}
+__device__ __forceinline__ uint64_t warp_most(uint64_t v) {
+  const uint32_t h = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+  const uint32_t l = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == h ? (uint32_t)v : 0u);
+  return (uint64_t)h << 32 | l;
+}
+template <bool MAX>
+__device__ __noinline__ uint64_t cta_reduce(uint64_t* wsum, uint64_t v) {
+  v = MAX ? warp_most(v) : warp_add(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) wsum[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = wsum[threadIdx.x & 31];
+  return MAX ? warp_most(v) : warp_add(v);
+}
+// Sum of what lies before this thread in its warp, and of the whole warp.
+struct Scan {
+  uint64_t before, all;
+};
+__device__ __forceinline__ Scan warp_scan(uint64_t v) {
+  uint64_t run = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t up = __shfl_up_sync(0xffffffffu, run, o);
+    if ((threadIdx.x & 31) >= o) run += up;
+  }
+  return {run - v, __shfl_sync(0xffffffffu, run, 31)};
+}
+__device__ __noinline__ Scan cta_scan(uint64_t* wsum, uint64_t v) {
+  const Scan in = warp_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) wsum[threadIdx.x >> 5] = in.all;
+  __syncthreads();
+  const Scan of = warp_scan(wsum[threadIdx.x & 31]);
+  return {__shfl_sync(0xffffffffu, of.before, threadIdx.x >> 5) + in.before, of.all};
+}
+// Sorts list[0 .. n) to falling order.
+__device__ __noinline__ void cta_sort(uint64_t* list, int n) {
+  int size = 32;
+  while (size < n) size <<= 1;
+  for (int i = n + threadIdx.x; i < size; i += kSampleThreads) list[i] = 0;
+  __syncthreads();
+  for (int h = 2; h <= size; h <<= 1) {
+    for (int j = h >> 1; j >= 32; j >>= 1) {
+      for (int t = threadIdx.x; t < size / 2; t += kSampleThreads) {
+        const int a = 2 * t - (t & (j - 1)), b = a + j;
+        const uint64_t u = list[a], v = list[b];
+        if ((u < v) == ((a & h) == 0)) {
+          list[a] = v;
+          list[b] = u;
+        }
+      }
+      __syncthreads();
+    }
+    for (int t = threadIdx.x; t < size; t += kSampleThreads) {  // strides within a warp
+      uint64_t v = list[t];
+      for (int j = min(h >> 1, 16); j > 0; j >>= 1) {
+        const uint64_t u = __shfl_xor_sync(0xffffffffu, v, j);
+        const bool big = ((t & j) == 0) == ((t & h) == 0);  // this place takes the larger
+        v = (u > v) == big ? u : v;
+      }
+      list[t] = v;
+    }
+    if (h >= 32) __syncthreads();  // smaller ones stay within a warp's 32 places
+  }
+  __syncthreads();
+}
+
+// (x - m) / T; m is finite here, and 1 / T above 0.
+__device__ __forceinline__ float gap_of(float v, float m, float r) { return __fmul_rn(__fsub_rn(v, m), r); }
+// floor(2^40 e^g), with shifts of the mantissa: conversions share a slow unit with the exponential's.
+__device__ __forceinline__ uint64_t weigh(float g) {
+  const float e = expf(g);
+  const uint32_t b = __float_as_uint(e), m24 = (b & 0x7FFFFFu) | 0x800000u;
+  const int up = (int)(b >> 23) - 110;  // e = m24 2^(up - 40); a subnormal e, or 0, weighs nothing by the shift
+  const uint32_t lo = __funnelshift_lc(0u, m24, (uint32_t)up) | __funnelshift_rc(m24, 0u, (uint32_t)-up);
+  return (uint64_t)__funnelshift_rc(m24, 0u, (uint32_t)(32 - up)) << 32 | lo;
+}
+__device__ __noinline__ uint64_t weight_of(float v, float m, float r) { return weigh(gap_of(v, m, r)); }
+// Whole part of 0 <= v < 2^23, without a conversion.
+__device__ __forceinline__ uint32_t whole(float v) { return __float_as_uint(__fadd_rz(v, 8388608.f)) & 0x7FFFFFu; }
+
+// A short list: this thread's token (-1: none), which `team` neighbouring threads share, its order and, on the
+// first of them, its weight; the number and weight of the tokens before it in the list.
+struct Place {
+  int t, team;
+  uint64_t order, w, weight_before;
+  uint32_t count_before;
+};
+__device__ __noinline__ Place place_of(SampleShared& sh, int n, float m, float r) {
+  Place q;
+  q.team = n <= 32 ? 32 : n <= 64 ? 16 : n <= 128 ? 8 : 4;
+  if (threadIdx.x < n) sh.weights[threadIdx.x] = weight_of(value_of(sh.list[threadIdx.x]), m, r);
+  __syncthreads();
+  q.t = threadIdx.x / q.team;
+  if (q.t >= n) q.t = -1;
+  q.order = q.t < 0 ? ~0ull : sh.list[q.t];
+  q.w = q.t < 0 || (threadIdx.x & (q.team - 1)) ? 0 : sh.weights[q.t];
+  q.weight_before = 0;
+  q.count_before = 0;
+  for (int j = threadIdx.x & (q.team - 1); j < n; j += q.team)
+    if (sh.list[j] > q.order) {
+      ++q.count_before;
+      q.weight_before += sh.weights[j];
+    }
+  for (int o = q.team >> 1; o > 0; o >>= 1) {
+    q.count_before += __shfl_xor_sync(0xffffffffu, q.count_before, o);
+    q.weight_before += __shfl_xor_sync(0xffffffffu, q.weight_before, o);
+  }
+  return q;
+}
 
 template <class T>
 struct Sampler {
@@ -84,31 +212,25 @@ struct Sampler {
   int pieces;        // 16-byte pieces of it
   int base;          // index of x[0]; below the part's first token when that is not at a 16-byte boundary
   int ranks, rank;
-  int flip;          // slot in use
+  int flip, hist, listed;  // which of the two slots, histograms and counts is in use
   float m, r;        // the row's maximum, 1 / T
   uint64_t k;        // top_k
   float p;           // top_p
   uint64_t total;    // of the last histogram
-  double want, least;  // weight before which a token is still taken by top_p; weight that min_p asks for
+  double want;       // weight before which a token is still taken by top_p
+  uint64_t least;    // weight that min_p asks for
   float xe;          // the edge: tokens above xe, and those equal to it up to index ie
   int ie;
 
-  // (x - m) / T; the maximum itself may be infinite.
-  __device__ __forceinline__ float gap(float v) const { return v == m ? 0.f : __fmul_rn(__fsub_rn(v, m), r); }
-  __device__ __forceinline__ uint64_t weigh(float g) const {  // g = NaN (an infinite gap times 1 / T = 0): nothing
-    const float e = expf(g);
-    return e > 0.f ? (uint64_t)__fmul_rn(e, kOne) : 0;
-  }
-  __device__ __forceinline__ uint64_t weight(float v) const { return weigh(gap(v)); }
+  __device__ __forceinline__ float gap(float v) const { return gap_of(v, m, r); }
+  __device__ __forceinline__ uint64_t weight(float v) const { return weight_of(v, m, r); }
   __device__ __forceinline__ bool above_edge(float v, int i) const { return v > xe || (v == xe && i <= ie); }
   __device__ __forceinline__ void set_edge(uint64_t o) {
     xe = value_of(o);
     ie = index_of(o);
   }
-  template <bool MASS>
-  __device__ __forceinline__ bool taken(uint64_t b) const {  // whether a token before which b lies is taken
-    return MASS ? b == 0 || (double)b < want : b < k;
-  }
+  // Whether a token before which b lies (weight, or tokens) is taken.
+  __device__ __forceinline__ bool taken(bool mass, uint64_t b) const { return mass ? b == 0 || (double)b < want : b < k; }
 
   __device__ __forceinline__ void sync() const {
     if (ranks > 1)
@@ -116,155 +238,227 @@ struct Sampler {
     else
       __syncthreads();
   }
-  // f(value, index) of this thread's tokens: each warp has a contiguous run of pieces, lanes interleaved.
+  __device__ __forceinline__ uint64_t sum(uint64_t v) const { return cta_reduce<false>(sh.wsum, v); }
+  __device__ __forceinline__ uint64_t most(uint64_t v) const { return cta_reduce<true>(sh.wsum, v); }
+  // Each warp has a contiguous run of pieces, its lanes interleaved.
   __device__ __forceinline__ void share(int& b, int& e) const {
     const int each = (pieces + kSampleWarps - 1) / kSampleWarps;
     b = min((int)(threadIdx.x >> 5) * each, pieces);
     e = min(b + each, pieces);
   }
-  __device__ __forceinline__ void piece(int c, float (&v)[E]) const {
+  // Bit j: f(value, index) of token j of piece c.
+  template <class F>
+  __device__ __forceinline__ uint32_t test(int c, F f) const {
     const uint4 u = reinterpret_cast<const uint4*>(x)[c];
     const T* t = reinterpret_cast<const T*>(&u);
+    uint32_t mask = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = to_f32(t[e]);
+    for (int j = 0; j < E; ++j)
+      if (f(to_f32(t[j]), base + c * E + j)) mask |= 1u << j;
+    return mask;
   }
+
+  // f(value, index, weight) of the kept tokens of this warp's share.  Few are kept as a rule: a thread marks its
+  // own first, then weighs those.
   template <class F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void each_kept(F f) const {
+    constexpr int kMark = 32 / E;  // pieces of a mask
     int b, e;
     share(b, e);
-#pragma unroll 2
-    for (int c = b + (threadIdx.x & 31); c < e; c += 32) {
-      float v[E];
-      piece(c, v);
+#pragma unroll 1
+    for (int c0 = b + (threadIdx.x & 31); c0 < e; c0 += 32 * kMark) {
+      uint32_t mask = 0;
 #pragma unroll
-      for (int j = 0; j < E; ++j) f(v[j], base + c * E + j);
+      for (int q = 0; q < kMark; ++q)
+        if (c0 + 32 * q < e) mask |= test(c0 + 32 * q, [&](float v, int i) { return above_edge(v, i); }) << (q * E);
+      while (mask) {
+        const int bit = __ffs((int)mask) - 1, i = (c0 + 32 * (bit / E)) * E + bit % E;
+        mask &= mask - 1;
+        const float v = to_f32(x[i]);
+        const uint64_t w = weigh(gap(v));
+        if (w >= least) f(v, base + i, w);
+      }
     }
   }
 
-  // One word of every CTA (its thread 0's), on every thread, combined in the order of the CTAs.
-  template <class F>
-  __device__ __forceinline__ uint64_t combine(uint64_t v, F f) {
+  // Two words of every CTA of the cluster (thread 0's), left in slot[flip].
+  __device__ __forceinline__ void exchange(uint64_t v, uint64_t w) {
     flip ^= 1;
-    if (ranks == 1) {
-      if (threadIdx.x == 0) sh.slot[flip][0] = v;
-    } else if (threadIdx.x < 32) {
+    if (threadIdx.x < 32) {
       v = __shfl_sync(0xffffffffu, v, 0);
-      if (threadIdx.x < ranks) *cg::this_cluster().map_shared_rank(&sh.slot[flip][rank], threadIdx.x) = v;
+      w = __shfl_sync(0xffffffffu, w, 0);
+      if (threadIdx.x < ranks) {
+        uint64_t* to = sh.slot[flip][rank];
+        if (ranks > 1) to = cg::this_cluster().map_shared_rank(to, threadIdx.x);
+        to[0] = v;
+        to[1] = w;
+      }
     }
     sync();
-    v = sh.slot[flip][0];
-    for (int c = 1; c < ranks; ++c) v = f(v, sh.slot[flip][c]);
-    return v;
   }
+  // Gathers the tokens with f(value, index) into every CTA's list, in no order.  Returns their number; a list
+  // is cut off at its length.
   template <class F>
-  __device__ __forceinline__ uint64_t reduce(uint64_t v, F f) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh.wsum[threadIdx.x >> 5] = v;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      v = sh.wsum[threadIdx.x];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __device__ __forceinline__ int gather(F f) {
+    listed ^= 1;
+    uint32_t* const count = &sh.count[listed];
+    int b, e;
+    share(b, e);
+#pragma unroll 1
+    for (int c = b + (threadIdx.x & 31); c < e; c += 32) {
+      uint32_t mask = test(c, f);
+      while (mask) {
+        const int i = c * E + __ffs((int)mask) - 1;
+        mask &= mask - 1;
+        const uint64_t o = order_of(to_f32(x[i]), base + i);
+#pragma unroll 1
+        for (int q = 0; q < ranks; ++q) {
+          const uint32_t at = atomicAdd(ranks > 1 ? cg::this_cluster().map_shared_rank(count, q) : count, 1u);
+          if (at < kSampleList) *(ranks > 1 ? cg::this_cluster().map_shared_rank(&sh.list[at], q) : &sh.list[at]) = o;
+        }
+      }
     }
-    return combine(v, f);
-  }
-  __device__ __forceinline__ uint64_t sum(uint64_t v) {
-    return reduce(v, [](uint64_t a, uint64_t b) { return a + b; });
-  }
-  __device__ __forceinline__ uint64_t largest(uint64_t v) {
-    return reduce(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+    sync();
+    const int n = (int)*(volatile uint32_t*)count;
+    __syncthreads();
+    if (threadIdx.x == 0) *count = 0;
+    return n;
   }
 
-  // ---- teams: the first warp, or the CTA
-  template <bool WARP>
-  __device__ __forceinline__ static void team_sync() {
-    if (WARP)
-      __syncwarp();
-    else
-      __syncthreads();
-  }
-  // Sum of what lies before this thread in the team; `all`: of the whole team.
-  template <bool WARP>
-  __device__ __forceinline__ uint64_t before(uint64_t v, uint64_t& all) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint64_t run = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
-    }
-    if (WARP) {
-      all = __shfl_sync(0xffffffffu, run, 31);
-      return run - v;
-    }
+  // A cleared histogram of f's tokens: f gives a token's step, or none (>= kSteps).
+  template <class F>
+  __device__ __forceinline__ void fill(bool mass, F f) {
+    hist ^= 1;
+    for (int i = threadIdx.x; i < kSteps; i += kSampleThreads) sh.lo[hist][i] = sh.hi[hist][i] = 0;
     __syncthreads();
-    if (lane == 31) sh.wsum[warp] = run;
-    __syncthreads();
-    if (warp == 0) {
-      uint64_t w = sh.wsum[lane], t = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t up = __shfl_up_sync(0xffffffffu, t, o);
-        if (lane >= o) t += up;
-      }
-      sh.wbase[lane] = t - w;
-      if (lane == 31) sh.all = t;
+    uint32_t* const lo = sh.lo[hist];
+    uint32_t* const hi = sh.hi[hist];
+#pragma unroll 4
+    for (int i = threadIdx.x; i < pieces * E; i += kSampleThreads) {
+      const float v = to_f32(x[i]), g = gap(v);
+      const uint32_t s = f(v, g, base + i);
+      if (s >= kSteps) continue;
+      uint64_t w = 1;
+      if (mass) w = weigh(g);
+      // the carry out of the low word is seen by the one thread that caused it, so the sum is exact
+      const uint32_t l = (uint32_t)w, was = atomicAdd(lo + s, l), h = (uint32_t)(w >> 32) + (was + l < l);
+      if (h) atomicAdd(hi + s, h);
     }
-    __syncthreads();
-    all = sh.all;
-    return sh.wbase[warp] + run - v;
   }
-  // Sorts list[0 .. n) to falling order.
-  template <bool WARP>
-  __device__ __noinline__ static void sort(uint64_t* list, int n) {
-    const int me = threadIdx.x;
-    constexpr int team = WARP ? 32 : kSampleThreads;
-    int size = 32;
-    while (size < n) size <<= 1;
-    for (int i = n + me; i < size; i += team) list[i] = 0;
-    team_sync<WARP>();
-    for (int h = 2; h <= size; h <<= 1) {
-      for (int j = h >> 1; j >= 32; j >>= 1) {
-        for (int t = me; t < size / 2; t += team) {
-          const int a = 2 * t - (t & (j - 1)), b = a + j;
-          const uint64_t u = list[a], v = list[b];
-          if ((u < v) == ((a & h) == 0)) {
-            list[a] = v;
-            list[b] = u;
-          }
-        }
-        team_sync<WARP>();
+  // Of the cluster's histogram: the last step, counted from the top, whose first token is taken.  `above`:
+  // what lies before it, at first what lies before step 0.  limit: top_p's is of this histogram's sum.
+  __device__ __forceinline__ uint32_t pick(bool mass, bool limit, uint64_t& above) {
+    if (threadIdx.x == 0) sh.pick = 0;
+    sync();
+    uint64_t v = 0;
+    if (threadIdx.x < kSteps) {
+#pragma unroll 1
+      for (int c = 0; c < ranks; ++c) {  // every CTA sums all: none has to tell the others
+        const SampleShared* o = ranks == 1 ? &sh : cg::this_cluster().map_shared_rank(&sh, c);
+        v += (uint64_t)o->hi[hist][threadIdx.x] << 32 | o->lo[hist][threadIdx.x];
       }
-      for (int t = me; t < size; t += team) {  // strides within a warp
-        uint64_t v = list[t];
-        for (int j = min(h >> 1, 16); j > 0; j >>= 1) {
-          const uint64_t u = __shfl_xor_sync(0xffffffffu, v, j);
-          const bool big = ((t & j) == 0) == ((t & h) == 0);  // this place takes the larger
-          v = (u > v) == big ? u : v;
-        }
-        list[t] = v;
-      }
-      if (h >= 32) team_sync<WARP>();  // smaller ones stay within a warp's 32 places
     }
-    team_sync<WARP>();
+    const Scan q = cta_scan(sh.wsum, v);
+    const uint64_t b = above + q.before;
+    total = q.all;
+    if (limit) want = (double)p * (double)total;
+    if (v && taken(mass, b)) atomicMax(&sh.pick, threadIdx.x);
+    __syncthreads();
+    const uint32_t s = sh.pick;
+    if (threadIdx.x == s) sh.word = b;
+    __syncthreads();
+    above = sh.word;
+    return s;
   }
-  // For a falling list of n tokens, `above` before them: how many are taken.
-  template <bool WARP, bool MASS>
-  __device__ __forceinline__ int taken_of_list(int n, uint64_t above) {
-    const int per = (n + (WARP ? 32 : kSampleThreads) - 1) / (WARP ? 32 : kSampleThreads), i0 = threadIdx.x * per;
-    uint64_t mine = 0, all;
-    for (int i = i0; i < min(i0 + per, n); ++i) mine += MASS ? weight(value_of(sh.list[i])) : 1;
-    uint64_t b = above + before<WARP>(mine, all);
+  // How many of a sorted list's n tokens are taken, `above` before them.
+  __device__ __forceinline__ int taken_of_sorted(bool mass, int n, uint64_t above) {
+    const int per = (n + kSampleThreads - 1) / kSampleThreads, i0 = threadIdx.x * per, i1 = min(i0 + per, n);
+    uint64_t mine = 0;
+    for (int i = i0; i < i1; ++i) mine += mass ? weight(value_of(sh.list[i])) : 1;
+    uint64_t b = above + cta_scan(sh.wsum, mine).before;
     uint32_t yes = 0;
-    for (int i = i0; i < min(i0 + per, n); ++i) {
-      yes += taken<MASS>(b);
-      b += MASS ? weight(value_of(sh.list[i])) : 1;
+    for (int i = i0; i < i1; ++i) {
+      yes += taken(mass, b);
+      b += mass ? weight(value_of(sh.list[i])) : 1;
     }
-    (void)before<WARP>(yes, all);
-    return (int)all;
+    return (int)sum(yes);
   }
+  // The edge within a list of n tokens with `above` before them.
+  __device__ __forceinline__ void edge_of_list(bool mass, int n, uint64_t above) {
+    if (n <= kShortList) {
+      const Place q = place_of(sh, n, m, r);
+      const bool keep = q.t >= 0 && taken(mass, above + (mass ? q.weight_before : q.count_before));
+      set_edge(~most(keep ? ~q.order : 0));
+    } else {
+      cta_sort(sh.list, n);
+      set_edge(sh.list[max(taken_of_sorted(mass, n, above), 1) - 1]);
+    }
+    __syncthreads();  // the list may be written again
+  }
+  // The edge among the tokens of step s1 where they are too many for a list: by 512ths of the step, and where
+  // those of one are too many as well, by halving: the lowest number above which little enough lies.
+  __device__ __noinline__ void refine(bool mass, uint32_t s1, uint64_t above) {
+    const float from = -0.0625f * (float)s1, to = fmaxf(from - 0.0625f, kFar);
+    fill(mass, [&](float v, float g, int i) { return g <= from && g > to && above_edge(v, i) ? whole(g * -8192.f) % kSteps : kSteps; });
+    const uint32_t s2 = s1 * kSteps + pick(mass, false, above);
+    auto in = [&](float v, int i) {
+      const float g = gap(v);
+      return g <= from && g > to && above_edge(v, i) && whole(g * -8192.f) == s2;
+    };
+    const int n = gather(in);
+    if (n <= kSampleList) return edge_of_list(mass, n, above);
+    uint64_t low = ~0ull, high = 0;
+    for (int i = threadIdx.x; i < pieces * E; i += kSampleThreads) {
+      const float v = to_f32(x[i]);
+      if (!in(v, base + i)) continue;
+      low = min(low, order_of(v, base + i));
+      high = max(high, order_of(v, base + i));
+    }
+    low = most(~low);
+    high = most(high);
+    exchange(low, high);
+    for (int c = 0; c < ranks; ++c) {
+      low = max(low, sh.slot[flip][c][0]);
+      high = max(high, sh.slot[flip][c][1]);
+    }
+    low = ~low;
+    while (low < high) {
+      const uint64_t mid = low + (high - low) / 2;
+      uint64_t b = 0;
+      for (int i = threadIdx.x; i < pieces * E; i += kSampleThreads) {
+        const float v = to_f32(x[i]);
+        if (in(v, base + i) && order_of(v, base + i) > mid) b += mass ? weight(v) : 1;
+      }
+      exchange(sum(b), 0);
+      b = above;
+      for (int c = 0; c < ranks; ++c) b += sh.slot[flip][c][0];
+      if (taken(mass, b))
+        high = mid;
+      else
+        low = mid + 1;
+    }
+    set_edge(low);
+  }
+  // The edge of top_k (by tokens) or top_p (by weight) among the tokens above the present one.
+  __device__ __forceinline__ void find_edge(bool mass) {
+    uint64_t above = 0;
+    fill(mass, [&](float v, float g, int i) { return g > kFar && above_edge(v, i) ? whole(g * -16.f) : kSteps; });
+    const uint32_t s1 = pick(mass, mass, above);
+    const float from = -0.0625f * (float)s1, to = fmaxf(from - 0.0625f, kFar);
+    const int n = gather([&](float v, int i) {
+      const float g = gap(v);
+      return g <= from && g > to && above_edge(v, i);
+    });
+    if (n <= kSampleList) return edge_of_list(mass, n, above);
+    Sampler rare = *this;  // a copy, so that this one can stay in registers
+    rare.refine(mass, s1, above);
+    flip = rare.flip;
+    hist = rare.hist;
+    listed = rare.listed;
+    xe = rare.xe;
+    ie = rare.ie;
+  }
+
   __device__ __forceinline__ uint64_t aim(float u, uint64_t z) const {
     return u > 0.f ? min((uint64_t)((double)u * (double)z), z - 1) : 0;
   }
@@ -274,43 +468,61 @@ struct Sampler {
     if (a.logprob) a.logprob[rw] = gap(v) - logf(__fdiv_rn((float)(double)z, kOne));
   }
   // Everything from a list that holds the top k tokens: the edge of top_p, the kept weight and the id.
-  template <bool WARP>
-  __device__ __forceinline__ void finish_list(const SampleArgs& a, int rw, int n) {
-    constexpr int team = WARP ? 32 : kSampleThreads;
-    const int me = threadIdx.x;
-    sort<WARP>(sh.list, n);
+  __device__ __forceinline__ uint64_t finish_short(const SampleArgs& a, int rw, float u, int n) {
+    Place q = place_of(sh, n, m, r);
+    bool keep = q.t >= 0 && q.count_before < k;
+    if (!(p >= 1.f)) {
+      want = (double)p * (double)sum(keep ? q.w : 0);
+      keep = keep && taken(true, q.weight_before);
+    }
+    if (a.probs) set_edge(~most(keep ? ~q.order : 0));
+    if (!keep || q.w < least) q.w = 0;
+    const uint64_t z = sum(q.w), at = aim(u, z);
+    const int kept = __syncthreads_count(q.w > 0);
+    if (q.t >= 0 && (threadIdx.x & (q.team - 1)) == 0) sh.weights[q.t] = q.w;
+    __syncthreads();
+    uint64_t b = 0;
+    for (int j = threadIdx.x & (q.team - 1); j < n; j += q.team)
+      if ((uint32_t)sh.list[j] > (uint32_t)q.order) b += sh.weights[j];  // lower indexes
+    for (int o = q.team >> 1; o > 0; o >>= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
+    if (rank == 0 && b <= at && at < b + q.w) answer(a, rw, index_of(q.order), value_of(q.order), z, kept);
+    return z;
+  }
+  __device__ __forceinline__ uint64_t finish_long(const SampleArgs& a, int rw, float u, int n) {
+    cta_sort(sh.list, n);
     int c = (int)min((uint64_t)n, k);
     if (!(p >= 1.f)) {
-      uint64_t total = 0, all;
-      for (int i = me; i < c; i += team) total += weight(value_of(sh.list[i]));
-      (void)before<WARP>(total, all);
-      want = (double)p * (double)all;
-      c = taken_of_list<WARP, true>(c, 0);
+      uint64_t all = 0;
+      for (int i = threadIdx.x; i < c; i += kSampleThreads) all += weight(value_of(sh.list[i]));
+      want = (double)p * (double)sum(all);
+      c = taken_of_sorted(true, c, 0);
     }
-    if (me == 0) sh.word[0] = sh.list[c - 1];
+    set_edge(sh.list[c - 1]);
+    __syncthreads();
     // the kept ones by rising index: sorted by (~index, key)
-    team_sync<WARP>();
-    for (int i = me; i < c; i += team) {
+    for (int i = threadIdx.x; i < c; i += kSampleThreads) {
       const uint64_t v = sh.list[i];
       sh.list[i] = v << 32 | v >> 32;
     }
-    team_sync<WARP>();
-    sort<WARP>(sh.list, c);
-    const int per = (c + team - 1) / team, i0 = me * per, i1 = min(i0 + per, c);
-    uint64_t mass = 0, some = 0, z, kept;
+    __syncthreads();
+    cta_sort(sh.list, c);
+    const int per = (c + kSampleThreads - 1) / kSampleThreads, i0 = threadIdx.x * per, i1 = min(i0 + per, c);
+    uint64_t mass = 0, some = 0;
     for (int i = i0; i < i1; ++i) {
       const uint64_t w = weight(of_key((uint32_t)sh.list[i]));
-      if (w == 0 || (double)w < least) continue;
+      if (w < least) continue;
       mass += w;
-      ++some;
+      some += w > 0;
     }
-    (void)before<WARP>(some, kept);
-    uint64_t b = before<WARP>(mass, z);
-    const uint64_t at = aim(a.u[rw], z);
-    if (b <= at && at < b + mass) {
+    const uint64_t kept = sum(some);
+    const Scan q = cta_scan(sh.wsum, mass);
+    const uint64_t z = q.all, at = aim(u, z);
+    uint64_t b = q.before;
+    if (rank == 0 && b <= at && at < b + mass) {
       for (int i = i0; i < i1; ++i) {
-        const uint64_t v = sh.list[i], w = weight(of_key((uint32_t)v));
-        if (w == 0 || (double)w < least) continue;
+        const uint64_t v = sh.list[i];
+        uint64_t w = weight(of_key((uint32_t)v));
+        if (w < least) w = 0;
         if (at < b + w) {
           answer(a, rw, index_of(v >> 32), of_key((uint32_t)v), z, kept);
           break;
@@ -318,149 +530,7 @@ struct Sampler {
         b += w;
       }
     }
-    if (me == 0) sh.word[1] = z;
-  }
-
-  // Gathers the tokens with f(value, index) into the first CTA's list, in no order.  Returns their number;
-  // the list is cut off at its length.  sh.count of the first CTA is 0 before.
-  template <class F>
-  __device__ __forceinline__ int gather(F f) {
-    uint64_t* list = sh.list;
-    uint32_t* count = &sh.count;
-    if (ranks > 1) {
-      list = cg::this_cluster().map_shared_rank(list, 0);
-      count = cg::this_cluster().map_shared_rank(count, 0);
-    }
-    each([&](float v, int i) {
-      if (!f(v, i)) return;
-      const uint32_t at = atomicAdd(count, 1u);
-      if (at < kSampleList) list[at] = order_of(v, i);
-    });
-    sync();
-    const int n = (int)*(volatile uint32_t*)count;
-    sync();
-    if (rank == 0 && threadIdx.x == 0) sh.count = 0;
-    return n;
-  }
-
-  // Histogram step: adds v to the 64-bit sum of step s.  The carry out of the low word is seen by the one
-  // thread that caused it, so the sum is exact.
-  __device__ __forceinline__ void add(uint32_t s, uint64_t v) {
-    const uint32_t l = (uint32_t)v;
-    const uint32_t was = atomicAdd(&sh.lo[s], l);
-    const uint32_t h = (uint32_t)(v >> 32) + (was + l < l);
-    if (h) atomicAdd(&sh.hi[s], h);
-  }
-  __device__ __forceinline__ void clear() {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kSteps; i += kSampleThreads) sh.lo[i] = sh.hi[i] = 0;
-    __syncthreads();
-  }
-  // Of the cluster's histogram: the last step, counted from the top, whose first token is taken.  `above`:
-  // what lies before it, at first what lies before step 0.  TOTAL: top_p's limit is of this histogram's sum.
-  template <bool MASS, bool TOTAL>
-  __device__ __forceinline__ uint32_t pick(uint64_t& above) {
-    sync();
-    uint64_t v = 0, all;
-    if (threadIdx.x < kSteps) {
-      for (int c = 0; c < ranks; ++c) {  // every CTA sums all: none has to tell the others
-        const SampleShared* o = ranks == 1 ? &sh : cg::this_cluster().map_shared_rank(&sh, c);
-        v += (uint64_t)o->hi[threadIdx.x] << 32 | o->lo[threadIdx.x];
-      }
-    }
-    if (threadIdx.x == 0) sh.pick = 0;
-    const uint64_t b = above + before<false>(v, all);
-    total = all;
-    if (TOTAL) want = (double)p * (double)all;
-    if (v && taken<MASS>(b)) atomicMax(&sh.pick, threadIdx.x);
-    __syncthreads();
-    const uint32_t s = sh.pick;
-    if (threadIdx.x == s) sh.word[1] = b;
-    sync();  // also: the other CTAs have read this one's sums
-    above = sh.word[1];
-    return s;
-  }
-  // The edge of top_k (by tokens) or top_p (by weight) among the tokens above the present one.
-  template <bool MASS>
-  __device__ __forceinline__ void find_edge() {
-    uint64_t above = 0;
-    clear();
-    each([&](float v, int i) {
-      const float g = gap(v);
-      if (!(g > kFar) || !above_edge(v, i)) return;
-      const uint32_t s = (uint32_t)(g * -16.f);
-      if (MASS) {
-        const uint64_t w = weigh(g);
-        if (w) add(s, w);
-      } else {
-        atomicAdd(&sh.lo[s], 1u);
-      }
-    });
-    const uint32_t s1 = pick<MASS, MASS>(above);
-    const float from = -0.0625f * (float)s1, to = from - 0.0625f;
-    auto in1 = [&](float v, int i) {
-      const float g = gap(v);
-      return g <= from && g > to && g > kFar && above_edge(v, i);
-    };
-    int n = gather(in1);
-    if (n > kSampleList) {
-      clear();
-      each([&](float v, int i) {
-        if (!in1(v, i)) return;
-        const float g = gap(v);
-        const uint32_t s = (uint32_t)(g * -8192.f) % kSteps;
-        if (MASS) {
-          const uint64_t w = weigh(g);
-          if (w) add(s, w);
-        } else {
-          atomicAdd(&sh.lo[s], 1u);
-        }
-      });
-      const uint32_t s2 = s1 * kSteps + pick<MASS, false>(above);
-      auto in2 = [&](float v, int i) { return in1(v, i) && (uint32_t)(gap(v) * -8192.f) == s2; };
-      n = gather(in2);
-      if (n > kSampleList) return halve<MASS>(above, in2);
-    }
-    if (rank == 0) {
-      if (n <= kWarpList) {
-        if (threadIdx.x < 32) {
-          sort<true>(sh.list, n);
-          const int c = taken_of_list<true, MASS>(n, above);
-          if (threadIdx.x == 0) sh.word[0] = sh.list[max(c, 1) - 1];
-        }
-      } else {
-        sort<false>(sh.list, n);
-        const int c = taken_of_list<false, MASS>(n, above);
-        if (threadIdx.x == 0) sh.word[0] = sh.list[max(c, 1) - 1];
-      }
-    }
-    sync();
-    set_edge(ranks == 1 ? sh.word[0] : *cg::this_cluster().map_shared_rank(&sh.word[0], 0));
-    sync();
-  }
-  // The lowest number above which little enough lies, among the tokens of `in`.
-  template <bool MASS, class F>
-  __device__ __forceinline__ void halve(uint64_t above, F in) {
-    uint64_t low = ~0ull, high = 0;
-    each([&](float v, int i) {
-      if (!in(v, i)) return;
-      low = min(low, order_of(v, i));
-      high = max(high, order_of(v, i));
-    });
-    low = ~largest(~low);
-    high = largest(high);
-    while (low < high) {
-      const uint64_t mid = low + (high - low) / 2;
-      uint64_t b = 0;
-      each([&](float v, int i) {
-        if (in(v, i) && order_of(v, i) > mid) b += MASS ? weight(v) : 1;
-      });
-      if (taken<MASS>(above + sum(b)))
-        high = mid;
-      else
-        low = mid + 1;
-    }
-    set_edge(low);
+    return z;
   }
 };
 
@@ -474,45 +544,50 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   S s{sh, reinterpret_cast<T*>(smem + sizeof(SampleShared))};
   s.ranks = gridDim.x;
   s.rank = blockIdx.x;
-  s.flip = 0;
+  s.flip = s.hist = s.listed = 0;
+  // no CTA's memory is written before it runs: the wait comes with the first exchange
+  if (s.ranks > 1) cg::this_cluster().barrier_arrive();
   const int first = min(s.rank * a.part, a.vocab), n = min(a.part, a.vocab - first);  // this CTA's tokens
   const T* const row = static_cast<const T*>(a.x) + (int64_t)rw * a.row_stride + first;
   const int lead = (int)((uintptr_t)row & 15) / (int)sizeof(T);
   s.base = first - lead;
   s.pieces = (lead + n + E - 1) / E;
   float* const probs = a.probs ? a.probs + (int64_t)rw * a.vocab : nullptr;
-  if (tid == 0) sh.count = 0;
-  for (int i = tid; i < kSteps; i += kSampleThreads) sh.lo[i] = sh.hi[i] = 0;
-  // ---- the row, and every thread's maximum
+  const float min_p = a.min_p ? a.min_p[rw] : 0.f, t = a.temperature ? a.temperature[rw] : 1.f, u = a.u[rw];
+  const int top_k = a.top_k ? a.top_k[rw] : 0;
+  s.p = a.top_p ? a.top_p[rw] : 1.f;
+  if (tid < 2) sh.count[tid] = 0;
+  for (int i = tid; i < kSteps; i += kSampleThreads) sh.lo[0][i] = sh.hi[0][i] = 0;
+  // ---- the row, and every thread's maximum; the first and last piece, which may hold less, by token
   float mine = -INFINITY;
   {
     const uint4* const from = reinterpret_cast<const uint4*>(row - lead);
+    const bool begins = lead > 0 || n < E, cut[2] = {begins, (lead + n) % E != 0 && !(begins && s.pieces == 1)};
     int b, e;
     s.share(b, e);
 #pragma unroll 4
     for (int c = b + lane; c < e; c += 32) {
-      uint4 u;
-      if (c * E >= lead && (c + 1) * E <= lead + n) {
-        u = __ldcs(from + c);
-      } else {  // the row ends within this piece: token by token
-        T v[E];
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const int i = c * E + j - lead;
-          v[j] = i >= 0 && i < n ? row[i] : from_f32<T>(-INFINITY);
-        }
-        u = *reinterpret_cast<const uint4*>(v);
-      }
+      if ((c == 0 && cut[0]) || (c == s.pieces - 1 && cut[1])) continue;
+      const uint4 u = __ldcs(from + c);
       reinterpret_cast<uint4*>(s.x)[c] = u;
       const T* t = reinterpret_cast<const T*>(&u);
 #pragma unroll
       for (int j = 0; j < E; ++j) mine = fmaxf(mine, to_f32(t[j]));  // not NaN's
     }
+    if (tid < 2 * E && cut[tid / E]) {
+      const int at = (tid < E ? 0 : s.pieces - 1) * E + tid % E, i = at - lead;
+      const T v = i >= 0 && i < n ? row[i] : from_f32<T>(-INFINITY);
+      s.x[at] = v;
+      mine = fmaxf(mine, to_f32(v));
+    }
   }
-  if (s.ranks > 1) s.sync();  // every CTA of the cluster runs before its memory is written
-  s.m = of_key((uint32_t)s.largest(key_of(mine)));
-  const float min_p = a.min_p ? a.min_p[rw] : 0.f, t = a.temperature ? a.temperature[rw] : 1.f;
-  s.least = (double)min_p * (double)kOne;
+  if (s.ranks > 1) cg::this_cluster().barrier_wait();
+  uint64_t top = s.most(key_of(mine));
+  if (s.ranks > 1) {
+    s.exchange(top, 0);
+    for (int c = 0; c < s.ranks; ++c) top = max(top, sh.slot[s.flip][c][0]);
+  }
+  s.m = of_key((uint32_t)top);
   if (s.m == -INFINITY || min_p > 1.f) {  // no token to draw
     if (s.rank == 0 && tid == 0) {
       a.id[rw] = -1;
@@ -521,142 +596,120 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     }
     if (probs)
       for (int i = tid; i < n; i += kSampleThreads) probs[first + i] = 0.f;
-    if (s.ranks > 1) s.sync();  // no CTA leaves while another may still write its words
     return;
   }
+  s.least = min_p > 0.f ? (uint64_t)ceil((double)min_p * (double)kOne) : 0;  // weights are whole numbers
   const bool greedy = !(t > 0.f);
-  s.r = greedy ? 1.f : __fdiv_rn(1.f, t);
-  int k = greedy ? 1 : (a.top_k ? a.top_k[rw] : 0);
+  s.r = greedy ? 1.f : fminf(fmaxf(__fdiv_rn(1.f, t), 1e-37f), 1e38f);  // not 0 for an infinite T, nor infinite for a tiny one
+  if (s.m == INFINITY) {  // infinite logits are all the row has: 0 among -inf
+    for (int i = tid; i < s.pieces * E; i += kSampleThreads) s.x[i] = from_f32<T>(to_f32(s.x[i]) == INFINITY ? 0.f : -INFINITY);
+    s.m = 0.f;
+    mine = mine == INFINITY ? 0.f : -INFINITY;
+    __syncthreads();
+  }
+  int k = greedy ? 1 : top_k;
   if (k <= 0 || k > a.vocab) k = a.vocab;
   s.k = k;
-  s.p = a.top_p ? a.top_p[rw] : 1.f;
-  s.xe = -INFINITY;  // every token that weighs anything
-  s.ie = -1;
+  s.xe = -INFINITY;  // every token above -inf, and none of what surrounds the part (its indexes may be below 0)
+  s.ie = INT_MIN;
 
   // ---- the edge: tokens at or above it are kept
-  bool listed = false;  // the first CTA's list holds the top k
-  if (k < a.vocab && k <= kSampleMaxK) {
-    // the step in which the k-th largest of the threads' maxima lies, and all that is above it
-    float to = 0.f;
-    if (k == 1) {
-      to = -1e-30f;
-    } else {
-      const float g = s.gap(mine);
-      if (g > kFar) atomicAdd(&sh.lo[(uint32_t)(g * -16.f)], 1u);
-      uint64_t above = 0;
-      to = -0.0625f * (float)(s.template pick<false, false>(above) + 1);
-      if (s.total < s.k) to = kFar;  // fewer threads than k hold a token of weight
-    }
-    const int c = s.gather([&](float v, int) {
-      const float g = s.gap(v);
-      return g > to && g > kFar;
-    });
-    if (c <= kSampleList) {
-      listed = true;
-      if (s.rank == 0) {
-        if (c > kWarpList)
-          s.template finish_list<false>(a, rw, c);
-        else if (tid < 32)
-          s.template finish_list<true>(a, rw, c);
+  bool done = false;
+  uint64_t z = 0;
+  if (k == 1) {  // the first of the tokens that are equal to the maximum
+    int b, e;
+    s.share(b, e);
+    uint32_t at = ~0u;
+    for (int c = b + lane; c < e; c += 32) {
+      const uint32_t mask = s.test(c, [&](float v, int) { return v == s.m; });
+      if (mask) {
+        at = (uint32_t)(s.base + c * E + __ffs((int)mask) - 1);
+        break;
       }
     }
-  }
-  uint64_t z = 0;
-  if (listed) {
-    if (probs) {
-      s.sync();
-      const uint64_t* word = s.ranks == 1 ? sh.word : cg::this_cluster().map_shared_rank(sh.word, 0);
-      s.set_edge(word[0]);
-      z = word[1];
+    uint64_t id = s.most(~at);
+    if (s.ranks > 1) {
+      s.exchange(id, 0);
+      for (int c = 0; c < s.ranks; ++c) id = max(id, sh.slot[s.flip][c][0]);
     }
-  } else {
-    if (k < a.vocab) s.template find_edge<false>();
-    if (!(s.p >= 1.f)) s.template find_edge<true>();
-    // ---- the kept weight Z, and the token in index order where the running weight passes floor(u Z).  Few
-    // tokens are kept as a rule: a thread marks its own first, then weighs those.
-    auto kept_weight = [&](float v, int i) -> uint64_t {
-      if (!s.above_edge(v, i)) return 0;
-      const uint64_t w = s.weight(v);
-      return (double)w >= s.least ? w : 0;
-    };
+    s.xe = s.m;
+    s.ie = (int)~(uint32_t)id;
+    z = (uint64_t)1 << 40;
+    if (s.rank == 0 && tid == 0) s.answer(a, rw, s.ie, s.m, z, 1);
+    done = true;
+  } else if (k < a.vocab && k <= kSampleMaxK) {
+    // the step in which the k-th largest of the threads' maxima lies, and all that is above it
+    const float g = s.gap(mine);
+    if (g > kFar) atomicAdd(&sh.lo[0][whole(g * -16.f)], 1u);
+    uint64_t above = 0;
+    float to = fmaxf(-0.0625f * (float)(s.pick(false, false, above) + 1), kFar);
+    if (s.total < s.k) to = kFar;  // fewer threads than k hold a token of weight
+    const int c = s.gather([&](float v, int) { return s.gap(v) > to; });
+    done = c <= kSampleList;
+    if (done) z = c <= kShortList ? s.finish_short(a, rw, u, c) : s.finish_long(a, rw, u, c);
+  }
+  if (!done) {
+#pragma unroll 1
+    for (int by = 0; by < 2; ++by)
+      if (by ? !(s.p >= 1.f) : k < a.vocab) s.find_edge(by);
+    // ---- the kept weight Z, and the token in index order where the running weight passes floor(u Z)
     int b, e;
     s.share(b, e);
     uint64_t v = 0, some = 0;
-    constexpr int kMark = 32 / E;  // pieces of a mask
-    for (int c0 = b + lane; c0 < e; c0 += 32 * kMark) {
-      uint32_t mask = 0;
-#pragma unroll
-      for (int q = 0; q < kMark; ++q) {
-        const int c = c0 + 32 * q;
-        if (c >= e) break;
-        float f[E];
-        s.piece(c, f);
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (s.above_edge(f[j], s.base + c * E + j)) mask |= 1u << (q * E + j);
-      }
-      while (mask) {
-        const int bit = __ffs((int)mask) - 1;
-        mask &= mask - 1;
-        const uint64_t w = s.weight(to_f32(s.x[(c0 + 32 * (bit / E)) * E + bit % E]));
-        if ((double)w < s.least) continue;
-        v += w;
-        some += w > 0;
-      }
+    s.each_kept([&](float, int, uint64_t w) {
+      v += w;
+      some += w > 0;
+    });
+    const Scan q = cta_scan(sh.wsum, v);
+    uint64_t kept = s.sum(some), ahead = q.before;
+    s.exchange(q.all, kept);
+    kept = 0;
+    for (int c = 0; c < s.ranks; ++c) {
+      if (c < s.rank) ahead += sh.slot[s.flip][c][0];
+      z += sh.slot[s.flip][c][0];
+      kept += sh.slot[s.flip][c][1];
     }
-    const uint64_t kept = s.sum(some);
-    uint64_t all;
-    uint64_t ahead = s.template before<false>(v, all);
-    z = s.combine(all, [](uint64_t x, uint64_t y) { return x + y; });
-    for (int c = 0; c < s.rank; ++c) ahead += sh.slot[s.flip][c];
     ahead = __shfl_sync(0xffffffffu, ahead, 0);  // before this warp's share
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    uint64_t aim = s.aim(a.u[rw], z);
-    if (ahead <= aim && aim < ahead + v) {  // one warp of one CTA: the place in its share
+    uint64_t aim = s.aim(u, z);
+    if (ahead <= aim && aim < ahead + warp_add(v)) {  // one warp of one CTA: the place in its share
       aim -= ahead;
+#pragma unroll 1
       for (int c = b; c < e; c += 32) {
-        float f[E];
-        uint64_t w[E], own = 0;
-#pragma unroll
-        for (int j = 0; j < E; ++j) w[j] = 0;
+        auto kept_weight = [&](int j) -> uint64_t {
+          const int i = (c + lane) * E + j;
+          const float f = to_f32(s.x[i]);
+          const uint64_t w = s.above_edge(f, s.base + i) ? s.weight(f) : 0;
+          return w < s.least ? 0 : w;
+        };
+        uint64_t own = 0;
         if (c + lane < e) {
-          s.piece(c + lane, f);
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            w[j] = kept_weight(f[j], s.base + (c + lane) * E + j);
-            own += w[j];
-          }
+#pragma unroll 1
+          for (int j = 0; j < E; ++j) own += kept_weight(j);
         }
-        uint64_t sum;
-        uint64_t before = s.template before<true>(own, sum);
-        if (aim < sum) {
-          if (before <= aim && aim < before + own) {
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-              if (before <= aim && aim < before + w[j]) s.answer(a, rw, s.base + (c + lane) * E + j, f[j], z, kept);
-              before += w[j];
-            }
-          }
-          break;
+        const Scan in = warp_scan(own);
+        if (aim >= in.all) {
+          aim -= in.all;
+          continue;
         }
-        aim -= sum;
+        if (in.before <= aim && aim < in.before + own) {
+          aim -= in.before;
+          int j = 0;
+          for (uint64_t w; aim >= (w = kept_weight(j)); ++j) aim -= w;
+          const int i = (c + lane) * E + j;
+          s.answer(a, rw, s.base + i, to_f32(s.x[i]), z, kept);
+        }
+        break;
       }
     }
   }
-  if (probs) {
-    const float zf = (float)z;
-    for (int i = tid; i < n; i += kSampleThreads) {
-      const float v = to_f32(s.x[lead + i]);
-      float q = 0.f;
-      if (s.above_edge(v, first + i)) {
-        const uint64_t w = s.weight(v);
-        if ((double)w >= s.least) q = __fdiv_rn((float)w, zf);
-      }
-      probs[first + i] = q;
-    }
+  if (probs) {  // nothing for all, then their shares for the few that are kept
+#pragma unroll 4
+    for (int i = tid; i < n; i += kSampleThreads) probs[first + i] = 0.f;
+    __syncthreads();
+    const float share = __fdiv_rn(1.f, (float)z);
+    s.each_kept([&](float, int i, uint64_t w) { probs[i] = (float)w * share; });
   }
-  if (s.ranks > 1) s.sync();  // no CTA leaves while another may still read or write its words
+  if (s.ranks > 1) s.sync();  // no CTA leaves while another may still read its histogram
 }
 
 // Opt in to the shared memory, and to clusters of 16, once per kernel and device.
@@ -682,6 +735,7 @@ int launch_sample(SampleArgs a, int rows, cudaStream_t st) {
   int ranks = 1;
   while (ranks < kMaxCluster && ((int64_t)ranks * room < a.vocab || ((int64_t)rows * ranks * 2 <= sms && a.vocab / (2 * ranks) >= 4096)))
     ranks *= 2;
+  if (const char* v = getenv("SR")) ranks = std::max(ranks, atoi(v));
   a.part = ((a.vocab + ranks - 1) / ranks + 31) / 32 * 32;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ranks, rows);
