@@ -5,8 +5,13 @@
 //
 // for the pairs (a, b) = (i, i + rope_dim / 2) or (2 i, 2 i + 1), c and s the table row of the position.
 // A few operations per element: bound by the bytes read and written, or by launch latency for few rows.
-// One warp takes one head of one row: it normalises into shared memory, where each lane finds the
-// partners of its elements whatever the layout and rope_dim.
+// A lane holds 8 neighbouring elements of a head (one or two 16-byte accesses), as many lanes as the head
+// needs share it, and a warp walks several heads of one token, so that the token's position, page and
+// table row are looked up once.  The norm's sum is a shuffle among the lanes of the head.  Pairs (2 i,
+// 2 i + 1) lie within a lane; pairs (i, i + rope_dim / 2) are exchanged by shuffles where rope_dim / 2 is
+// whole lanes, through shared memory otherwise.
+#include <algorithm>
+
 #include "device_common.cuh"
 #include "paged.cuh"
 
@@ -16,6 +21,7 @@ namespace {
 using namespace paged;
 
 constexpr int kRopeWarps = 4;
+enum RopePairs { kNoPairs, kAdjacent, kHalvesByLane, kAnyPairs };  // how a lane finds the partners of its elements
 
 struct RopeArgs {
   void *k, *v;
@@ -30,76 +36,168 @@ struct RopeArgs {
   float eps;
   const float *cs, *sn;
   int n_pos, rope_dim, interleaved;
+  int splits;  // warps of a token
   void* q;
   int64_t q_stride;
 };
 
-template <class A, class C>
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  uint4 u[sizeof(T) == 4 ? 2 : 1];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(u) / 16); ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  const T* e = reinterpret_cast<const T*>(u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  T e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
+}
+
+// LANES: lanes of a head, a power of two with 8 LANES >= head_dim.
+template <class A, class C, int LANES, RopePairs PAIRS>
 __global__ void __launch_bounds__(kRopeWarps * 32) rope_append_kernel(const RopeArgs a) {
-  __shared__ float y[kRopeWarps][256];
+  __shared__ float staged[PAIRS == kAnyPairs ? kRopeWarps : 1][PAIRS == kAnyPairs ? 256 : 1];
+  constexpr int kHeads = 32 / LANES;  // heads of a warp at a time
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t unit = (int64_t)blockIdx.x * kRopeWarps + warp;
-  const int per_tok = a.n_heads + 2 * a.n_kv;
-  const int64_t t = unit / per_tok;
+  const int64_t t = unit / a.splits;
   if (t >= a.n_tok) return;
-  const int h = (int)(unit - t * per_tok);
   const int seq = a.seq ? a.seq[t] : (int)t;
-  if (seq < 0) return;  // padding
   const int pos = a.pos[t];
+  const int per_tok = a.n_heads + 2 * a.n_kv, group = lane / LANES, d = lane % LANES * 8;
+  const int step = a.splits * kHeads, h0 = (int)(unit - t * a.splits) * kHeads + group;
+  const A* const x = static_cast<const A*>(a.qkv) + t * a.row_stride + d;
+  A* const q = static_cast<A*>(a.q) + t * a.q_stride + d;
+  const bool mine = d < a.dim;
+  // the first head's elements travel while the page is looked up
+  float v[8];
+  if (mine && h0 < per_tok && seq >= 0) load8(x + (int64_t)h0 * a.dim, v);
+  if (seq < 0) return;  // padding
   const int pg = pos / a.page_len;
   int page = -1;
   if (seq < a.n_seq && pos >= 0 && pg < a.table_stride && (pos < a.n_pos || a.rope_dim == 0))
-    page = a.table[(int64_t)seq * a.table_stride + pg];
-  const bool good = page >= 0 && page < a.n_pages;
-  const A* x = static_cast<const A*>(a.qkv) + t * a.row_stride + (int64_t)h * a.dim;
-  const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
-  if (!good) {
-    if (is_q) {
-      A* out = static_cast<A*>(a.q) + t * a.q_stride + (int64_t)h * a.dim;
-      for (int d = lane; d < a.dim; d += 32) out[d] = from_f32<A>(__int_as_float(0x7FC00000));
-    }
-    return;
-  }
-  const float* gain = is_q ? a.q_gain : (is_v ? nullptr : a.k_gain);
-  float ss = 0.f;
-  for (int d = lane; d < a.dim; d += 32) {
-    const float f = to_f32(x[d]);
-    y[warp][d] = f;
-    ss = fmaf(f, f, ss);
-  }
-  if (gain) {
-    const float r = sqrtf(warp_sum(ss) / (float)a.dim + a.eps);
-    for (int d = lane; d < a.dim; d += 32) y[warp][d] = y[warp][d] / r * gain[d];
-  }
-  __syncwarp();
-  C* kv = nullptr;
-  if (!is_q) {
-    const int hk = h - a.n_heads - (is_v ? a.n_kv : 0);
-    kv = static_cast<C*>(is_v ? a.v : a.k) + page * a.page_stride + hk * a.head_stride +
-         (int64_t)(pos - pg * a.page_len) * a.pos_stride;
-  }
-  A* out = static_cast<A*>(a.q) + t * a.q_stride + (int64_t)h * a.dim;
+    page = __ldg(a.table + (int64_t)seq * a.table_stride + pg);
+  const bool good = (unsigned)page < (unsigned)a.n_pages;
   const int half = a.rope_dim >> 1;
-  for (int d = lane; d < a.dim; d += 32) {
-    float f = y[warp][d];
-    if (!is_v && d < a.rope_dim) {
-      const int i = a.interleaved ? d >> 1 : (d < half ? d : d - half);
-      const bool second = a.interleaved ? d & 1 : d >= half;
-      const float p = y[warp][a.interleaved ? d ^ 1 : (second ? d - half : d + half)];
-      const float c = a.cs[(int64_t)pos * half + i], s = a.sn[(int64_t)pos * half + i];
-      f = second ? fmaf(f, c, p * s) : fmaf(f, c, -(p * s));
+  float c[8], s[8];  // of this lane's elements
+  if constexpr (PAIRS == kAdjacent || PAIRS == kHalvesByLane) {
+    if (good && d < a.rope_dim) {
+      constexpr int N = PAIRS == kAdjacent ? 4 : 8;
+      const int64_t at = (int64_t)pos * half + (PAIRS == kAdjacent ? d / 2 : (d < half ? d : d - half));
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        *reinterpret_cast<float4*>(c + i) = __ldg(reinterpret_cast<const float4*>(a.cs + at + i));
+        *reinterpret_cast<float4*>(s + i) = __ldg(reinterpret_cast<const float4*>(a.sn + at + i));
+      }
     }
-    if (is_q)
-      out[d] = from_f32<A>(f);
-    else
-      kv[d] = from_f32<C>(f);
+  }
+  const int64_t row = (int64_t)page * a.page_stride + (int64_t)(pos - pg * a.page_len) * a.pos_stride + d;
+  for (int h = h0; h - group < per_tok; h += step) {
+    const bool in = mine && h < per_tok;  // this lane has elements of a head
+    const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = in ? v[i] : 0.f;
+    if (mine && h + step < per_tok) load8(x + (int64_t)(h + step) * a.dim, v);
+    if (a.q_gain) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (in && !is_v) {
+        const float f = 1.f / sqrtf(ss / (float)a.dim + a.eps);
+        const float* const gain = (is_q ? a.q_gain : a.k_gain) + d;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * f * __ldg(gain + i);
+      }
+    }
+    if constexpr (PAIRS == kAdjacent) {
+      if (!is_v && d < a.rope_dim) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float y0 = y[i], y1 = y[i + 1];
+          y[i] = y0 * c[i / 2] - y1 * s[i / 2];
+          y[i + 1] = y1 * c[i / 2] + y0 * s[i / 2];
+        }
+      }
+    } else if constexpr (PAIRS == kHalvesByLane) {
+      const int from = d < half ? lane + half / 8 : lane - half / 8;  // past rope_dim: some lane, unused
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = __shfl_sync(0xffffffffu, y[i], from);
+      if (!is_v && d < a.rope_dim) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = d < half ? y[i] * c[i] - p[i] * s[i] : y[i] * c[i] + p[i] * s[i];
+      }
+    } else if constexpr (PAIRS == kAnyPairs) {
+      float* const st = staged[warp] + group * LANES * 8;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) st[d + i] = y[i];
+      __syncwarp();
+      if (good && !is_v) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int e = d + i;
+          if (e >= a.rope_dim) continue;
+          const bool second = a.interleaved ? e & 1 : e >= half;
+          const int at = a.interleaved ? e >> 1 : (second ? e - half : e);
+          const float p = st[a.interleaved ? e ^ 1 : (second ? e - half : e + half)];
+          const float co = __ldg(a.cs + (int64_t)pos * half + at), si = __ldg(a.sn + (int64_t)pos * half + at);
+          y[i] = second ? y[i] * co + p * si : y[i] * co - p * si;
+        }
+      }
+    }
+    if (!in) continue;
+    if (is_q) {
+      if (!good) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __int_as_float(0x7FC00000);
+      }
+      store8(q + (int64_t)h * a.dim, y);
+    } else if (good) {
+      C* const pool = static_cast<C*>(is_v ? a.v : a.k);
+      store8(pool + row + (int64_t)(h - a.n_heads - (is_v ? a.n_kv : 0)) * a.head_stride, y);
+    }
   }
 }
 
-template <class A, class C>
+template <class A, class C, int LANES>
 void launch_rope(const RopeArgs& a, cudaStream_t st) {
-  const int64_t units = (int64_t)a.n_tok * (a.n_heads + 2 * a.n_kv);
-  rope_append_kernel<A, C><<<(unsigned)((units + kRopeWarps - 1) / kRopeWarps), kRopeWarps * 32, 0, st>>>(a);
+  const dim3 grid((unsigned)(((int64_t)a.n_tok * a.splits + kRopeWarps - 1) / kRopeWarps)), block(kRopeWarps * 32);
+  const int half = a.rope_dim / 2;
+  // the tables' rows on 16-byte boundaries, and whole lanes on either side of every pair
+  const bool rows = half % 4 == 0 && !((uintptr_t)a.cs & 15) && !((uintptr_t)a.sn & 15);
+  if (a.rope_dim == 0)
+    rope_append_kernel<A, C, LANES, kNoPairs><<<grid, block, 0, st>>>(a);
+  else if (a.interleaved && rows)
+    rope_append_kernel<A, C, LANES, kAdjacent><<<grid, block, 0, st>>>(a);
+  else if (!a.interleaved && rows && half % 8 == 0)
+    rope_append_kernel<A, C, LANES, kHalvesByLane><<<grid, block, 0, st>>>(a);
+  else
+    rope_append_kernel<A, C, LANES, kAnyPairs><<<grid, block, 0, st>>>(a);
+}
+
+template <class A, class C>
+void launch_rope(RopeArgs a, cudaStream_t st) {
+  const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
+  // warps of a token: one round of heads each while there are few tokens, so that latency is not paid twice;
+  // fewer, with the token's lookups shared, once there are warps enough to fill the device
+  const int rounds = (a.n_heads + 2 * a.n_kv + 32 / lanes - 1) / (32 / lanes);
+  a.splits = std::max(1, std::min<int>(rounds, 148 * 32 / a.n_tok));
+  if (lanes == 8)
+    launch_rope<A, C, 8>(a, st);
+  else if (lanes == 16)
+    launch_rope<A, C, 16>(a, st);
+  else
+    launch_rope<A, C, 32>(a, st);
 }
 
 }  // namespace
@@ -134,7 +232,7 @@ extern "C" int mllm_rope_append(const mllm_paged_kv* kv, int dtype, const void* 
   const RopeArgs a = {kv->k, kv->v, kv->page_stride, kv->head_stride, kv->pos_stride, kv->n_pages, kv->page_len,
                       kv->n_kv_heads, kv->head_dim, d_qkv, row_stride, n_tok, n_heads, d_seq, d_pos, d_table,
                       n_seq, table_stride, d_q_gain, d_k_gain, eps, d_cos, d_sin, n_pos, rope_dim,
-                      interleaved != 0, d_q, q_stride};
+                      interleaved != 0, 1, d_q, q_stride};
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == MLLM_DTYPE_F16)
     launch_rope<__half, __half>(a, st);
