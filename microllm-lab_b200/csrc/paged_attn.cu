@@ -52,15 +52,30 @@ struct AttnArgs {
   uint32_t* counter;  // [n_seq][n_kv][groups]
   float* part;        // [CTA][2]: o [group][dim], (m, l) [group]
   int rep, group_size, groups;  // query heads per kv head, of a group, groups of a kv head
+  uint64_t page_mult;           // p / page_len = (p page_mult) >> page_shift for 0 <= p < 2^31
+  int page_shift;
 };
 
 // ---------------------------------------------------------------------------------------------
-// Cached rows travel by asynchronous 16-byte copies into a ring in shared memory of which each lane reads
-// back only what it asked for itself: many more bytes are under way than registers could take, and no
-// barrier is needed, only the lane's own count of copies.
+// Cached rows travel by asynchronous 16-byte copies into a warp's own ring in shared memory: many more bytes
+// are under way than registers could take, and no barrier is needed, only the lanes' counts of copies and the
+// warp in step.  Eight lanes copy 128 neighbouring bytes of a row: with 64 bytes a time, L2 sent every line
+// twice.  Each 16-byte piece goes to the place where the lane whose operand it is reads it, such that neither
+// the copies nor the reads meet in a bank.
 // ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ void copy16(uint4* to, const void* from, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(ok ? 16 : 0) : "memory");
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(ok ? 16 : 0) : "memory");
+}
+// The same for rows that are known to be there; further pieces of a row at constant distances.
+template <int TO, int FROM>
+__device__ __forceinline__ void copy16_at(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
+}
+// N pieces of a row, FROM bytes apart, to places TO bytes apart from the AT-th byte on.
+template <int AT, int TO, int FROM, int N, int I = 0>
+__device__ __forceinline__ void copy_rows(uint32_t to, const void* from) {
+  copy16_at<AT + I * TO, I * FROM>(to, from);
+  if constexpr (I + 1 < N) copy_rows<AT, TO, FROM, N, I + 1>(to, from);
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -76,132 +91,94 @@ __device__ __forceinline__ int blocks_of(const AttnArgs& a, int s) {
   const int n = __ldg(a.len + s);
   return n <= 0 || (int64_t)n > (int64_t)a.table_stride * a.page_len ? 0 : (n - 1) / kBlock + 1;
 }
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {  // a >= 0, b > 0; nearly always of 32 bits
-  return ((uint64_t)a | (uint64_t)b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
-}
 
-// A place in the batch: block b of segment (seq, j), j = kv head * groups + group.
+// A place in the batch: block b of segment (seq, kv head, group).  Block numbers fit 31 bits (checked on the host
+// for the longest lengths that the table can hold).
 struct Place {
-  int seq, j, b, nb, len;
+  int seq, kv, group, b, nb, len;
   __device__ __forceinline__ void at_seq(const AttnArgs& a, int s) {
     seq = s;
     nb = blocks_of(a, s);
     len = __ldg(a.len + s);
   }
-  // To the next block; only called while more blocks follow.
-  __device__ __forceinline__ void next(const AttnArgs& a) {
-    if (++b < nb) return;
+  // To the next block; only called while more blocks follow.  True where another segment begins.
+  __device__ __forceinline__ bool next(const AttnArgs& a) {
+    if (++b < nb) return false;
     b = 0;
-    if (++j < a.n_kv * a.groups) return;
-    j = 0;
-    do at_seq(a, seq + 1);
-    while (!nb);
+    if (++group == a.groups) {
+      group = 0;
+      if (++kv == a.n_kv) {
+        kv = 0;
+        do at_seq(a, seq + 1);
+        while (!nb);
+      }
+    }
+    return true;
   }
 };
 
 // What a CTA knows of the partition, and this warp's run.
 struct Run {
-  int64_t q;      // blocks of a CTA's run
-  int64_t u, n;   // first block of this warp's run, blocks in it (0: none)
-  bool whole;     // every CTA has one whole segment (numbered as if all were equally long)
+  uint32_t q;     // blocks of a CTA's run
+  uint32_t u0;    // the first of them
+  int n;          // blocks of this warp's run (0: none)
   Place from;
 };
 
+// Every warp on its own: lanes sum the lengths of neighbouring sequences.
 __device__ __forceinline__ Run find_run(const AttnArgs& a) {
-  __shared__ int64_t wsum[kAttnWarps], s_before[kAttnWarps];
-  __shared__ int wused[kAttnWarps], wlong[kAttnWarps], s_seq[kAttnWarps];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (a.n_seq + kAttnThreads - 1) / kAttnThreads;
-  const int s0 = min(tid * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
-  int64_t mine = 0;          // blocks of this thread's sequences
-  int used = 0, longest = 0;  // those that have any, the longest
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (a.n_seq + 31) / 32, s0 = min(lane * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
+  uint32_t mine = 0, longest = 0;
+#pragma unroll 4
   for (int s = s0; s < s1; ++s) {
-    const int nb = blocks_of(a, s);
+    const uint32_t nb = blocks_of(a, s);
     mine += nb;
-    used += nb > 0;
     longest = max(longest, nb);
   }
-  int64_t sum = mine;
-  int count = used;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-    const int uc = __shfl_up_sync(0xffffffffu, count, o);
-    if (lane >= o) {
-      sum += up;
-      count += uc;
-    }
-    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  }
-  if (lane == 31) {
-    wsum[warp] = sum;
-    wused[warp] = count;
-    wlong[warp] = longest;
-  }
-  __syncthreads();
-  int64_t total = 0, lead = 0;
-  int all_used = 0, lead_used = 0;
-#pragma unroll
-  for (int w = 0; w < kAttnWarps; ++w) {
-    if (w == warp) {
-      lead = total;
-      lead_used = all_used;
-    }
-    total += wsum[w];
-    all_used += wused[w];
-    longest = max(longest, wlong[w]);
-  }
-  const int per_block = a.n_kv * a.groups;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  const uint32_t per_seq = a.n_kv * a.groups;
   Run r;
-  r.whole = longest <= kWholeBlocks && (int64_t)all_used * per_block <= gridDim.x;
-  int64_t all, before;  // of this thread's sequences
-  if (r.whole) {
-    all = (int64_t)all_used * longest;
-    before = (int64_t)(lead_used + count - used) * longest;
-    r.q = longest;
-  } else {
-    all = total;
-    before = lead + sum - mine;
-    r.q = max(max(divide(all * per_block + gridDim.x - 1, gridDim.x), (int64_t)kMinBlocks), (int64_t)(longest + kMaxParts - 1) / kMaxParts);
-  }
-  // the sequences in which the warps' runs begin
-  const int64_t u0 = blockIdx.x * r.q, end = min(u0 + r.q, all * per_block);
   r.n = 0;
-  if (u0 >= end) return r;
-  const int64_t each = r.whole ? 0 : (end - u0 + kAttnWarps - 1) / kAttnWarps;
-#pragma unroll
-  for (int w = 0; w < kAttnWarps; ++w) {
-    const int64_t u = u0 + w * each, mine_all = r.whole ? (int64_t)used * longest : mine;
-    if (u >= before * per_block && u < (before + mine_all) * per_block) {
-      int64_t b = before;
-      int s = s0;
-      for (;; ++s) {
-        const int nb = blocks_of(a, s), n = r.whole && nb ? longest : nb;
-        if (u < (b + n) * per_block) break;
-        b += n;
-      }
-      s_seq[w] = s;
-      s_before[w] = b;
-    }
-  }
-  __syncthreads();
-  r.u = u0 + warp * each;
-  r.n = min(each, end - r.u);
-  if (!r.whole && r.n <= 0) {
-    r.n = 0;
-    return r;
-  }
-  r.from.at_seq(a, s_seq[warp]);
-  const int64_t in = r.u - s_before[warp] * per_block;
-  const int n = r.whole ? longest : r.from.nb;
-  r.from.j = (int)divide(in, n);
-  r.from.b = (int)(in - (int64_t)r.from.j * n);
-  if (r.whole) {  // the warps share the blocks of the one segment
+  if (longest <= kWholeBlocks && (uint64_t)a.n_seq * per_seq <= gridDim.x) {  // one segment, its blocks shared by the warps
+    r.q = r.u0 = 0;
+    const uint32_t seq = blockIdx.x / per_seq, j = blockIdx.x - seq * per_seq;
+    if (seq >= a.n_seq) return r;
+    r.from.at_seq(a, seq);
+    r.from.kv = j / a.groups;
+    r.from.group = j - r.from.kv * a.groups;
     const int share = (r.from.nb + kAttnWarps - 1) / kAttnWarps;
     r.from.b = warp * share;
-    r.u += r.from.b;
     r.n = max(min(share, r.from.nb - r.from.b), 0);
+    return r;
   }
+  uint32_t upto = mine;  // this lane's sequences and those before them
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += up;
+  }
+  const uint32_t all = __shfl_sync(0xffffffffu, upto, 31) * per_seq;
+  r.q = max(max((all + gridDim.x - 1) / gridDim.x, (uint32_t)kMinBlocks), (longest + kMaxParts - 1) / kMaxParts);
+  r.u0 = blockIdx.x * r.q;
+  if ((uint64_t)blockIdx.x * r.q >= all) return r;
+  const uint32_t end = min(r.u0 + r.q, all), each = (end - r.u0 + kAttnWarps - 1) / kAttnWarps, u = r.u0 + warp * each;
+  if (u >= end) return r;
+  r.n = min(each, end - u);
+  // the lane whose sequences hold block u, then the one of them
+  const int who = __ffs(__ballot_sync(0xffffffffu, u < upto * per_seq)) - 1;
+  uint32_t before = __shfl_sync(0xffffffffu, upto - mine, who) * per_seq;
+  int s = who * per;
+  for (;; ++s) {
+    const uint32_t nb = blocks_of(a, s) * per_seq;
+    if (u < before + nb) break;
+    before += nb;
+  }
+  r.from.at_seq(a, s);
+  const uint32_t j = (u - before) / r.from.nb;
+  r.from.b = u - before - j * r.from.nb;
+  r.from.kv = j / a.groups;
+  r.from.group = j - r.from.kv * a.groups;
   return r;
 }
 
@@ -210,24 +187,20 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a) {
 __device__ __forceinline__ int64_t row_offset(const AttnArgs& a, const Place& c, int lane, uint32_t& bad, int ord) {
   const int p = c.b * kBlock + lane;
   if (p >= c.len) return -1;
-  const int pg = p / a.page_len;
+  const int pg = (int)((uint64_t)p * a.page_mult >> a.page_shift);
   const int page = __ldg(a.table + (int64_t)c.seq * a.table_stride + pg);
   if ((unsigned)page >= (unsigned)a.n_pages) {
     bad |= 1u << (ord & 31);
     return -1;
   }
-  return page * a.page_stride + c.j / a.groups * a.head_stride + (int64_t)(p - pg * a.page_len) * a.pos_stride;
+  return page * a.page_stride + c.kv * a.head_stride + (int64_t)(p - pg * a.page_len) * a.pos_stride;
 }
-__device__ __forceinline__ int first_head(const AttnArgs& a, int j) {
-  return j / a.groups * a.rep + j % a.groups * a.group_size;
-}
-__device__ __forceinline__ int heads_of(const AttnArgs& a, int j) {
-  return min(a.rep - j % a.groups * a.group_size, a.group_size);
-}
-
 // A part of a segment: what one run holds of it.
 struct Part {
-  int seq, j, b0, blocks, nb;  // blocks 0: none
+  int seq, kv, group, b0, blocks, nb;  // blocks 0: none
+  __device__ __forceinline__ int first_head(const AttnArgs& a) const { return kv * a.rep + group * a.group_size; }
+  __device__ __forceinline__ int heads(const AttnArgs& a) const { return min(a.rep - group * a.group_size, a.group_size); }
+  __device__ __forceinline__ bool same(const Part& o) const { return seq == o.seq && kv == o.kv && group == o.group; }
 };
 // The parts that a CTA's warps leave for the join: of a run's first segment (slot 0) and of its last (slot
 // 1).  m is in units of log 2.  A page id outside the pool makes l, and with it the result, NaN.
@@ -257,121 +230,121 @@ __device__ __forceinline__ void store4(A* p, const float4& v) {  // p on a 4-ele
 }
 // Four elements of a finished row of head h of the group; l == 0: no position had a weight.
 template <class A>
-__device__ __forceinline__ void write_out(const AttnArgs& a, int seq, int j, int h, int d, const float4& o, float l) {
-  A* out = static_cast<A*>(a.out) + seq * a.out_stride + (int64_t)(first_head(a, j) + h) * a.dim + d;
-  store4(out, l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x / l, o.y / l, o.z / l, o.w / l));
+__device__ __forceinline__ void write_out(const AttnArgs& a, const Part& p, int h, int d, const float4& o, float l) {
+  A* out = static_cast<A*>(a.out) + p.seq * a.out_stride + (int64_t)(p.first_head(a) + h) * a.dim + d;
+  store4(out, rows4(o, l == 0.f ? 0.f : 1.f / l));
 }
-__device__ __forceinline__ void write_lse(const AttnArgs& a, int seq, int j, int h, float m, float l) {
-  if (a.lse) a.lse[(int64_t)seq * a.n_heads + first_head(a, j) + h] = (m + log2f(l)) * (1.f / kLog2e);
+__device__ __forceinline__ void write_lse(const AttnArgs& a, const Part& p, int h, float m, float l) {
+  if (a.lse) a.lse[(int64_t)p.seq * a.n_heads + p.first_head(a) + h] = (m + log2f(l)) * (1.f / kLog2e);
+}
+// (m, l, o) joined with another.
+__device__ __forceinline__ void join2(float& m, float& l, float4& o, float m1, float l1, const float4& o1) {
+  const float top = fmaxf(m, m1);
+  const float f0 = m == -INFINITY ? 0.f : pow2(m - top), f1 = m1 == -INFINITY ? 0.f : pow2(m1 - top);
+  l = l * f0 + l1 * f1;
+  o = fma4(f1, o1, rows4(o, f0));
+  m = top;
 }
 
-// Joins the parts that the warps left, and those of other CTAs where this is the last CTA of a segment.
+// Joins the parts that the warps left, each segment by the warp that has its first part here, and those of all
+// CTAs where this is the last one of a segment to come.
 template <class A, int DP>
-__device__ void join(const AttnArgs& a, const Run& r, const Joint& w) {
-  __shared__ int s_last[2];
-  const int tid = threadIdx.x, quads = a.dim / 4;
+__device__ __noinline__ void join(const AttnArgs& a, const Run& r, const Joint& w) {
+  struct Open {  // a segment whose last part this CTA left
+    Part p;
+    int first, parts;
+  };
+  __shared__ Open open[2];  // one that began before this CTA, one that began in it
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quads = a.dim / 4;
   const size_t slot = (size_t)a.group_size * (a.dim + 4);  // o, then m and l; 16-byte aligned for any group
-  Part open[2];  // the segments that go on in other CTAs: begun before this CTA, or in it
-  open[0].blocks = open[1].blocks = 0;
+  if (tid < 2) open[tid].parts = 0;
   __syncthreads();
-  for (int i = 0; i < 2 * kAttnWarps;) {
+#pragma unroll 1
+  for (int i = 2 * warp; i < 2 * warp + 2; ++i) {
     const Part p = w.part[i];
-    if (!p.blocks) {
-      ++i;
-      continue;
-    }
-    int have = 0, end = i;  // parts i .. end - 1 are of this segment
+    if (!p.blocks || (i && p.b0)) continue;  // none, or it goes on from another warp's
+    int have = p.blocks, end = i + 1;        // parts i .. end - 1 are of this segment
     for (; end < 2 * kAttnWarps; ++end) {
-      const Part& q = w.part[end];
-      if (!q.blocks) continue;
-      if (q.seq != p.seq || q.j != p.j) break;
-      have += q.blocks;
+      const Part& o = w.part[end];
+      if (!o.blocks) continue;
+      if (!o.same(p)) break;
+      have += o.blocks;
     }
     const bool done = have == p.nb;
-    const int side = p.b0 == 0;
+    const int side = p.b0 == 0, items = p.heads(a) * quads;
     float* const out = a.part + ((size_t)blockIdx.x * 2 + side) * slot;
-    const int heads = heads_of(a, p.j);
-    for (int x = tid; x < heads * quads; x += kAttnThreads) {
+#pragma unroll 1
+    for (int x = lane; x < items; x += 32) {
       const int h = x / quads, d = (x - h * quads) * 4;
       float m = -INFINITY, l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = i; k < end; ++k)
-        if (w.part[k].blocks) m = fmaxf(m, w.m[k * a.group_size + h]);
-      for (int k = i; k < end; ++k) {
-        if (!w.part[k].blocks) continue;
-        const float mk = w.m[k * a.group_size + h], f = mk == -INFINITY ? 0.f : pow2(mk - m);
-        l = fmaf(f, w.l[k * a.group_size + h], l);
-        o = fma4(f, *reinterpret_cast<const float4*>(w.o<DP>(a, k >> 1, k & 1) + h * DP + d), o);
-      }
+        if (w.part[k].blocks)
+          join2(m, l, o, w.m[k * a.group_size + h], w.l[k * a.group_size + h],
+                *reinterpret_cast<const float4*>(w.o<DP>(a, k >> 1, k & 1) + h * DP + d));
       if (done) {
-        write_out<A>(a, p.seq, p.j, h, d, o, l);
-        if (d == 0) write_lse(a, p.seq, p.j, h, m, l);
+        write_out<A>(a, p, h, d, o, l);
+        if (d == 0) write_lse(a, p, h, m, l);
       } else {
         *reinterpret_cast<float4*>(out + h * a.dim + d) = o;
         if (d == 0) *reinterpret_cast<float2*>(out + a.group_size * a.dim + 2 * h) = make_float2(m, l);
       }
     }
-    if (!done && side == 0) {
-      open[0] = p;
-      open[0].blocks = have;
-    } else if (!done) {
-      open[1] = p;
-      open[1].blocks = have;
-    }
-    i = end;
-  }
-  if (!open[0].blocks && !open[1].blocks) return;
-  // which CTAs have a part, from the segment's first block in the batch: one that begins in this CTA's run
-  // goes on to its end
-  const int64_t u0 = blockIdx.x * r.q;
-  int first[2], parts[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t start = i == 0 ? u0 - open[0].b0 : u0 + r.q - open[1].blocks;
-    first[i] = open[i].blocks ? (int)divide(start, r.q) : 0;
-    parts[i] = open[i].blocks ? (int)divide(start + open[i].nb - 1, r.q) - first[i] + 1 : 0;
-  }
-  __threadfence();
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (tid == 32 * i && open[i].blocks) {
-      uint32_t* c = a.counter + (int64_t)open[i].seq * a.n_kv * a.groups + open[i].j;
-      s_last[i] = atomicAdd(c, 1u) == (uint32_t)parts[i] - 1;
-      if (s_last[i]) *c = 0;
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (!open[i].blocks || !s_last[i]) continue;
+    if (done) continue;
     __threadfence();
-    const Part& p = open[i];
-    const int heads = heads_of(a, p.j);
-    for (int x = tid; x < heads * quads; x += kAttnThreads) {
+    __syncwarp();
+    if (lane == 0) {
+      // which CTAs have a part, by the segment's first block: one that began in this run goes on to its end
+      const uint32_t start = side ? r.u0 + r.q - have : r.u0 - p.b0, first = start / r.q;
+      const int parts = (int)((start + p.nb - 1) / r.q - first) + 1;
+      uint32_t* const c = a.counter + ((int64_t)p.seq * a.n_kv + p.kv) * a.groups + p.group;
+      if (atomicAdd(c, 1u) == (uint32_t)parts - 1) {
+        *c = 0;
+        open[side] = Open{p, (int)first, parts};
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    const Open& s = open[side];
+    if (!s.parts) continue;
+    __threadfence();
+    // every fourth part by each warp, then the four in order: (m, l) and o of [warp][item] at the rings' place
+    const int items = s.p.heads(a) * quads;
+    float2* const ml = reinterpret_cast<float2*>(w.ring);
+    float4* const os = reinterpret_cast<float4*>(ml + kAttnWarps * items);
+#pragma unroll 1
+    for (int x = lane; x < items; x += 32) {
       const int h = x / quads, d = (x - h * quads) * 4;
       float m = -INFINITY, l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (int k = 0; k < parts[i]; ++k) {
-        const float* q = a.part + ((size_t)(first[i] + k) * 2 + (k == 0)) * slot;
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + a.group_size * a.dim) + h);
-        const float4 ok = __ldcg(reinterpret_cast<const float4*>(q + h * a.dim + d));
-        const float top = fmaxf(m, ml.x);
-        const float f0 = m == -INFINITY ? 0.f : pow2(m - top), f1 = ml.x == -INFINITY ? 0.f : pow2(ml.x - top);
-        l = l * f0 + ml.y * f1;
-        o = fma4(f1, ok, rows4(o, f0));
-        m = top;
+      for (int k = warp; k < s.parts; k += kAttnWarps) {
+        const float* q = a.part + ((size_t)(s.first + k) * 2 + (k == 0)) * slot;
+        const float2 mk = __ldcg(reinterpret_cast<const float2*>(q + a.group_size * a.dim) + h);
+        join2(m, l, o, mk.x, mk.y, __ldcg(reinterpret_cast<const float4*>(q + h * a.dim + d)));
       }
-      write_out<A>(a, p.seq, p.j, h, d, o, l);
-      if (d == 0) write_lse(a, p.seq, p.j, h, m, l);
+      ml[warp * items + x] = make_float2(m, l);
+      os[warp * items + x] = o;
     }
+    __syncthreads();
+#pragma unroll 1
+    for (int x = tid; x < items; x += kAttnThreads) {
+      const int h = x / quads, d = (x - h * quads) * 4;
+      float m = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < min(kAttnWarps, s.parts); ++k) join2(m, l, o, ml[k * items + x].x, ml[k * items + x].y, os[k * items + x]);
+      write_out<A>(a, s.p, h, d, o, l);
+      if (d == 0) write_lse(a, s.p, h, m, l);
+    }
+    __syncthreads();
   }
 }
 
 // Sequences without positions, and those whose length the table cannot hold.
 template <class A>
-__device__ void finish_empty(const AttnArgs& a) {
+__device__ __noinline__ void finish_empty(const AttnArgs& a) {
   for (int s = blockIdx.x; s < a.n_seq; s += gridDim.x) {
     if (blocks_of(a, s)) continue;
     const float v = a.len[s] > 0 ? __int_as_float(0x7FC00000) : 0.f;
@@ -386,7 +359,7 @@ __device__ void finish_empty(const AttnArgs& a) {
 // Caches of 16 bits: both products on the tensor cores, m16n8k16 with positions (then head_dim) as the
 // 16 rows and 8 query heads as the columns, so that a group of few heads wastes little.  The order of the
 // summed index is free as long as both operands share it, so the 16-byte pieces of cached rows that a lane
-// copies are its operands as they are: for the scores its 8 neighbouring elements of a key row serve two
+// reads are its operands as they are: for the scores its 8 neighbouring elements of a key row serve two
 // steps; for the output, pairs of value rows are woven by byte permutes.  The scores' accumulators, packed
 // and transposed by movmatrix, are the second product's operand.
 //
@@ -464,7 +437,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Part parts[2 * kAttnWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, quad = lane & 3;
-  uint4* const ring = reinterpret_cast<uint4*>(smem + warp * mma_ring_bytes<DP>()) + lane;  // piece i of stage s: [(s PIECES + i) 32]
+  const uint4* const ring = reinterpret_cast<const uint4*>(smem + warp * mma_ring_bytes<DP>());  // piece i of stage s: [(s PIECES + i) 32]
   uint4* const qs = reinterpret_cast<uint4*>(smem + kAttnWarps * mma_ring_bytes<DP>() + warp * mma_query_bytes<T, A, DP, NT>()) + lane;
   Joint joint;
   joint.part = parts;
@@ -478,7 +451,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
 
   const Run run = find_run(a);
   if (lane == 0) parts[2 * warp].blocks = parts[2 * warp + 1].blocks = 0;
-  const int n = (int)run.n;  // blocks; two stages each
+  const int n = run.n;  // blocks; two stages each
   if (n) {
     Place ahead = run.from, c = run.from;
     uint32_t bad = 0;  // by segment, numbered along the run: this lane has met a page outside the pool
@@ -486,35 +459,37 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
     int64_t off = row_offset(a, ahead, lane, bad, ahead_ord), off_next = -1;
     auto look = [&](int k) {  // the rows of block k of the run
       if (k < n) {
-        const int j = ahead.j, seq = ahead.seq;
-        ahead.next(a);
-        ahead_ord += ahead.j != j || ahead.seq != seq;
+        ahead_ord += ahead.next(a);
         off_next = row_offset(a, ahead, lane, bad, ahead_ord);
       }
     };
     look(1);
+    // places of this lane's copies within a stage: rows 4 i + part, 64-element chunks of 8 pieces
+    const int part = lane >> 3, chunk = lane & 7;
+    const uint32_t ring32 = smem_u32(smem + warp * mma_ring_bytes<DP>());
+    const uint32_t k_to = (chunk >> 2) * 1024 + ((part ^ (chunk >> 2)) * 4 + (chunk & 3)) * 16;
+    const uint32_t v_to = 2 * C * 512 + (part & 1) * 512 + chunk * 64;
+    const uint32_t v_even = v_to + ((part >> 1) ^ (chunk >> 1)) * 16, v_odd = v_to + ((part >> 1) ^ (chunk >> 1) ^ 2) * 16;
     auto issue = [&](int i) {
       if (i < 2 * n) {
-        uint4* const to = ring + (i % S) * PIECES * 32;
-        const int half = (i & 1) * 16;
+        const uint32_t to = ring32 + (i % S) * PIECES * 512;
+        const bool whole = a.dim == DP && __all_sync(0xffffffffu, off >= 0);  // every row of the block
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {  // key rows row, row + 8
-          const int64_t at = __shfl_sync(0xffffffffu, off, half + row + 8 * e);
+        for (int x = 0; x < 4; ++x) {
+          const int64_t at = __shfl_sync(0xffffffffu, off, (i & 1) * 16 + 4 * x + part);
+          const T* const kr = kp + at + chunk * 8;
+          const T* const vr = vp + at + chunk * 8;
+          const uint32_t kt = to + k_to + (x >> 1) * 512 + (x & 1) * 256, vt = to + (x & 1 ? v_odd : v_even) + (x >> 1) * 1024;
+          if (whole) {
+            copy_rows<0, 2048, 128, V>(kt, kr);
+            copy_rows<0, 2048, 128, V>(vt, vr);
+          } else {
 #pragma unroll
-          for (int x = 0; x < C; ++x) {
-            const int d = x * 32 + quad * 8;
-            const bool ok = at >= 0 && d < a.dim;
-            copy16(to + (2 * x + e) * 32, kp + (ok ? at + d : 0), ok);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {  // value rows 2 quad, 2 quad + 1, 2 quad + 8, 2 quad + 9
-          const int64_t at = __shfl_sync(0xffffffffu, off, half + (e >> 1) * 8 + quad * 2 + (e & 1));
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const int d = v * 64 + row * 8;
-            const bool ok = at >= 0 && d < a.dim;
-            copy16(to + (2 * C + 4 * v + e) * 32, vp + (ok ? at + d : 0), ok);
+            for (int y = 0; y < V; ++y) {
+              const bool ok = at >= 0 && y * 64 + chunk * 8 < a.dim;
+              copy16(kt + y * 2048, ok ? kr + y * 64 : kp, ok);
+              copy16(vt + y * 2048, ok ? vr + y * 64 : vp, ok);
+            }
           }
         }
         if (i & 1) {
@@ -524,7 +499,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
       }
       copies_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < S - 1; ++i) issue(i);
 
     uint4 qr[QREG ? C : 1][QREG ? TERMS : 1][QREG ? NT : 1] = {};
@@ -540,8 +515,9 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
     for (int k = 0; k < n; ++k) {
       if (k == 0 || c.b == 0) {  // a segment begins: its queries, every head's row of 8 * NT (0 past the group)
         b0 = c.b;
-        const int heads = heads_of(a, c.j);
-        const A* const q = static_cast<const A*>(a.q) + c.seq * a.q_stride + (int64_t)first_head(a, c.j) * a.dim;
+        const Part p = {c.seq, c.kv, c.group};
+        const int heads = p.heads(a);
+        const A* const q = static_cast<const A*>(a.q) + c.seq * a.q_stride + (int64_t)p.first_head(a) * a.dim;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int h = nt * 8 + row;
@@ -609,13 +585,15 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
               for (int e = 0; e < 4; ++e) o[v][x][nt][e] = 0.f;
         }
       }
-#pragma unroll
+#pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         const int i = 2 * k + half;
         copies_wait<S - 2>();
-        issue(i + S - 1);  // into the stage that the last round read
+        __syncwarp();      // all lanes' copies are there, and all have read the last round's stage
+        issue(i + S - 1);  // into that one
         if (c.b * kBlock + half * 16 >= c.len) continue;
-        const uint4* const st = ring + (i % S) * PIECES * 32;
+        const uint4* const sk = ring + (i % S) * PIECES * 32;                               // key pieces
+        const uint4* const sv = sk + 2 * C * 32 + row * 4 + (quad ^ (row >> 1));            // value pieces of this lane
         const int p0 = c.b * kBlock + half * 16 + row;
         // ---- scores: 16 positions x heads
         float s[NT][4];
@@ -629,7 +607,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
         };
 #pragma unroll
         for (int x = 0; x < C; ++x) {
-          const uint4 k0 = st[(2 * x) * 32], k1 = st[(2 * x + 1) * 32];
+          const uint4 k0 = sk[(2 * x) * 32 + (lane ^ (x & 1) * 4)], k1 = sk[(2 * x + 1) * 32 + (lane ^ (x & 1) * 4)];
 #pragma unroll
           for (int t = 0; t < TERMS; ++t)
 #pragma unroll
@@ -648,7 +626,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
             for (int nt = 0; nt < NT; ++nt) {
               float f[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int x = 0; x < C; ++x) score(f, st[(2 * x) * 32], st[(2 * x + 1) * 32], query(x, 0, nt));
+              for (int x = 0; x < C; ++x) score(f, sk[(2 * x) * 32 + (lane ^ (x & 1) * 4)], sk[(2 * x + 1) * 32 + (lane ^ (x & 1) * 4)], query(x, 0, nt));
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (s[nt][e] != s[nt][e]) s[nt][e] = f[e];
@@ -702,7 +680,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
         for (int v = 0; v < V; ++v) {
           uint4 x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = st[(2 * C + 4 * v + e) * 32];
+          for (int e = 0; e < 4; ++e) x[e] = sv[(4 * v + e) * 32];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             const uint32_t a0 = __byte_perm(word(x[0], y), word(x[1], y), 0x5410), a1 = __byte_perm(word(x[0], y), word(x[1], y), 0x7632);
@@ -718,7 +696,8 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
       if (ends || k + 1 == n) {  // all that this run has of the segment
         const bool done = ends && b0 == 0;
         const int slot = k + 1 - (c.b + 1 - b0) == 0 ? 0 : 1;
-        const int heads = heads_of(a, c.j);
+        const Part mine = {c.seq, c.kv, c.group, b0, c.b + 1 - b0, c.nb};
+        const int heads = mine.heads(a);
         const bool nan = __any_sync(0xffffffffu, bad >> (ord & 31) & 1u);
         bad &= ~(1u << (ord & 31));
         if (slot == 1 && !done) {  // the run's end: the ring is free
@@ -743,8 +722,8 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
               const float4 lo = make_float4(o[v][0][nt][e], o[v][0][nt][2 + e], o[v][1][nt][e], o[v][1][nt][2 + e]);
               const float4 hi = make_float4(o[v][2][nt][e], o[v][2][nt][2 + e], o[v][3][nt][e], o[v][3][nt][2 + e]);
               if (done) {
-                write_out<A>(a, c.seq, c.j, h, d, lo, sum);
-                write_out<A>(a, c.seq, c.j, h, d + 4, hi, sum);
+                write_out<A>(a, mine, h, d, lo, sum);
+                write_out<A>(a, mine, h, d + 4, hi, sum);
               } else {
                 *reinterpret_cast<float4*>(jo + h * DP + d) = lo;
                 *reinterpret_cast<float4*>(jo + h * DP + d + 4) = hi;
@@ -752,14 +731,14 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
             }
             if (row == 0) {
               if (done) {
-                write_lse(a, c.seq, c.j, h, m[nt][e], sum);
+                write_lse(a, mine, h, m[nt][e], sum);
               } else {
                 joint.m[(2 * warp + slot) * a.group_size + h] = m[nt][e];
                 joint.l[(2 * warp + slot) * a.group_size + h] = sum;
               }
             }
           }
-        if (!done && lane == 0) parts[2 * warp + slot] = Part{c.seq, c.j, b0, c.b + 1 - b0, c.nb};
+        if (!done && lane == 0) parts[2 * warp + slot] = mine;
         ++ord;
       }
       if (k + 1 < n) c.next(a);
@@ -795,7 +774,7 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Part parts[2 * kAttnWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, quad = lane & 3;
-  uint4* const ring = reinterpret_cast<uint4*>(smem + warp * f32_ring_bytes<DP>()) + lane;
+  const float4* const ring = reinterpret_cast<const float4*>(smem + warp * f32_ring_bytes<DP>());
   float* const qs = reinterpret_cast<float*>(smem + kAttnWarps * f32_ring_bytes<DP>() + warp * f32_query_bytes<DP, G>());  // [G][DP]
   float* const pw = qs + G * DP;                                                                                            // [position][G]
   Joint joint;
@@ -811,7 +790,7 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
 
   const Run run = find_run(a);
   if (lane == 0) parts[2 * warp].blocks = parts[2 * warp + 1].blocks = 0;
-  const int n = (int)run.n;  // blocks
+  const int n = run.n;  // blocks
   if (n) {
     Place ahead = run.from, c = run.from;
     uint32_t bad = 0;
@@ -819,35 +798,42 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
     int64_t off = row_offset(a, ahead, lane, bad, ahead_ord), off_next = -1;
     auto look = [&](int k) {
       if (k < n) {
-        const int j = ahead.j, seq = ahead.seq;
-        ahead.next(a);
-        ahead_ord += ahead.j != j || ahead.seq != seq;
+        ahead_ord += ahead.next(a);
         off_next = row_offset(a, ahead, lane, bad, ahead_ord);
       }
     };
     look(1);
+    const int part = lane >> 3, chunk = lane & 7;  // of the key copies: rows 4 i + part, 32-element chunks of 8 pieces
+    const uint32_t ring32 = smem_u32(smem + warp * f32_ring_bytes<DP>());
+    const uint32_t k_to = (chunk >> 2) * R * 512 + ((part ^ (chunk >> 2)) * 4 + (chunk & 3)) * 16;
     auto issue = [&](int i) {
       if (i < PARTS * n) {
-        uint4* const to = ring + (i % S) * PIECES * 32;
-        const int part = (i % PARTS) * P;
+        const uint32_t to = ring32 + (i % S) * PIECES * 512;
+        const int first = (i % PARTS) * P;
+        const bool whole = a.dim == DP && __all_sync(0xffffffffu, off >= 0);  // every row of the block
 #pragma unroll
-        for (int e = 0; e < R; ++e) {  // key rows row, row + 8, ...
-          const int64_t at = __shfl_sync(0xffffffffu, off, part + row + 8 * e);
-#pragma unroll
-          for (int x = 0; x < C; ++x) {
-            const int d = x * 16 + quad * 4;
-            const bool ok = at >= 0 && d < a.dim;
-            copy16(to + (x * R + e) * 32, kp + (ok ? at + d : 0), ok);
+        for (int x = 0; x < 2 * R; ++x) {
+          const int64_t at = __shfl_sync(0xffffffffu, off, first + 4 * x + part);
+          const float* const kr = kp + at + chunk * 4;
+          const uint32_t kt = to + k_to + (x >> 1) * 512 + (x & 1) * 256;
+          if (whole) {
+            copy_rows<0, 2 * R * 512, 128, C / 2>(kt, kr);
+          } else {
+#pragma unroll 1
+            for (int y = 0; y < C / 2; ++y) {
+              const bool ok = at >= 0 && y * 32 + chunk * 4 < a.dim;
+              copy16(kt + y * 2 * R * 512, ok ? kr + y * 32 : kp, ok);
+            }
           }
         }
 #pragma unroll
         for (int p = 0; p < P / ROWS; ++p) {
-          const int64_t at = __shfl_sync(0xffffffffu, off, part + p * ROWS + lane / PER);
+          const int64_t at = __shfl_sync(0xffffffffu, off, first + p * ROWS + lane / PER);
+          const float* const from = vp + at + lane % PER * 4;
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const int d = (v * PER + lane % PER) * 4;
-            const bool ok = at >= 0 && d < a.dim;
-            copy16(to + (R * C + p * V + v) * 32, vp + (ok ? at + d : 0), ok);
+            const bool ok = whole || (at >= 0 && (v * PER + lane % PER) * 4 < a.dim);
+            copy16(to + (R * C + p * V + v) * 512 + lane * 16, ok ? from + v * PER * 4 : vp, ok);
           }
         }
         if (i % PARTS == PARTS - 1) {
@@ -857,7 +843,7 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
       }
       copies_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < S - 1; ++i) issue(i);
     float m[G], l[G];  // of every head: m the same on every lane, l of this lane's positions
     float o[V][G][4];
@@ -865,8 +851,9 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
     for (int k = 0; k < n; ++k) {
       if (k == 0 || c.b == 0) {
         b0 = c.b;
-        const int heads = heads_of(a, c.j);
-        const float* const q = static_cast<const float*>(a.q) + c.seq * a.q_stride + (int64_t)first_head(a, c.j) * a.dim;
+        const Part p = {c.seq, c.kv, c.group};
+        const int heads = p.heads(a);
+        const float* const q = static_cast<const float*>(a.q) + c.seq * a.q_stride + (int64_t)p.first_head(a) * a.dim;
         __syncwarp();  // the last segment's queries are read
 #pragma unroll
         for (int x = 0; x < G * DP / 128; ++x) {
@@ -887,13 +874,14 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
         }
       }
 #pragma unroll 1
-      for (int part = 0; part < PARTS; ++part) {
-        const int i = PARTS * k + part;
+      for (int turn = 0; turn < PARTS; ++turn) {
+        const int i = PARTS * k + turn;
         copies_wait<S - 2>();
+        __syncwarp();  // all lanes' copies are there, and all have read the last round's stage
         issue(i + S - 1);
-        if (c.b * kBlock + part * P >= c.len) continue;
-        const float4* const st = reinterpret_cast<const float4*>(ring + (i % S) * PIECES * 32);
-        const int p0 = c.b * kBlock + part * P + row;
+        if (c.b * kBlock + turn * P >= c.len) continue;
+        const float4* const st = ring + (i % S) * PIECES * 32;
+        const int p0 = c.b * kBlock + turn * P + row;
         // ---- scores of rows row, row + 8, ...
         float s[R][G];
 #pragma unroll
@@ -904,7 +892,7 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
         for (int x = 0; x < C; ++x) {
           float4 key[R];
 #pragma unroll
-          for (int e = 0; e < R; ++e) key[e] = st[(x * R + e) * 32];
+          for (int e = 0; e < R; ++e) key[e] = st[(x * R + e) * 32 + (lane ^ (x & 1) * 4)];
 #pragma unroll
           for (int h = 0; h < G; ++h) {
             const float4 q = *reinterpret_cast<const float4*>(qs + h * DP + x * 16 + quad * 4);
@@ -958,7 +946,7 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
             *reinterpret_cast<float4*>(w + h) = *reinterpret_cast<const float4*>(pw + (p * ROWS + lane / PER) * G + h);
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const float4 x = st[(R * C + p * V + v) * 32];
+            const float4 x = st[(R * C + p * V + v) * 32 + lane];
 #pragma unroll
             for (int h = 0; h < G; ++h) {
               o[v][h][0] = fmaf(w[h], x.x, o[v][h][0]);
@@ -973,7 +961,8 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
       if (ends || k + 1 == n) {  // all that this run has of the segment
         const bool done = ends && b0 == 0;
         const int slot = k + 1 - (c.b + 1 - b0) == 0 ? 0 : 1;
-        const int heads = heads_of(a, c.j);
+        const Part mine = {c.seq, c.kv, c.group, b0, c.b + 1 - b0, c.nb};
+        const int heads = mine.heads(a);
         const bool nan = __any_sync(0xffffffffu, bad >> (ord & 31) & 1u);
         bad &= ~(1u << (ord & 31));
         if (slot == 1 && !done) {  // the run's end: the ring is free
@@ -997,20 +986,20 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
             if (lane >= PER || d >= a.dim) continue;
             const float4 x = make_float4(o[v][h][0], o[v][h][1], o[v][h][2], o[v][h][3]);
             if (done)
-              write_out<float>(a, c.seq, c.j, h, d, x, sum);
+              write_out<float>(a, mine, h, d, x, sum);
             else
               *reinterpret_cast<float4*>(jo + h * DP + d) = x;
           }
           if (lane == 0) {
             if (done) {
-              write_lse(a, c.seq, c.j, h, m[h], sum);
+              write_lse(a, mine, h, m[h], sum);
             } else {
               joint.m[(2 * warp + slot) * a.group_size + h] = m[h];
               joint.l[(2 * warp + slot) * a.group_size + h] = sum;
             }
           }
         }
-        if (!done && lane == 0) parts[2 * warp + slot] = Part{c.seq, c.j, b0, c.b + 1 - b0, c.nb};
+        if (!done && lane == 0) parts[2 * warp + slot] = mine;
         ++ord;
       }
       if (k + 1 < n) c.next(a);
@@ -1047,6 +1036,8 @@ int launch(const AttnArgs& a, int dp, int per_sm, size_t smem, cudaStream_t st) 
   per_sm = std::min(per_sm, (int)(228 * 1024 / (smem + 1024 + 512)));
   // no more CTAs than runs of the shortest length over the whole table
   const int64_t blocks = ((int64_t)a.table_stride * a.page_len + kBlock - 1) / kBlock;
+  if ((double)blocks * a.n_seq * a.n_kv * a.groups > 2147483648.0 - 65536.0)
+    return refuse(MLLM_ERR_UNSUPPORTED, "mllm_paged_attn: the table can hold 2^31 blocks of 32 positions, over all kv heads");
   const int64_t most = (blocks + kMinBlocks - 1) / kMinBlocks * a.n_seq * a.n_kv * a.groups;
   const int grid = (int)std::min<int64_t>(most, std::min(kMaxCtas, sms * per_sm));
   KERNEL<<<grid, kAttnThreads, smem, st>>>(a);
@@ -1114,6 +1105,10 @@ extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d
                 kv->n_kv_heads, kv->head_dim, d_q, q_stride, n_seq, n_heads, d_len, d_table, table_stride,
                 scale, d_out, out_stride, d_lse};
   a.rep = n_heads / kv->n_kv_heads;
+  int bits = 0;  // ceil(log2 page_len)
+  while (((int64_t)1 << bits) < kv->page_len) ++bits;
+  a.page_shift = 31 + bits;
+  a.page_mult = ((uint64_t)1 << a.page_shift) / kv->page_len + 1;
   a.counter = static_cast<uint32_t*>(d_ws);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + counter_bytes(n_seq, n_heads));
   cudaStream_t st = (cudaStream_t)stream;
