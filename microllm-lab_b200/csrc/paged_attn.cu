@@ -64,12 +64,12 @@ struct AttnArgs {
 // the copies nor the reads meet in a bank.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(ok ? 16 : 0) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(ok ? 16 : 0) : "memory");
 }
 // The same for rows that are known to be there; further pieces of a row at constant distances.
 template <int TO, int FROM>
 __device__ __forceinline__ void copy16_at(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
 }
 // N pieces of a row, FROM bytes apart, to places TO bytes apart from the AT-th byte on.
 template <int AT, int TO, int FROM, int N, int I = 0>
@@ -82,7 +82,11 @@ template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // 2^x for the softmax; x <= 0, or -inf.
-__device__ __forceinline__ float pow2(float x) { return exp2f(x); }
+__device__ __forceinline__ float pow2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 // ---------------------------------------------------------------------------------------------
 // Runs of blocks.
@@ -414,11 +418,12 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 template <class T, class A>
 constexpr int terms_of() { return sizeof(A) == 2 ? 1 : (__is_same(T, __half) ? 2 : 3); }
 
-// Ring stages of 16 positions, and CTAs per SM: 130 to 190 KB of copies under way on each SM.
+// Ring stages of 16 positions, and CTAs per SM: the copies under way (100 KB on an SM) need few stages, the chain
+// of dependent steps from scores to output many warps.
+template <int DP, int NT>
+constexpr int mma_ctas() { return DP == 64 ? (NT == 1 ? 4 : 3) : DP == 128 ? (NT == 1 ? 3 : 2) : 1; }
 template <int DP>
-constexpr int mma_stages() { return DP == 64 ? 4 : DP == 128 ? 3 : 2; }
-template <int DP>
-constexpr int mma_ctas() { return DP == 64 ? 3 : DP == 128 ? 2 : 1; }
+constexpr int mma_stages() { return DP == 64 ? 3 : 2; }
 template <int DP>
 constexpr int mma_ring_bytes() { return mma_stages<DP>() * 16 * 2 * DP * 2; }  // of a warp
 // Operand words of the queries of a warp's segment: in registers where they are few.
@@ -430,7 +435,7 @@ template <class T, class A, int DP, int NT>
 constexpr int mma_query_bytes() { return mma_query_regs<T, A, DP, NT>() ? 0 : mma_query_words<T, A, DP, NT>() * 512; }  // of a warp
 
 template <class T, class A, int DP, int NT>
-__global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_kernel(const AttnArgs a) {
   constexpr int C = DP / 32, V = DP / 64, S = mma_stages<DP>(), TERMS = terms_of<T, A>(), WT = TERMS == 1 ? 2 : TERMS;
   constexpr int PIECES = 2 * C + 4 * V;  // 16-byte pieces of a stage per lane
   constexpr bool QREG = mma_query_regs<T, A, DP, NT>();
@@ -596,14 +601,14 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
         const uint4* const sv = sk + 2 * C * 32 + row * 4 + (quad ^ (row >> 1));            // value pieces of this lane
         const int p0 = c.b * kBlock + half * 16 + row;
         // ---- scores: 16 positions x heads
-        float s[NT][4];
+        float s[NT][4], s2[NT][4];  // two sums, so that the products' latencies overlap
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-        auto score = [&](float (&f)[4], const uint4& k0, const uint4& k1, const uint4& b) {
+          for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
+        auto score = [&](float (&f)[4], float (&f2)[4], const uint4& k0, const uint4& k1, const uint4& b) {
           mma<T>(f, k0.x, k1.x, k0.y, k1.y, b.x, b.y);
-          mma<T>(f, k0.z, k1.z, k0.w, k1.w, b.z, b.w);
+          mma<T>(f2, k0.z, k1.z, k0.w, k1.w, b.z, b.w);
         };
 #pragma unroll
         for (int x = 0; x < C; ++x) {
@@ -611,8 +616,12 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
 #pragma unroll
           for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) score(s[nt], k0, k1, query(x, t, nt));
+            for (int nt = 0; nt < NT; ++nt) score(s[nt], s2[nt], k0, k1, query(x, t, nt));
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
         if constexpr (TERMS > 1) {
           // A key of +-inf times a later term of a query (of any sign, or 0) is NaN: there the first
           // term alone gives the score that f32 products would.
@@ -626,7 +635,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP>()) attn_mma_kernel(
             for (int nt = 0; nt < NT; ++nt) {
               float f[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int x = 0; x < C; ++x) score(f, sk[(2 * x) * 32 + (lane ^ (x & 1) * 4)], sk[(2 * x + 1) * 32 + (lane ^ (x & 1) * 4)], query(x, 0, nt));
+              for (int x = 0; x < C; ++x) score(f, f, sk[(2 * x) * 32 + (lane ^ (x & 1) * 4)], sk[(2 * x + 1) * 32 + (lane ^ (x & 1) * 4)], query(x, 0, nt));
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (s[nt][e] != s[nt][e]) s[nt][e] = f[e];
@@ -1046,7 +1055,7 @@ int launch(const AttnArgs& a, int dp, int per_sm, size_t smem, cudaStream_t st) 
 
 template <class T, class A, int DP, int NT>
 int launch_mma(const AttnArgs& a, cudaStream_t st) {
-  return launch<attn_mma_kernel<T, A, DP, NT>>(a, DP, mma_ctas<DP>(), kAttnWarps * (mma_ring_bytes<DP>() + mma_query_bytes<T, A, DP, NT>()), st);
+  return launch<attn_mma_kernel<T, A, DP, NT>>(a, DP, mma_ctas<DP, NT>(), kAttnWarps * (mma_ring_bytes<DP>() + mma_query_bytes<T, A, DP, NT>()), st);
 }
 template <class T, class A>
 int run_mma(AttnArgs& a, cudaStream_t st) {
