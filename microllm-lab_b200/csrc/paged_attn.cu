@@ -59,17 +59,18 @@ struct AttnArgs {
 // ---------------------------------------------------------------------------------------------
 // Cached rows travel by asynchronous 16-byte copies into a warp's own ring in shared memory: many more bytes
 // are under way than registers could take, and no barrier is needed, only the lanes' counts of copies and the
-// warp in step.  Eight lanes copy 128 neighbouring bytes of a row: with 64 bytes a time, L2 sent every line
-// twice.  Each 16-byte piece goes to the place where the lane whose operand it is reads it, such that neither
-// the copies nor the reads meet in a bank.
+// warp in step.  Eight lanes copy 128 neighbouring bytes of a row into one 128-byte line: where either side
+// was split further, L2 sent lines twice (3 sequences to 100,003 f16: 206 us), and where the copies passed
+// through L1 they waited for room in what shared memory leaves of it (188 us).  Within a line the
+// 16-byte pieces are exchanged by an exclusive or of the row's number, so that no reads meet in a bank.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool ok) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(ok ? 16 : 0) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(ok ? 16 : 0) : "memory");
 }
 // The same for rows that are known to be there; further pieces of a row at constant distances.
 template <int TO, int FROM>
 __device__ __forceinline__ void copy16_at(uint32_t to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
 }
 // N pieces of a row, FROM bytes apart, to places TO bytes apart from the AT-th byte on.
 template <int AT, int TO, int FROM, int N, int I = 0>
@@ -469,12 +470,12 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
       }
     };
     look(1);
-    // places of this lane's copies within a stage: rows 4 i + part, 64-element chunks of 8 pieces
+    // A stage: keys, then values, each [64-element chunk][16 rows][8 pieces]; piece c of row p at c ^ 4 (p & 1) (keys),
+    // at c ^ (p & 6) (values).  This lane copies piece `chunk` of rows 4 x + part.
     const int part = lane >> 3, chunk = lane & 7;
     const uint32_t ring32 = smem_u32(smem + warp * mma_ring_bytes<DP>());
-    const uint32_t k_to = (chunk >> 2) * 1024 + ((part ^ (chunk >> 2)) * 4 + (chunk & 3)) * 16;
-    const uint32_t v_to = 2 * C * 512 + (part & 1) * 512 + chunk * 64;
-    const uint32_t v_even = v_to + ((part >> 1) ^ (chunk >> 1)) * 16, v_odd = v_to + ((part >> 1) ^ (chunk >> 1) ^ 2) * 16;
+    const uint32_t k_to = part * 128 + (chunk ^ (part & 1) * 4) * 16;
+    const uint32_t v_even = V * 2048 + part * 128 + (chunk ^ (part & 2)) * 16, v_odd = V * 2048 + part * 128 + (chunk ^ (part & 2) ^ 4) * 16;
     auto issue = [&](int i) {
       if (i < 2 * n) {
         const uint32_t to = ring32 + (i % S) * PIECES * 512;
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
           const int64_t at = __shfl_sync(0xffffffffu, off, (i & 1) * 16 + 4 * x + part);
           const T* const kr = kp + at + chunk * 8;
           const T* const vr = vp + at + chunk * 8;
-          const uint32_t kt = to + k_to + (x >> 1) * 512 + (x & 1) * 256, vt = to + (x & 1 ? v_odd : v_even) + (x >> 1) * 1024;
+          const uint32_t kt = to + k_to + x * 512, vt = to + (x & 1 ? v_odd : v_even) + x * 512;
           if (whole) {
             copy_rows<0, 2048, 128, V>(kt, kr);
             copy_rows<0, 2048, 128, V>(vt, vr);
@@ -597,8 +598,9 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
         __syncwarp();      // all lanes' copies are there, and all have read the last round's stage
         issue(i + S - 1);  // into that one
         if (c.b * kBlock + half * 16 >= c.len) continue;
-        const uint4* const sk = ring + (i % S) * PIECES * 32;                               // key pieces
-        const uint4* const sv = sk + 2 * C * 32 + row * 4 + (quad ^ (row >> 1));            // value pieces of this lane
+        const uint4* const sk = ring + (i % S) * PIECES * 32 + row * 8 + (quad ^ (row & 1) * 4);           // this lane's key pieces
+        const uint4* const sk2 = ring + (i % S) * PIECES * 32 + row * 8 + ((quad + 4) ^ (row & 1) * 4);    // of odd 32-element steps
+        const uint4* const sv = ring + ((i % S) * PIECES + 2 * C) * 32 + quad * 16 + (row ^ quad * 2);     // and value pieces
         const int p0 = c.b * kBlock + half * 16 + row;
         // ---- scores: 16 positions x heads
         float s[NT][4], s2[NT][4];  // two sums, so that the products' latencies overlap
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
         };
 #pragma unroll
         for (int x = 0; x < C; ++x) {
-          const uint4 k0 = sk[(2 * x) * 32 + (lane ^ (x & 1) * 4)], k1 = sk[(2 * x + 1) * 32 + (lane ^ (x & 1) * 4)];
+          const uint4 k0 = (x & 1 ? sk2 : sk)[(x >> 1) * 128], k1 = (x & 1 ? sk2 : sk)[(x >> 1) * 128 + 64];
 #pragma unroll
           for (int t = 0; t < TERMS; ++t)
 #pragma unroll
@@ -635,7 +637,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
             for (int nt = 0; nt < NT; ++nt) {
               float f[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int x = 0; x < C; ++x) score(f, f, sk[(2 * x) * 32 + (lane ^ (x & 1) * 4)], sk[(2 * x + 1) * 32 + (lane ^ (x & 1) * 4)], query(x, 0, nt));
+              for (int x = 0; x < C; ++x) score(f, f, (x & 1 ? sk2 : sk)[(x >> 1) * 128], (x & 1 ? sk2 : sk)[(x >> 1) * 128 + 64], query(x, 0, nt));
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (s[nt][e] != s[nt][e]) s[nt][e] = f[e];
@@ -689,7 +691,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
         for (int v = 0; v < V; ++v) {
           uint4 x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = sv[(4 * v + e) * 32];
+          for (int e = 0; e < 4; ++e) x[e] = sv[v * 128 + (e >> 1) * 64 + (e & 1) * 8];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             const uint32_t a0 = __byte_perm(word(x[0], y), word(x[1], y), 0x5410), a1 = __byte_perm(word(x[0], y), word(x[1], y), 0x7632);
@@ -814,7 +816,7 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
     look(1);
     const int part = lane >> 3, chunk = lane & 7;  // of the key copies: rows 4 i + part, 32-element chunks of 8 pieces
     const uint32_t ring32 = smem_u32(smem + warp * f32_ring_bytes<DP>());
-    const uint32_t k_to = (chunk >> 2) * R * 512 + ((part ^ (chunk >> 2)) * 4 + (chunk & 3)) * 16;
+    const uint32_t k_to = part * 128 + (chunk ^ (part & 1) * 4) * 16;  // as above
     auto issue = [&](int i) {
       if (i < PARTS * n) {
         const uint32_t to = ring32 + (i % S) * PIECES * 512;
@@ -824,14 +826,14 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
         for (int x = 0; x < 2 * R; ++x) {
           const int64_t at = __shfl_sync(0xffffffffu, off, first + 4 * x + part);
           const float* const kr = kp + at + chunk * 4;
-          const uint32_t kt = to + k_to + (x >> 1) * 512 + (x & 1) * 256;
+          const uint32_t kt = to + k_to + x * 512;
           if (whole) {
-            copy_rows<0, 2 * R * 512, 128, C / 2>(kt, kr);
+            copy_rows<0, P * 128, 128, C / 2>(kt, kr);
           } else {
 #pragma unroll 1
             for (int y = 0; y < C / 2; ++y) {
               const bool ok = at >= 0 && y * 32 + chunk * 4 < a.dim;
-              copy16(kt + y * 2 * R * 512, ok ? kr + y * 32 : kp, ok);
+              copy16(kt + y * P * 128, ok ? kr + y * 32 : kp, ok);
             }
           }
         }
@@ -901,7 +903,7 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
         for (int x = 0; x < C; ++x) {
           float4 key[R];
 #pragma unroll
-          for (int e = 0; e < R; ++e) key[e] = st[(x * R + e) * 32 + (lane ^ (x & 1) * 4)];
+          for (int e = 0; e < R; ++e) key[e] = st[((x >> 1) * P + row + 8 * e) * 8 + (((x & 1) * 4 + quad) ^ (row & 1) * 4)];
 #pragma unroll
           for (int h = 0; h < G; ++h) {
             const float4 q = *reinterpret_cast<const float4*>(qs + h * DP + x * 16 + quad * 4);
