@@ -254,7 +254,7 @@ __device__ __forceinline__ void join2(float& m, float& l, float4& o, float m1, f
 // Joins the parts that the warps left, each segment by the warp that has its first part here, and those of all
 // CTAs where this is the last one of a segment to come.
 template <class A, int DP>
-__device__ __noinline__ void join(const AttnArgs& a, const Run& r, const Joint& w) {
+__device__ __forceinline__ void join(const AttnArgs& a, const Run& r, const Joint& w) {
   struct Open {  // a segment whose last part this CTA left
     Part p;
     int first, parts;
@@ -349,7 +349,7 @@ __device__ __noinline__ void join(const AttnArgs& a, const Run& r, const Joint& 
 
 // Sequences without positions, and those whose length the table cannot hold.
 template <class A>
-__device__ __noinline__ void finish_empty(const AttnArgs& a) {
+__device__ __forceinline__ void finish_empty(const AttnArgs& a) {
   for (int s = blockIdx.x; s < a.n_seq; s += gridDim.x) {
     if (blocks_of(a, s)) continue;
     const float v = a.len[s] > 0 ? __int_as_float(0x7FC00000) : 0.f;
