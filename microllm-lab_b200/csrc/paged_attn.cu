@@ -52,6 +52,7 @@ struct AttnArgs {
   uint32_t* counter;  // [n_seq][n_kv][groups]
   float* part;        // [CTA][2]: o [group][dim], (m, l) [group]
   int rep, group_size, groups;  // query heads per kv head, of a group, groups of a kv head
+  int max_len;                  // positions that a row of the table can hold
   uint64_t page_mult;           // p / page_len = (p page_mult) >> page_shift for 0 <= p < 2^31
   int page_shift;
 };
@@ -92,10 +93,10 @@ __device__ __forceinline__ float pow2(float x) {
 // ---------------------------------------------------------------------------------------------
 // Runs of blocks.
 // ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ int blocks_of(const AttnArgs& a, int s) {
-  const int n = __ldg(a.len + s);
-  return n <= 0 || (int64_t)n > (int64_t)a.table_stride * a.page_len ? 0 : (n - 1) / kBlock + 1;
+__device__ __forceinline__ int blocks_of_len(const AttnArgs& a, int n) {
+  return n <= 0 || n > a.max_len ? 0 : (n - 1) / kBlock + 1;
 }
+__device__ __forceinline__ int blocks_of(const AttnArgs& a, int s) { return blocks_of_len(a, __ldg(a.len + s)); }
 
 // A place in the batch: block b of segment (seq, kv head, group).  Block numbers fit 31 bits (checked on the host
 // for the longest lengths that the table can hold).
@@ -103,8 +104,8 @@ struct Place {
   int seq, kv, group, b, nb, len;
   __device__ __forceinline__ void at_seq(const AttnArgs& a, int s) {
     seq = s;
-    nb = blocks_of(a, s);
     len = __ldg(a.len + s);
+    nb = blocks_of_len(a, len);
   }
   // To the next block; only called while more blocks follow.  True where another segment begins.
   __device__ __forceinline__ bool next(const AttnArgs& a) {
@@ -135,7 +136,7 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (a.n_seq + 31) / 32, s0 = min(lane * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
   uint32_t mine = 0, longest = 0;
-#pragma unroll 4
+#pragma unroll 8
   for (int s = s0; s < s1; ++s) {
     const uint32_t nb = blocks_of(a, s);
     mine += nb;
@@ -170,16 +171,29 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a) {
   const uint32_t end = min(r.u0 + r.q, all), each = (end - r.u0 + kAttnWarps - 1) / kAttnWarps, u = r.u0 + warp * each;
   if (u >= end) return r;
   r.n = min(each, end - u);
-  // the lane whose sequences hold block u, then the one of them
+  // the lane whose sequences hold block u, then the one of them, 32 at a time
   const int who = __ffs(__ballot_sync(0xffffffffu, u < upto * per_seq)) - 1;
   uint32_t before = __shfl_sync(0xffffffffu, upto - mine, who) * per_seq;
-  int s = who * per;
-  for (;; ++s) {
-    const uint32_t nb = blocks_of(a, s) * per_seq;
-    if (u < before + nb) break;
-    before += nb;
+  for (int s = who * per;; s += 32) {
+    const int len = s + lane < a.n_seq ? __ldg(a.len + s + lane) : 0;
+    const uint32_t nb = blocks_of_len(a, len);
+    uint32_t sum = nb;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, u < before + sum * per_seq);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      r.from.seq = s + at;
+      r.from.nb = __shfl_sync(0xffffffffu, nb, at);
+      r.from.len = __shfl_sync(0xffffffffu, len, at);
+      before += __shfl_sync(0xffffffffu, sum - nb, at) * per_seq;
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31) * per_seq;
   }
-  r.from.at_seq(a, s);
   const uint32_t j = (u - before) / r.from.nb;
   r.from.b = u - before - j * r.from.nb;
   r.from.kv = j / a.groups;
@@ -203,10 +217,11 @@ __device__ __forceinline__ int64_t row_offset(const AttnArgs& a, const Place& c,
 // A part of a segment: what one run holds of it.
 struct Part {
   int seq, kv, group, b0, blocks, nb;  // blocks 0: none
+  __device__ __forceinline__ uint32_t segment(const AttnArgs& a) const { return ((uint32_t)seq * a.n_kv + kv) * a.groups + group; }
   __device__ __forceinline__ int first_head(const AttnArgs& a) const { return kv * a.rep + group * a.group_size; }
   __device__ __forceinline__ int heads(const AttnArgs& a) const { return min(a.rep - group * a.group_size, a.group_size); }
-  __device__ __forceinline__ bool same(const Part& o) const { return seq == o.seq && kv == o.kv && group == o.group; }
 };
+
 // The parts that a CTA's warps leave for the join: of a run's first segment (slot 0) and of its last (slot
 // 1).  m is in units of log 2.  A page id outside the pool makes l, and with it the result, NaN.
 struct Joint {
@@ -270,10 +285,10 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Run& r, const Join
     if (!p.blocks || (i && p.b0)) continue;  // none, or it goes on from another warp's
     int have = p.blocks, end = i + 1;        // parts i .. end - 1 are of this segment
     for (; end < 2 * kAttnWarps; ++end) {
-      const Part& o = w.part[end];
-      if (!o.blocks) continue;
-      if (!o.same(p)) break;
-      have += o.blocks;
+      const int more = w.part[end].blocks;
+      if (!more) continue;
+      if (w.part[end].b0 == 0) break;  // another segment
+      have += more;
     }
     const bool done = have == p.nb;
     const int side = p.b0 == 0, items = p.heads(a) * quads;
@@ -302,7 +317,7 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Run& r, const Join
       // which CTAs have a part, by the segment's first block: one that began in this run goes on to its end
       const uint32_t start = side ? r.u0 + r.q - have : r.u0 - p.b0, first = start / r.q;
       const int parts = (int)((start + p.nb - 1) / r.q - first) + 1;
-      uint32_t* const c = a.counter + ((int64_t)p.seq * a.n_kv + p.kv) * a.groups + p.group;
+      uint32_t* const c = a.counter + p.segment(a);
       if (atomicAdd(c, 1u) == (uint32_t)parts - 1) {
         *c = 0;
         open[side] = Open{p, (int)first, parts};
@@ -315,31 +330,39 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Run& r, const Join
     const Open& s = open[side];
     if (!s.parts) continue;
     __threadfence();
-    // every fourth part by each warp, then the four in order: (m, l) and o of [warp][item] at the rings' place
-    const int items = s.p.heads(a) * quads;
+    // few parts: a thread takes all of an item's; many: every fourth by each warp, then the four in order, as
+    // (m, l) and o of [warp][item] at the rings' place
+    const bool many = s.parts > 8;
+    const int items = s.p.heads(a) * quads, step = many ? kAttnWarps : 1;
     float2* const ml = reinterpret_cast<float2*>(w.ring);
     float4* const os = reinterpret_cast<float4*>(ml + kAttnWarps * items);
 #pragma unroll 1
-    for (int x = lane; x < items; x += 32) {
+    for (int x = many ? lane : tid; x < items; x += many ? 32 : kAttnThreads) {
       const int h = x / quads, d = (x - h * quads) * 4;
       float m = -INFINITY, l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (int k = warp; k < s.parts; k += kAttnWarps) {
+      for (int k = many ? warp : 0; k < s.parts; k += step) {
         const float* q = a.part + ((size_t)(s.first + k) * 2 + (k == 0)) * slot;
         const float2 mk = __ldcg(reinterpret_cast<const float2*>(q + a.group_size * a.dim) + h);
         join2(m, l, o, mk.x, mk.y, __ldcg(reinterpret_cast<const float4*>(q + h * a.dim + d)));
       }
-      ml[warp * items + x] = make_float2(m, l);
-      os[warp * items + x] = o;
+      if (many) {
+        ml[warp * items + x] = make_float2(m, l);
+        os[warp * items + x] = o;
+      } else {
+        write_out<A>(a, s.p, h, d, o, l);
+        if (d == 0) write_lse(a, s.p, h, m, l);
+      }
     }
+    if (!many) continue;
     __syncthreads();
 #pragma unroll 1
     for (int x = tid; x < items; x += kAttnThreads) {
       const int h = x / quads, d = (x - h * quads) * 4;
       float m = -INFINITY, l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = 0; k < min(kAttnWarps, s.parts); ++k) join2(m, l, o, ml[k * items + x].x, ml[k * items + x].y, os[k * items + x]);
+      for (int k = 0; k < kAttnWarps; ++k) join2(m, l, o, ml[k * items + x].x, ml[k * items + x].y, os[k * items + x]);
       write_out<A>(a, s.p, h, d, o, l);
       if (d == 0) write_lse(a, s.p, h, m, l);
     }
@@ -423,10 +446,9 @@ constexpr int terms_of() { return sizeof(A) == 2 ? 1 : (__is_same(T, __half) ? 2
 // of dependent steps from scores to output many warps.
 template <int DP, int NT>
 constexpr int mma_ctas() { return DP == 64 ? (NT == 1 ? 4 : 3) : DP == 128 ? (NT == 1 ? 3 : 2) : 1; }
+constexpr int kMmaStages = 2;
 template <int DP>
-constexpr int mma_stages() { return DP == 64 ? 3 : 2; }
-template <int DP>
-constexpr int mma_ring_bytes() { return mma_stages<DP>() * 16 * 2 * DP * 2; }  // of a warp
+constexpr int mma_ring_bytes() { return kMmaStages * 16 * 2 * DP * 2; }  // of a warp
 // Operand words of the queries of a warp's segment: in registers where they are few.
 template <class T, class A, int DP, int NT>
 constexpr int mma_query_words() { return (DP / 32) * terms_of<T, A>() * NT; }  // uint4 of a lane
@@ -437,7 +459,7 @@ constexpr int mma_query_bytes() { return mma_query_regs<T, A, DP, NT>() ? 0 : mm
 
 template <class T, class A, int DP, int NT>
 __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_kernel(const AttnArgs a) {
-  constexpr int C = DP / 32, V = DP / 64, S = mma_stages<DP>(), TERMS = terms_of<T, A>(), WT = TERMS == 1 ? 2 : TERMS;
+  constexpr int C = DP / 32, V = DP / 64, S = kMmaStages, TERMS = terms_of<T, A>(), WT = TERMS == 1 ? 2 : TERMS;
   constexpr int PIECES = 2 * C + 4 * V;  // 16-byte pieces of a stage per lane
   constexpr bool QREG = mma_query_regs<T, A, DP, NT>();
   extern __shared__ __align__(16) uint8_t smem[];
@@ -1118,6 +1140,7 @@ extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d
   a.rep = n_heads / kv->n_kv_heads;
   int bits = 0;  // ceil(log2 page_len)
   while (((int64_t)1 << bits) < kv->page_len) ++bits;
+  a.max_len = (int)std::min<int64_t>((int64_t)table_stride * kv->page_len, 0x7FFFFFFF);
   a.page_shift = 31 + bits;
   a.page_mult = ((uint64_t)1 << a.page_shift) / kv->page_len + 1;
   a.counter = static_cast<uint32_t*>(d_ws);
