@@ -18,8 +18,8 @@
 //     or of a 512th of it where they are too many for a list;
 //   - and by halving, one pass per bit, where those are too many as well (thousands of tokens of one value).
 // A short list is not sorted either: several threads per token count, and weigh, what precedes it.
-// Every CTA of a cluster keeps its own copy of a list and comes to the same edge, so that they meet at a
-// barrier only to exchange a maximum, a histogram, a list or a sum.
+// The CTAs of a cluster meet at a barrier only to exchange a maximum, a histogram, a list (the first one's) or
+// a sum.
 //
 // Of a few microseconds per row much goes into fetching instructions, so the code is kept small: what runs
 // once is called, not inlined, and the passes over the row either test 16 bytes at a time and do the rest
@@ -43,7 +43,7 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleList = 2048;   // tokens of a list
-constexpr int kShortList = 256;     // tokens of a list that is counted instead of sorted
+constexpr int kShortList = 384;     // tokens of a list that is counted (the square of them) instead of sorted
 constexpr int kSampleMaxK = 512;    // top_k that starts from the threads' maxima
 constexpr int kSteps = 512;         // steps of a histogram level
 constexpr int kMaxCluster = 16;
@@ -81,7 +81,7 @@ struct alignas(16) SampleShared {
   uint64_t slot[2][kMaxCluster][2];       // two words from every CTA of the cluster
   uint64_t weights[kShortList];
   uint64_t wsum[kSampleWarps];
-  uint64_t word;
+  uint64_t word, word2;
   uint32_t pick, count[2];
 };
 
@@ -183,7 +183,7 @@ struct Place {
 };
 __device__ __noinline__ Place place_of(SampleShared& sh, int n, float m, float r) {
   Place q;
-  q.team = n <= 32 ? 32 : n <= 64 ? 16 : n <= 128 ? 8 : 4;
+  q.team = n <= 32 ? 32 : n <= 64 ? 16 : n <= 128 ? 8 : n <= 256 ? 4 : 2;
   if (threadIdx.x < n) sh.weights[threadIdx.x] = weight_of(value_of(sh.list[threadIdx.x]), m, r);
   __syncthreads();
   q.t = threadIdx.x / q.team;
@@ -296,12 +296,17 @@ struct Sampler {
     }
     sync();
   }
-  // Gathers the tokens with f(value, index) into every CTA's list, in no order.  Returns their number; a list
-  // is cut off at its length.
+  // Gathers the tokens with f(value, index) into the first CTA's list, in no order.  Returns their number; the
+  // list is cut off at its length.
   template <class F>
   __device__ __forceinline__ int gather(F f) {
     listed ^= 1;
-    uint32_t* const count = &sh.count[listed];
+    uint32_t* count = &sh.count[listed];
+    uint64_t* list = sh.list;
+    if (ranks > 1) {
+      count = cg::this_cluster().map_shared_rank(count, 0);
+      list = cg::this_cluster().map_shared_rank(list, 0);
+    }
     int b, e;
     share(b, e);
 #pragma unroll 1
@@ -310,18 +315,15 @@ struct Sampler {
       while (mask) {
         const int i = c * E + __ffs((int)mask) - 1;
         mask &= mask - 1;
-        const uint64_t o = order_of(to_f32(x[i]), base + i);
-#pragma unroll 1
-        for (int q = 0; q < ranks; ++q) {
-          const uint32_t at = atomicAdd(ranks > 1 ? cg::this_cluster().map_shared_rank(count, q) : count, 1u);
-          if (at < kSampleList) *(ranks > 1 ? cg::this_cluster().map_shared_rank(&sh.list[at], q) : &sh.list[at]) = o;
-        }
+        const uint32_t at = atomicAdd(count, 1u);
+        if (at < kSampleList) list[at] = order_of(to_f32(x[i]), base + i);
       }
     }
     sync();
     const int n = (int)*(volatile uint32_t*)count;
-    __syncthreads();
-    if (threadIdx.x == 0) *count = 0;
+    // The other count was read by all before the barrier above, and is used again only after another one: there is
+    // an exchange between any two gathers.  (This one may still be read by other CTAs.)
+    if (rank == 0 && threadIdx.x == 0) sh.count[listed ^ 1] = 0;
     return n;
   }
 
@@ -352,7 +354,7 @@ struct Sampler {
     sync();
     uint64_t v = 0;
     if (threadIdx.x < kSteps) {
-#pragma unroll 1
+#pragma unroll 4
       for (int c = 0; c < ranks; ++c) {  // every CTA sums all: none has to tell the others
         const SampleShared* o = ranks == 1 ? &sh : cg::this_cluster().map_shared_rank(&sh, c);
         v += (uint64_t)o->hi[hist][threadIdx.x] << 32 | o->lo[hist][threadIdx.x];
@@ -383,17 +385,25 @@ struct Sampler {
     }
     return (int)sum(yes);
   }
-  // The edge within a list of n tokens with `above` before them.
+  // The edge within a list of n tokens with `above` before them: the first CTA finds it and tells the others.
   __device__ __forceinline__ void edge_of_list(bool mass, int n, uint64_t above) {
-    if (n <= kShortList) {
-      const Place q = place_of(sh, n, m, r);
-      const bool keep = q.t >= 0 && taken(mass, above + (mass ? q.weight_before : q.count_before));
-      set_edge(~most(keep ? ~q.order : 0));
-    } else {
-      cta_sort(sh.list, n);
-      set_edge(sh.list[max(taken_of_sorted(mass, n, above), 1) - 1]);
+    uint64_t o = 0;
+    if (rank == 0) {
+      if (n <= kShortList) {
+        const Place q = place_of(sh, n, m, r);
+        const bool keep = q.t >= 0 && taken(mass, above + (mass ? q.weight_before : q.count_before));
+        o = ~most(keep ? ~q.order : 0);
+      } else {
+        cta_sort(sh.list, n);
+        o = sh.list[max(taken_of_sorted(mass, n, above), 1) - 1];
+        __syncthreads();  // the list may be written again
+      }
     }
-    __syncthreads();  // the list may be written again
+    if (ranks > 1) {
+      exchange(o, 0);
+      o = sh.slot[flip][0][0];
+    }
+    set_edge(o);
   }
   // The edge among the tokens of step s1 where they are too many for a list: by 512ths of the step, and where
   // those of one are too many as well, by halving: the lowest number above which little enough lies.
@@ -467,46 +477,65 @@ struct Sampler {
     if (a.kept) a.kept[rw] = (int32_t)kept;
     if (a.logprob) a.logprob[rw] = gap(v) - logf(__fdiv_rn((float)(double)z, kOne));
   }
-  // Everything from a list that holds the top k tokens: the edge of top_p, the kept weight and the id.
-  __device__ __forceinline__ uint64_t finish_short(const SampleArgs& a, int rw, float u, int n) {
-    Place q = place_of(sh, n, m, r);
-    bool keep = q.t >= 0 && q.count_before < k;
-    if (!(p >= 1.f)) {
-      want = (double)p * (double)sum(keep ? q.w : 0);
-      keep = keep && taken(true, q.weight_before);
+  // Everything from the first CTA's list, which holds the top k tokens: the edge of top_p, the kept weight and
+  // the id.  Leaves the edge and Z for the others in sh.word and sh.word2.
+  __device__ __forceinline__ void finish_list(const SampleArgs& a, int rw, float u, int n) {
+    int t = -1, team = 1;  // this thread's kept token, and how many neighbours share it
+    uint64_t order = 0, w = 0;
+    if (n <= kShortList) {
+      const Place q = place_of(sh, n, m, r);
+      t = q.t;
+      team = q.team;
+      order = q.order;
+      bool keep = t >= 0 && q.count_before < k;
+      if (!(p >= 1.f)) {
+        want = (double)p * (double)sum(keep ? q.w : 0);
+        keep = keep && taken(true, q.weight_before);
+      }
+      if (a.probs) {
+        const uint64_t o = ~most(keep ? ~order : 0);
+        if (threadIdx.x == 0) sh.word = o;
+      }
+      w = keep && q.w >= least ? q.w : 0;
+    } else {
+      cta_sort(sh.list, n);
+      n = (int)min((uint64_t)n, k);
+      if (!(p >= 1.f)) {
+        uint64_t all = 0;
+        for (int i = threadIdx.x; i < n; i += kSampleThreads) all += weight(value_of(sh.list[i]));
+        want = (double)p * (double)sum(all);
+        n = taken_of_sorted(true, n, 0);
+      }
+      if (threadIdx.x == 0) sh.word = sh.list[n - 1];
+      if (n > kShortList) return finish_sorted(a, rw, u, n);
+      team = n <= 32 ? 32 : n <= 64 ? 16 : n <= 128 ? 8 : n <= 256 ? 4 : 2;
+      t = threadIdx.x / team;
+      if (t >= n) t = -1;
+      order = t < 0 ? 0 : sh.list[t];
+      if (t >= 0 && (threadIdx.x & (team - 1)) == 0) w = weight(value_of(order));
+      if (w < least) w = 0;
     }
-    if (a.probs) set_edge(~most(keep ? ~q.order : 0));
-    if (!keep || q.w < least) q.w = 0;
-    const uint64_t z = sum(q.w), at = aim(u, z);
-    const int kept = __syncthreads_count(q.w > 0);
-    if (q.t >= 0 && (threadIdx.x & (q.team - 1)) == 0) sh.weights[q.t] = q.w;
+    const uint64_t z = sum(w), at = aim(u, z);
+    const int kept = __syncthreads_count(w > 0);
+    if (t >= 0 && (threadIdx.x & (team - 1)) == 0) sh.weights[t] = w;
     __syncthreads();
-    uint64_t b = 0;
-    for (int j = threadIdx.x & (q.team - 1); j < n; j += q.team)
-      if ((uint32_t)sh.list[j] > (uint32_t)q.order) b += sh.weights[j];  // lower indexes
-    for (int o = q.team >> 1; o > 0; o >>= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
-    if (rank == 0 && b <= at && at < b + q.w) answer(a, rw, index_of(q.order), value_of(q.order), z, kept);
-    return z;
+    uint64_t b = 0;  // kept weight at lower indexes
+    for (int j = threadIdx.x & (team - 1); j < n; j += team)
+      if ((uint32_t)sh.list[j] > (uint32_t)order) b += sh.weights[j];
+    for (int o = team >> 1; o > 0; o >>= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
+    if (b <= at && at < b + w) answer(a, rw, index_of(order), value_of(order), z, kept);
+    if (threadIdx.x == 0) sh.word2 = z;
   }
-  __device__ __forceinline__ uint64_t finish_long(const SampleArgs& a, int rw, float u, int n) {
-    cta_sort(sh.list, n);
-    int c = (int)min((uint64_t)n, k);
-    if (!(p >= 1.f)) {
-      uint64_t all = 0;
-      for (int i = threadIdx.x; i < c; i += kSampleThreads) all += weight(value_of(sh.list[i]));
-      want = (double)p * (double)sum(all);
-      c = taken_of_sorted(true, c, 0);
-    }
-    set_edge(sh.list[c - 1]);
+  // The same for a sorted list of n kept tokens that is not short: sorted again, by rising index.
+  __device__ __forceinline__ void finish_sorted(const SampleArgs& a, int rw, float u, int n) {
     __syncthreads();
-    // the kept ones by rising index: sorted by (~index, key)
-    for (int i = threadIdx.x; i < c; i += kSampleThreads) {
+    for (int i = threadIdx.x; i < n; i += kSampleThreads) {
       const uint64_t v = sh.list[i];
       sh.list[i] = v << 32 | v >> 32;
     }
     __syncthreads();
-    cta_sort(sh.list, c);
-    const int per = (c + kSampleThreads - 1) / kSampleThreads, i0 = threadIdx.x * per, i1 = min(i0 + per, c);
+    cta_sort(sh.list, n);
+    const int per = (n + kSampleThreads - 1) / kSampleThreads, i0 = threadIdx.x * per, i1 = min(i0 + per, n);
     uint64_t mass = 0, some = 0;
     for (int i = i0; i < i1; ++i) {
       const uint64_t w = weight(of_key((uint32_t)sh.list[i]));
@@ -518,7 +547,7 @@ struct Sampler {
     const Scan q = cta_scan(sh.wsum, mass);
     const uint64_t z = q.all, at = aim(u, z);
     uint64_t b = q.before;
-    if (rank == 0 && b <= at && at < b + mass) {
+    if (b <= at && at < b + mass) {
       for (int i = i0; i < i1; ++i) {
         const uint64_t v = sh.list[i];
         uint64_t w = weight(of_key((uint32_t)v));
@@ -530,7 +559,7 @@ struct Sampler {
         b += w;
       }
     }
-    return z;
+    if (threadIdx.x == 0) sh.word2 = z;
   }
 };
 
@@ -646,7 +675,15 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     if (s.total < s.k) to = kFar;  // fewer threads than k hold a token of weight
     const int c = s.gather([&](float v, int) { return s.gap(v) > to; });
     done = c <= kSampleList;
-    if (done) z = c <= kShortList ? s.finish_short(a, rw, u, c) : s.finish_long(a, rw, u, c);
+    if (done) {
+      if (s.rank == 0) s.finish_list(a, rw, u, c);
+      if (probs) {
+        s.sync();
+        const SampleShared* o = s.ranks > 1 ? cg::this_cluster().map_shared_rank(&sh, 0) : &sh;
+        s.set_edge(o->word);
+        z = o->word2;
+      }
+    }
   }
   if (!done) {
 #pragma unroll 1
