@@ -17,7 +17,9 @@
 //   - otherwise by a histogram of tokens or weight over 512 such steps, then among the tokens of one step,
 //     or of a 512th of it where they are too many for a list;
 //   - and by halving, one pass per bit, where those are too many as well (thousands of tokens of one value).
-// A short list is not sorted either: several threads per token count, and weigh, what precedes it.
+// A short list is not sorted either: several threads per token count, and weigh, what precedes it.  A longer
+// one goes through the same two levels of steps until few enough are left, for the id by steps of the index;
+// it is sorted where one step holds too many.
 // The CTAs of a cluster meet at a barrier only to exchange a maximum, a histogram, a list (the first one's) or
 // a sum.
 //
@@ -27,8 +29,8 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <cstdlib>
 #include <atomic>
+#include <cstdlib>
 #include <climits>
 
 #include "device_common.cuh"
@@ -43,7 +45,8 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleList = 2048;   // tokens of a list
-constexpr int kShortList = 384;     // tokens of a list that is counted (the square of them) instead of sorted
+constexpr int kShortList = 192;     // tokens of a list that is counted at once (the square of them)
+constexpr int kMiniList = 64;       // tokens of a step of a longer list
 constexpr int kSampleMaxK = 512;    // top_k that starts from the threads' maxima
 constexpr int kSteps = 512;         // steps of a histogram level
 constexpr int kMaxCluster = 16;
@@ -79,10 +82,10 @@ struct alignas(16) SampleShared {
   uint64_t list[kSampleList];
   uint32_t lo[2][kSteps], hi[2][kSteps];  // a histogram of 64-bit sums
   uint64_t slot[2][kMaxCluster][2];       // two words from every CTA of the cluster
-  uint64_t weights[kShortList];
+  uint64_t weights[kShortList], mini[kMiniList];
   uint64_t wsum[kSampleWarps];
   uint64_t word, word2;
-  uint32_t pick, count[2];
+  uint32_t pick, count[2], minis;
 };
 
 // ---- over a CTA's threads
@@ -183,7 +186,7 @@ struct Place {
 };
 __device__ __noinline__ Place place_of(SampleShared& sh, int n, float m, float r) {
   Place q;
-  q.team = n <= 32 ? 32 : n <= 64 ? 16 : n <= 128 ? 8 : n <= 256 ? 4 : 2;
+  q.team = n <= 32 ? 32 : n <= 64 ? 16 : n <= 128 ? 8 : 4;
   if (threadIdx.x < n) sh.weights[threadIdx.x] = weight_of(value_of(sh.list[threadIdx.x]), m, r);
   __syncthreads();
   q.t = threadIdx.x / q.team;
@@ -192,11 +195,13 @@ __device__ __noinline__ Place place_of(SampleShared& sh, int n, float m, float r
   q.w = q.t < 0 || (threadIdx.x & (q.team - 1)) ? 0 : sh.weights[q.t];
   q.weight_before = 0;
   q.count_before = 0;
-  for (int j = threadIdx.x & (q.team - 1); j < n; j += q.team)
-    if (sh.list[j] > q.order) {
-      ++q.count_before;
-      q.weight_before += sh.weights[j];
-    }
+#pragma unroll 4
+  for (int j = threadIdx.x & (q.team - 1); j < n; j += q.team) {
+    const uint64_t w = sh.weights[j];
+    const bool higher = sh.list[j] > q.order;
+    q.count_before += higher;
+    q.weight_before += higher ? w : 0;
+  }
   for (int o = q.team >> 1; o > 0; o >>= 1) {
     q.count_before += __shfl_xor_sync(0xffffffffu, q.count_before, o);
     q.weight_before += __shfl_xor_sync(0xffffffffu, q.weight_before, o);
@@ -327,6 +332,27 @@ struct Sampler {
     return n;
   }
 
+  // Adds to a 64-bit sum.  The carry out of the low word is seen by the one thread that caused it: exact.
+  __device__ __forceinline__ static void add(uint32_t* lo, uint32_t* hi, uint64_t w) {
+    const uint32_t l = (uint32_t)w, was = atomicAdd(lo, l), h = (uint32_t)(w >> 32) + (was + l < l);
+    if (h) atomicAdd(hi, h);
+  }
+  // Thread s has the sum v of step s (0 past the last): the last step that holds something and before which
+  // b with taken(b) lies.  `above`: what lies before step 0, then before that step; total: the sum of all.
+  template <class F>
+  __device__ __forceinline__ uint32_t choose(uint64_t v, bool limit, uint64_t& above, F taken) {
+    const Scan q = cta_scan(sh.wsum, v);
+    const uint64_t b = above + q.before;
+    total = q.all;
+    if (limit) want = (double)p * (double)total;  // top_p's limit is of this histogram's sum
+    if (v && taken(b)) atomicMax(&sh.pick, threadIdx.x);
+    __syncthreads();
+    const uint32_t s = sh.pick;
+    if (threadIdx.x == s) sh.word = b;
+    __syncthreads();
+    above = sh.word;
+    return s;
+  }
   // A cleared histogram of f's tokens: f gives a token's step, or none (>= kSteps).
   template <class F>
   __device__ __forceinline__ void fill(bool mass, F f) {
@@ -342,9 +368,7 @@ struct Sampler {
       if (s >= kSteps) continue;
       uint64_t w = 1;
       if (mass) w = weigh(g);
-      // the carry out of the low word is seen by the one thread that caused it, so the sum is exact
-      const uint32_t l = (uint32_t)w, was = atomicAdd(lo + s, l), h = (uint32_t)(w >> 32) + (was + l < l);
-      if (h) atomicAdd(hi + s, h);
+      add(lo + s, hi + s, w);
     }
   }
   // Of the cluster's histogram: the last step, counted from the top, whose first token is taken.  `above`:
@@ -360,17 +384,7 @@ struct Sampler {
         v += (uint64_t)o->hi[hist][threadIdx.x] << 32 | o->lo[hist][threadIdx.x];
       }
     }
-    const Scan q = cta_scan(sh.wsum, v);
-    const uint64_t b = above + q.before;
-    total = q.all;
-    if (limit) want = (double)p * (double)total;
-    if (v && taken(mass, b)) atomicMax(&sh.pick, threadIdx.x);
-    __syncthreads();
-    const uint32_t s = sh.pick;
-    if (threadIdx.x == s) sh.word = b;
-    __syncthreads();
-    above = sh.word;
-    return s;
+    return choose(v, limit, above, [&](uint64_t b) { return taken(mass, b); });
   }
   // How many of a sorted list's n tokens are taken, `above` before them.
   __device__ __forceinline__ int taken_of_sorted(bool mass, int n, uint64_t above) {
@@ -385,6 +399,60 @@ struct Sampler {
     }
     return (int)sum(yes);
   }
+  // The same over this CTA's list: step(o) of its tokens, or none (>= kSteps), each with weight(o).
+  template <class S, class W, class F>
+  __device__ __forceinline__ uint32_t list_level(int n, uint64_t& above, S step, W weight, F taken) {
+    uint32_t* const lo = sh.lo[hist];  // nobody else reads it any more
+    uint32_t* const hi = sh.hi[hist];
+    __syncthreads();
+    if (threadIdx.x < kSteps) lo[threadIdx.x] = hi[threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.pick = sh.minis = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kSampleThreads) {
+      const uint64_t o = sh.list[i];
+      const uint32_t s = step(o);
+      if (s < kSteps) add(lo + s, hi + s, weight(o));
+    }
+    __syncthreads();
+    const int s = threadIdx.x;
+    return choose(s < kSteps ? (uint64_t)hi[s] << 32 | lo[s] : 0, false, above, taken);
+  }
+  // The list's tokens with f(o), in no order; false when they are too many.
+  template <class F>
+  __device__ __forceinline__ bool mini_list(int n, F f) {
+    for (int i = threadIdx.x; i < n; i += kSampleThreads) {
+      const uint64_t o = sh.list[i];
+      if (!f(o)) continue;
+      const uint32_t at = atomicAdd(&sh.minis, 1u);
+      if (at < kMiniList) sh.mini[at] = o;
+    }
+    __syncthreads();
+    return sh.minis <= kMiniList;
+  }
+  // The edge among the list's tokens above the present one, `above` before them; false: undecided, by a step
+  // with too many tokens.
+  __device__ __forceinline__ bool edge_in_list(bool mass, int n, uint64_t above) {
+    auto weigh_one = [&](uint64_t o) { return mass ? weight(value_of(o)) : (uint64_t)1; };
+    auto is_taken = [&](uint64_t b) { return taken(mass, b); };
+    auto in = [&](uint64_t o) { return above_edge(value_of(o), index_of(o)) && gap(value_of(o)) > kFar; };
+    const uint32_t s1 = list_level(n, above, [&](uint64_t o) { return in(o) ? whole(gap(value_of(o)) * -16.f) : kSteps; }, weigh_one, is_taken);
+    auto fine = [&](uint64_t o) { return whole(gap(value_of(o)) * -8192.f); };
+    const uint32_t s2 = list_level(n, above, [&](uint64_t o) { return in(o) && fine(o) / kSteps == s1 ? fine(o) % kSteps : kSteps; },
+                                   weigh_one, is_taken);
+    if (!mini_list(n, [&](uint64_t o) { return in(o) && fine(o) == s1 * kSteps + s2; })) return false;
+    const int c = sh.minis;
+    if (threadIdx.x < c) sh.weights[threadIdx.x] = weigh_one(sh.mini[threadIdx.x]);
+    __syncthreads();
+    uint64_t low = 0;
+    if (threadIdx.x < c) {
+      const uint64_t o = sh.mini[threadIdx.x];
+      uint64_t b = above;
+      for (int j = 0; j < c; ++j) b += sh.mini[j] > o ? sh.weights[j] : 0;
+      if (taken(mass, b)) low = ~o;
+    }
+    set_edge(~most(low));
+    return true;
+  }
   // The edge within a list of n tokens with `above` before them: the first CTA finds it and tells the others.
   __device__ __forceinline__ void edge_of_list(bool mass, int n, uint64_t above) {
     uint64_t o = 0;
@@ -393,11 +461,13 @@ struct Sampler {
         const Place q = place_of(sh, n, m, r);
         const bool keep = q.t >= 0 && taken(mass, above + (mass ? q.weight_before : q.count_before));
         o = ~most(keep ? ~q.order : 0);
+      } else if (edge_in_list(mass, n, above)) {
+        o = order_of(xe, ie);
       } else {
         cta_sort(sh.list, n);
         o = sh.list[max(taken_of_sorted(mass, n, above), 1) - 1];
-        __syncthreads();  // the list may be written again
       }
+      __syncthreads();  // the list may be written again
     }
     if (ranks > 1) {
       exchange(o, 0);
@@ -498,35 +568,81 @@ struct Sampler {
       }
       w = keep && q.w >= least ? q.w : 0;
     } else {
-      cta_sort(sh.list, n);
-      n = (int)min((uint64_t)n, k);
-      if (!(p >= 1.f)) {
-        uint64_t all = 0;
-        for (int i = threadIdx.x; i < n; i += kSampleThreads) all += weight(value_of(sh.list[i]));
-        want = (double)p * (double)sum(all);
-        n = taken_of_sorted(true, n, 0);
-      }
-      if (threadIdx.x == 0) sh.word = sh.list[n - 1];
-      if (n > kShortList) return finish_sorted(a, rw, u, n);
-      team = n <= 32 ? 32 : n <= 64 ? 16 : n <= 128 ? 8 : n <= 256 ? 4 : 2;
-      t = threadIdx.x / team;
-      if (t >= n) t = -1;
-      order = t < 0 ? 0 : sh.list[t];
-      if (t >= 0 && (threadIdx.x & (team - 1)) == 0) w = weight(value_of(order));
-      if (w < least) w = 0;
+      return finish_long(a, rw, u, n);
     }
     const uint64_t z = sum(w), at = aim(u, z);
     const int kept = __syncthreads_count(w > 0);
     if (t >= 0 && (threadIdx.x & (team - 1)) == 0) sh.weights[t] = w;
     __syncthreads();
     uint64_t b = 0;  // kept weight at lower indexes
-    for (int j = threadIdx.x & (team - 1); j < n; j += team)
-      if ((uint32_t)sh.list[j] > (uint32_t)order) b += sh.weights[j];
+#pragma unroll 4
+    for (int j = threadIdx.x & (team - 1); j < n; j += team) {
+      const uint64_t v = sh.weights[j];
+      b += (uint32_t)sh.list[j] > (uint32_t)order ? v : 0;
+    }
     for (int o = team >> 1; o > 0; o >>= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
     if (b <= at && at < b + w) answer(a, rw, index_of(order), value_of(order), z, kept);
     if (threadIdx.x == 0) sh.word2 = z;
   }
-  // The same for a sorted list of n kept tokens that is not short: sorted again, by rising index.
+  // The same for a list that is not short.
+  __device__ __forceinline__ void finish_long(const SampleArgs& a, int rw, float u, int n) {
+    bool sure = (uint64_t)n <= k || edge_in_list(false, n, 0);
+    auto kept_weight = [&](uint64_t o) -> uint64_t {
+      if (!above_edge(value_of(o), index_of(o))) return 0;
+      const uint64_t w = weight(value_of(o));
+      return w < least ? 0 : w;
+    };
+    if (sure && !(p >= 1.f)) {
+      uint64_t all = 0;
+      for (int i = threadIdx.x; i < n; i += kSampleThreads) {
+        const uint64_t o = sh.list[i];
+        if (above_edge(value_of(o), index_of(o))) all += weight(value_of(o));
+      }
+      want = (double)p * (double)sum(all);
+      sure = edge_in_list(true, n, 0);
+    }
+    if (sure) {
+      uint64_t mine = 0, some = 0;
+      for (int i = threadIdx.x; i < n; i += kSampleThreads) {
+        const uint64_t w = kept_weight(sh.list[i]);
+        mine += w;
+        some += w > 0;
+      }
+      const uint64_t z = sum(mine), at = aim(u, z);
+      const uint64_t kept = sum(some);
+      // the step of the index in which the running weight passes `at`, then the place in it
+      const int width = (a.vocab + kSteps - 1) / kSteps;
+      uint64_t before = 0;
+      const int s = list_level(n, before, [&](uint64_t o) { return kept_weight(o) ? (uint32_t)(index_of(o) / width) : kSteps; },
+                               kept_weight, [&](uint64_t b) { return b <= at; });
+      if (mini_list(n, [&](uint64_t o) { return index_of(o) / width == s && kept_weight(o) > 0; })) {
+        const int c = sh.minis;
+        if (threadIdx.x < c) sh.weights[threadIdx.x] = kept_weight(sh.mini[threadIdx.x]);
+        __syncthreads();
+        if (threadIdx.x < c) {
+          const uint64_t o = sh.mini[threadIdx.x];
+          for (int j = 0; j < c; ++j) before += index_of(sh.mini[j]) < index_of(o) ? sh.weights[j] : 0;
+          if (before <= at && at < before + sh.weights[threadIdx.x]) answer(a, rw, index_of(o), value_of(o), z, kept);
+        }
+        if (threadIdx.x == 0) {
+          sh.word = order_of(xe, ie);
+          sh.word2 = z;
+        }
+        return;
+      }
+    }
+    cta_sort(sh.list, n);
+    n = (int)min((uint64_t)n, k);
+    if (!(p >= 1.f)) {
+      uint64_t all = 0;
+      for (int i = threadIdx.x; i < n; i += kSampleThreads) all += weight(value_of(sh.list[i]));
+      want = (double)p * (double)sum(all);
+      n = taken_of_sorted(true, n, 0);
+    }
+    if (threadIdx.x == 0) sh.word = sh.list[n - 1];
+    finish_sorted(a, rw, u, n);
+  }
+  // The same for a sorted list of n kept tokens: sorted again, by rising index.
   __device__ __forceinline__ void finish_sorted(const SampleArgs& a, int rw, float u, int n) {
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kSampleThreads) {
