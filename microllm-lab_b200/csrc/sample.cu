@@ -67,6 +67,8 @@ struct SampleArgs {
   const void* x;
   int64_t row_stride;
   int vocab, part;  // part: tokens per CTA of a cluster
+  int rows;
+  bool long_first;  // more rows than run at once: those without a small top_k, which take longest, begin first
   const float* temperature;
   const int32_t* top_k;
   const float *top_p, *min_p, *u;
@@ -685,13 +687,23 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
   using S = Sampler<T>;
   constexpr int E = S::E;
   SampleShared& sh = *reinterpret_cast<SampleShared*>(smem);
-  const int rw = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  int rw = blockIdx.y;
   S s{sh, reinterpret_cast<T*>(smem + sizeof(SampleShared))};
   s.ranks = gridDim.x;
   s.rank = blockIdx.x;
   s.flip = s.hist = s.listed = 0;
   // no CTA's memory is written before it runs: the wait comes with the first exchange
   if (s.ranks > 1) cg::this_cluster().barrier_arrive();
+  if (a.long_first) {  // CTA c takes the c-th of the long rows, then of the others
+    const float t = tid < a.rows && a.temperature ? a.temperature[tid] : 1.f;
+    const int k = tid < a.rows && a.top_k ? a.top_k[tid] : 0;
+    const bool is_long = tid < a.rows && t > 0.f && (k <= 0 || k > kSampleMaxK);
+    const Scan q = cta_scan(sh.wsum, is_long);
+    if (tid < a.rows && (int)(is_long ? q.before : q.all + tid - q.before) == rw) sh.pick = tid;
+    __syncthreads();
+    rw = sh.pick;
+  }
   const int first = min(s.rank * a.part, a.vocab), n = min(a.part, a.vocab - first);  // this CTA's tokens
   const T* const row = static_cast<const T*>(a.x) + (int64_t)rw * a.row_stride + first;
   const int lead = (int)((uintptr_t)row & 15) / (int)sizeof(T);
@@ -890,6 +902,8 @@ int launch_sample(SampleArgs a, int rows, cudaStream_t st) {
     ranks *= 2;
   if (const char* v = getenv("SR")) ranks = std::max(ranks, atoi(v));
   a.part = ((a.vocab + ranks - 1) / ranks + 31) / 32 * 32;
+  a.rows = rows;
+  a.long_first = (int64_t)rows * ranks > sms && rows <= kSampleThreads && a.top_k;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ranks, rows);
   cfg.blockDim = dim3(kSampleThreads);
@@ -923,7 +937,7 @@ extern "C" int mllm_sample(int dtype, const void* d_logits, int64_t row_stride, 
   if (rows == 0) return MLLM_OK;
   if (!d_logits || !d_u || !d_id) return refuse(MLLM_ERR_ARG, "mllm_sample: null pointer");
   if ((uintptr_t)d_logits % esize(dtype)) return refuse(MLLM_ERR_ARG, "mllm_sample: misaligned logits");
-  const SampleArgs a = {d_logits, row_stride, vocab, 0, d_temperature, d_top_k, d_top_p, d_min_p, d_u, d_id, d_logprob,
+  const SampleArgs a = {d_logits, row_stride, vocab, 0, rows, false, d_temperature, d_top_k, d_top_p, d_min_p, d_u, d_id, d_logprob,
                         d_kept, d_probs};
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == MLLM_DTYPE_F16) return launch_sample<__half>(a, rows, st);
