@@ -581,3 +581,26 @@ def test_sample_in_a_graph_on_a_stream(cuda_ok):
         P.sample_device("f32", x.data_ptr(), 32000, 7, 32000, u.data_ptr(), i.data_ptr(), top_p_ptr=top_p.data_ptr())
         torch.cuda.synchronize()
         assert torch.equal(got, i)
+
+
+def test_sample_more_rows_than_run_at_once(cuda_ok):
+    """Rows are begun in another order then (those without a small top_k first); each keeps its own answer."""
+    rng = np.random.default_rng(8)
+    rows, v = 700, 2000
+    x = (2.5 * rng.standard_normal((rows, v))).astype(np.float32)
+    top_k = np.where(rng.random(rows) < 0.6, rng.integers(1, 1200, rows), 0)
+    temp = np.where(rng.random(rows) < 0.15, 0.0, rng.uniform(0.5, 1.5, rows))
+    _check_sample(x, temp, top_k, rng.uniform(0.3, 1.05, rows))
+    _check_sample(x, None, top_k)
+    _check_sample(x[:, :300], temp, np.minimum(top_k, 299), None, rng.uniform(0.0, 0.1, rows))
+
+
+@pytest.mark.parametrize("k", [193, 256, 300, 512, 513, 2047, 2049, 6000])
+def test_sample_list_sizes(k, cuda_ok):
+    """top_k around the sizes at which lists are counted, stepped through or given up, ties at the cut among them."""
+    rng = np.random.default_rng(k)
+    x = (2.5 * rng.standard_normal((6, 40000))).astype(np.float32)
+    x[3:] = np.round(x[3:], 1)  # many equal logits
+    x[5] = np.round(x[5] / 4)
+    _check_sample(x, None, np.full(6, k))
+    _check_sample(x, rng.uniform(0.6, 1.2, 6), np.full(6, k), rng.uniform(0.5, 0.99, 6), rng.uniform(0, 0.01, 6))
