@@ -1,7 +1,8 @@
 // Page copies of a paged cache (mllm_copy_pages): page dst[i] of every layer, k and v, becomes a copy of
 // page src[i].  Nothing is computed: bound by HBM (each byte read and written once), or by launch
 // latency for a few pages.  The page ids travel as kernel parameters, so a call needs no device copy of
-// them, takes no workspace and may be captured.
+// them, takes no workspace and may be captured.  A CTA copies up to 32 KB of a page, every thread's loads
+// issued before its stores: large pages spread over the SMs, and few of them fill the device.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -14,22 +15,32 @@ namespace {
 using namespace paged;
 
 constexpr int kCopyThreads = 256;
+constexpr int kCopyEach = 8;                               // 16-byte units of a thread
+constexpr int kCopyUnits = kCopyThreads * kCopyEach;       // of a CTA: 32 KB
 
 template <int N>
 struct CopyArgs {
   uint4 *k, *v;
   int64_t page_stride, layer_stride;  // 16-byte units
-  int page_units;
+  int page_units, chunks;  // of a page, and CTAs that share it
   int32_t src[N], dst[N];
 };
 
-// grid: (moves, layers, k or v)
+// grid: (moves x chunks, layers, k or v)
 template <int N>
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs<N> a) {
+  const int move = blockIdx.x / a.chunks, chunk = blockIdx.x - move * a.chunks;
   uint4* pool = (blockIdx.z ? a.v : a.k) + (int64_t)blockIdx.y * a.layer_stride;
-  const uint4* from = pool + (int64_t)a.src[blockIdx.x] * a.page_stride;
-  uint4* to = pool + (int64_t)a.dst[blockIdx.x] * a.page_stride;
-  for (int i = threadIdx.x; i < a.page_units; i += kCopyThreads) to[i] = from[i];
+  const uint4* from = pool + (int64_t)a.src[move] * a.page_stride;
+  uint4* to = pool + (int64_t)a.dst[move] * a.page_stride;
+  const int first = chunk * kCopyUnits + threadIdx.x;
+  uint4 u[kCopyEach];
+#pragma unroll
+  for (int i = 0; i < kCopyEach; ++i)
+    if (first + i * kCopyThreads < a.page_units) u[i] = __ldcs(from + first + i * kCopyThreads);
+#pragma unroll
+  for (int i = 0; i < kCopyEach; ++i)
+    if (first + i * kCopyThreads < a.page_units) to[first + i * kCopyThreads] = u[i];
 }
 
 template <int N>
@@ -42,9 +53,10 @@ void launch_copy(const mllm_paged_kv* kv, int layers, int64_t layer_stride, cons
   a.page_stride = kv->page_stride / per;
   a.layer_stride = layer_stride / per;
   a.page_units = kv->n_kv_heads * kv->page_len * (kv->head_dim / per);
+  a.chunks = (a.page_units + kCopyUnits - 1) / kCopyUnits;
   std::copy(src, src + n, a.src);
   std::copy(dst, dst + n, a.dst);
-  copy_pages_kernel<N><<<dim3(n, layers, 2), kCopyThreads, 0, st>>>(a);
+  copy_pages_kernel<N><<<dim3((unsigned)n * a.chunks, layers, 2), kCopyThreads, 0, st>>>(a);
 }
 
 }  // namespace

@@ -41,15 +41,16 @@ struct RopeArgs {
   int64_t q_stride;
 };
 
+// Eight elements as they lie in memory.
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  uint4 u[sizeof(T) == 4 ? 2 : 1];
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(u) / 16); ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-  const T* e = reinterpret_cast<const T*>(u);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
-}
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ float at(int i) const { return to_f32(reinterpret_cast<const T*>(u)[i]); }
+};
 template <class T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   T e[8];
@@ -75,9 +76,10 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_append_kernel(const Rope
   const A* const x = static_cast<const A*>(a.qkv) + t * a.row_stride + d;
   A* const q = static_cast<A*>(a.q) + t * a.q_stride + d;
   const bool mine = d < a.dim;
-  // the first head's elements travel while the page is looked up
-  float v[8];
-  if (mine && h0 < per_tok && seq >= 0) load8(x + (int64_t)h0 * a.dim, v);
+  // the first heads' elements travel while the page is looked up, and each round's two rounds ahead
+  Raw8<A> v0, v1;
+  if (mine && h0 < per_tok && seq >= 0) v0.load(x + (int64_t)h0 * a.dim);
+  if (mine && h0 + step < per_tok && seq >= 0) v1.load(x + (int64_t)(h0 + step) * a.dim);
   if (seq < 0) return;  // padding
   const int pg = pos / a.page_len;
   int page = -1;
@@ -103,8 +105,9 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_append_kernel(const Rope
     const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv;
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = in ? v[i] : 0.f;
-    if (mine && h + step < per_tok) load8(x + (int64_t)(h + step) * a.dim, v);
+    for (int i = 0; i < 8; ++i) y[i] = in ? v0.at(i) : 0.f;
+    v0 = v1;
+    if (mine && h + 2 * step < per_tok) v1.load(x + (int64_t)(h + 2 * step) * a.dim);
     if (a.q_gain) {
       float ss = 0.f;
 #pragma unroll
