@@ -31,7 +31,7 @@ constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kBlock = 32;       // positions per block: one per lane for the page lookups
 constexpr int kMinBlocks = 4;    // a CTA's run is at least one block per warp
 constexpr int kWholeBlocks = 16; // segments up to this long get a CTA of their own where there are enough CTAs
-constexpr int kMaxParts = 64;    // CTAs that one segment is spread over: one CTA reads all their parts
+constexpr int kFan = 16;         // a segment in more than twice as many parts is joined by so many of them first
 constexpr int kMaxCtas = 1024;   // partial slots in the workspace
 constexpr int kMaxGroup = 16;    // query heads of a group
 constexpr float kLog2e = 1.4426950408889634f;
@@ -50,6 +50,8 @@ struct AttnArgs {
   int64_t out_stride;
   float* lse;
   uint32_t* counter;  // [n_seq][n_kv][groups]
+  uint32_t* counter2; // [CTA][2]
+  float2* top;        // [CTA][2][kMaxGroup]: (m, l) of joined parts
   float* part;        // [CTA][2]: o [group][dim], (m, l) [group]
   int rep, group_size, groups;  // query heads per kv head, of a group, groups of a kv head
   int max_len;                  // positions that a row of the table can hold
@@ -165,7 +167,7 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a) {
     if (lane >= o) upto += up;
   }
   const uint32_t all = __shfl_sync(0xffffffffu, upto, 31) * per_seq;
-  r.q = max(max((all + gridDim.x - 1) / gridDim.x, (uint32_t)kMinBlocks), (longest + kMaxParts - 1) / kMaxParts);
+  r.q = max((all + gridDim.x - 1) / gridDim.x, (uint32_t)kMinBlocks);
   r.u0 = blockIdx.x * r.q;
   if ((uint64_t)blockIdx.x * r.q >= all) return r;
   const uint32_t end = min(r.u0 + r.q, all), each = (end - r.u0 + kAttnWarps - 1) / kAttnWarps, u = r.u0 + warp * each;
@@ -266,17 +268,24 @@ __device__ __forceinline__ void join2(float& m, float& l, float4& o, float m1, f
   m = top;
 }
 
-// Joins the parts that the warps left, each segment by the warp that has its first part here, and those of all
-// CTAs where this is the last one of a segment to come.
+// Joins the parts that the warps left, each segment by the warp that has its first part here.  A segment that
+// spans CTAs is joined by the last of them to come; of one that spans more than 2 kFan, every kFan neighbours
+// first, each time by the last to come, so that no CTA reads more than some dozens of parts (one sequence of
+// 100,000 positions and 9 heads over one kv head, bf16: 29 us; joined by one CTA from at most 64 parts, 54 us).
 template <class A, int DP>
 __device__ __forceinline__ void join(const AttnArgs& a, const Run& r, const Joint& w) {
-  struct Open {  // a segment whose last part this CTA left
+  struct Open {  // parts that this CTA joins: `parts` of them (0: none), `stride` CTAs apart from CTA `first` on
     Part p;
-    int first, parts;
+    int begin, first, parts, stride, groups;  // begin: the segment's first CTA; groups > 0: of so many such joins
   };
-  __shared__ Open open[2];  // one that began before this CTA, one that began in it
+  __shared__ Open open[2];  // of a segment that began before this CTA, of one that began in it
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quads = a.dim / 4;
   const size_t slot = (size_t)a.group_size * (a.dim + 4);  // o, then m and l; 16-byte aligned for any group
+  auto arrive = [](uint32_t* c, int n) {  // true for the last of n, which leaves the counter at 0
+    const bool last = atomicAdd(c, 1u) == (uint32_t)n - 1;
+    if (last) *c = 0;
+    return last;
+  };
   if (tid < 2) open[tid].parts = 0;
   __syncthreads();
 #pragma unroll 1
@@ -315,58 +324,59 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Run& r, const Join
     __syncwarp();
     if (lane == 0) {
       // which CTAs have a part, by the segment's first block: one that began in this run goes on to its end
-      const uint32_t start = side ? r.u0 + r.q - have : r.u0 - p.b0, first = start / r.q;
-      const int parts = (int)((start + p.nb - 1) / r.q - first) + 1;
-      uint32_t* const c = a.counter + p.segment(a);
-      if (atomicAdd(c, 1u) == (uint32_t)parts - 1) {
-        *c = 0;
-        open[side] = Open{p, (int)first, parts};
+      const uint32_t start = side ? r.u0 + r.q - have : r.u0 - p.b0, begin = start / r.q;
+      const int parts = (int)((start + p.nb - 1) / r.q - begin) + 1;
+      if (parts <= 2 * kFan) {
+        if (arrive(a.counter + p.segment(a), parts)) open[side] = Open{p, (int)begin, (int)begin, parts, 1, 0};
+      } else {
+        const int k = (blockIdx.x - begin) / kFan * kFan, n = min(kFan, parts - k);
+        if (arrive(a.counter2 + (begin + k) * 2 + (k == 0), n))
+          open[side] = Open{p, (int)begin, (int)begin + k, n, 1, (parts + kFan - 1) / kFan};
       }
     }
   }
   __syncthreads();
 #pragma unroll 1
   for (int side = 0; side < 2; ++side) {
-    const Open& s = open[side];
-    if (!s.parts) continue;
-    __threadfence();
-    // few parts: a thread takes all of an item's; many: every fourth by each warp, then the four in order, as
-    // (m, l) and o of [warp][item] at the rings' place
-    const bool many = s.parts > 8;
-    const int items = s.p.heads(a) * quads, step = many ? kAttnWarps : 1;
-    float2* const ml = reinterpret_cast<float2*>(w.ring);
-    float4* const os = reinterpret_cast<float4*>(ml + kAttnWarps * items);
 #pragma unroll 1
-    for (int x = many ? lane : tid; x < items; x += many ? 32 : kAttnThreads) {
-      const int h = x / quads, d = (x - h * quads) * 4;
-      float m = -INFINITY, l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    while (open[side].parts) {
+      const Open s = open[side];
+      __threadfence();
+      const int items = s.p.heads(a) * quads;
+      // (m, l) of a part: beside it, or of parts that were joined (their o is at the first one's place)
+      auto ml = [&](int c, int h) {
+        return s.stride == 1 ? reinterpret_cast<const float2*>(a.part + ((size_t)c * 2 + (c == s.begin)) * slot + a.group_size * a.dim) + h
+                             : a.top + (c * 2 + (c == s.begin)) * kMaxGroup + h;
+      };
+#pragma unroll 1
+      for (int x = tid; x < items; x += kAttnThreads) {
+        const int h = x / quads, d = (x - h * quads) * 4;
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-      for (int k = many ? warp : 0; k < s.parts; k += step) {
-        const float* q = a.part + ((size_t)(s.first + k) * 2 + (k == 0)) * slot;
-        const float2 mk = __ldcg(reinterpret_cast<const float2*>(q + a.group_size * a.dim) + h);
-        join2(m, l, o, mk.x, mk.y, __ldcg(reinterpret_cast<const float4*>(q + h * a.dim + d)));
+        for (int k = 0; k < s.parts; ++k) {
+          const int c = s.first + k * s.stride;
+          const float2 mk = __ldcg(ml(c, h));
+          join2(m, l, o, mk.x, mk.y,
+                __ldcg(reinterpret_cast<const float4*>(a.part + ((size_t)c * 2 + (c == s.begin)) * slot + h * a.dim + d)));
+        }
+        if (s.groups == 0) {
+          write_out<A>(a, s.p, h, d, o, l);
+          if (d == 0) write_lse(a, s.p, h, m, l);
+        } else {  // nobody else reads this element of o any more; (m, l) of the parts are still in use
+          const int c = s.first * 2 + (s.first == s.begin);
+          *reinterpret_cast<float4*>(a.part + c * slot + h * a.dim + d) = o;
+          if (d == 0) a.top[c * kMaxGroup + h] = make_float2(m, l);
+        }
       }
-      if (many) {
-        ml[warp * items + x] = make_float2(m, l);
-        os[warp * items + x] = o;
-      } else {
-        write_out<A>(a, s.p, h, d, o, l);
-        if (d == 0) write_lse(a, s.p, h, m, l);
+      if (s.groups) __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        open[side].parts = 0;
+        if (s.groups && arrive(a.counter + s.p.segment(a), s.groups)) open[side] = Open{s.p, s.begin, s.begin, s.groups, kFan, 0};
       }
+      __syncthreads();
     }
-    if (!many) continue;
-    __syncthreads();
-#pragma unroll 1
-    for (int x = tid; x < items; x += kAttnThreads) {
-      const int h = x / quads, d = (x - h * quads) * 4;
-      float m = -INFINITY, l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = 0; k < kAttnWarps; ++k) join2(m, l, o, ml[k * items + x].x, ml[k * items + x].y, os[k * items + x]);
-      write_out<A>(a, s.p, h, d, o, l);
-      if (d == 0) write_lse(a, s.p, h, m, l);
-    }
-    __syncthreads();
   }
 }
 
@@ -1046,6 +1056,8 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(
 // ---------------------------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------------------------
+// The workspace: counters of segments, then of groups of parts, (m, l) of joined parts, parts.
+constexpr size_t kCounter2Bytes = (size_t)kMaxCtas * 2 * 4, kTopBytes = (size_t)kMaxCtas * 2 * kMaxGroup * 8;
 size_t counter_bytes(int n_seq, int n_heads) { return (((size_t)n_seq * n_heads * 4 + 255) / 256) * 256; }
 
 // Opt in to more than 48 KB of shared memory, once per kernel and device.
@@ -1109,7 +1121,7 @@ int run_f32(AttnArgs& a, cudaStream_t st) {
 extern "C" size_t mllm_paged_attn_workspace(int n_seq, int n_heads, int head_dim) {
   using namespace mllm;
   if (n_seq < 1 || n_heads < 1 || head_dim < 8 || head_dim > 256) return 0;
-  return counter_bytes(n_seq, n_heads) + (size_t)kMaxCtas * 2 * std::min(n_heads, kMaxGroup) * (head_dim + 4) * 4;
+  return counter_bytes(n_seq, n_heads) + kCounter2Bytes + kTopBytes + (size_t)kMaxCtas * 2 * std::min(n_heads, kMaxGroup) * (head_dim + 4) * 4;
 }
 
 extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d_q, int64_t q_stride, int n_seq,
@@ -1144,7 +1156,10 @@ extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d
   a.page_shift = 31 + bits;
   a.page_mult = ((uint64_t)1 << a.page_shift) / kv->page_len + 1;
   a.counter = static_cast<uint32_t*>(d_ws);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + counter_bytes(n_seq, n_heads));
+  uint8_t* at = static_cast<uint8_t*>(d_ws) + counter_bytes(n_seq, n_heads);
+  a.counter2 = reinterpret_cast<uint32_t*>(at);
+  a.top = reinterpret_cast<float2*>(at + kCounter2Bytes);
+  a.part = reinterpret_cast<float*>(at + kCounter2Bytes + kTopBytes);
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == MLLM_DTYPE_F16) return run_mma<__half, __half>(a, st);
   if (dtype == MLLM_DTYPE_BF16) return run_mma<__nv_bfloat16, __nv_bfloat16>(a, st);
