@@ -270,10 +270,11 @@ int mllm_rope_append(const mllm_paged_kv* kv, int dtype, const void* d_qkv, int6
  * f32 over a cache of any type.  d_lse (nullable) is f32 [n_seq][n_heads].  A length of zero (or below)
  * gives out = 0 and lse = -inf.  Cache rows past a sequence's length, and table entries past its last
  * page, are never read.  A sequence whose length exceeds table_stride pages, or with a page id outside
- * the pool, gives NaN.  n_heads / n_kv_heads <= 64.  Scores, sums and the join are f32.
+ * the pool, gives NaN.  n_seq <= 65,535; n_heads / n_kv_heads <= 64; the table may hold up to about 2^31
+ * blocks of 32 positions over all sequences and kv heads.  Scores, sums and the joins are f32.
  * d_ws: mllm_paged_attn_workspace bytes, 16-byte aligned, zeroed once before its first use (each call
- * leaves its counters at zero again); one workspace serves one stream at a time.  The result does not
- * depend on timing: the length's parts are joined in a fixed order.
+ * leaves its counters at zero again); one workspace serves one call at a time.  The result does not
+ * depend on timing: a length's parts are joined in the order of their positions.
  */
 int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d_q, int64_t q_stride, int n_seq, int n_heads,
                     const int32_t* d_len, const int32_t* d_table, int table_stride, float scale, void* d_out,

