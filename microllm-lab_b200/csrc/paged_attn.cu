@@ -803,19 +803,18 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
 // ---------------------------------------------------------------------------------------------
 // Key rows of a stage that a lane shares (stages of 8 R positions), ring stages, CTAs per SM.
 template <int DP>
-constexpr int f32_rows() { return DP == 256 ? 1 : 2; }
+constexpr int f32_rows() { return DP == 64 ? 2 : 1; }
+constexpr int kF32Stages = 2;
+template <int DP, int G>
+constexpr int f32_ctas() { return DP == 256 ? 1 : G == 4 ? 3 : 2; }
 template <int DP>
-constexpr int f32_stages() { return DP == 64 ? 3 : 2; }
-template <int DP>
-constexpr int f32_ctas() { return DP == 64 ? 2 : 1; }
-template <int DP>
-constexpr int f32_ring_bytes() { return f32_stages<DP>() * 8 * f32_rows<DP>() * 2 * DP * 4; }  // of a warp
+constexpr int f32_ring_bytes() { return kF32Stages * 8 * f32_rows<DP>() * 2 * DP * 4; }  // of a warp
 template <int DP, int G>
 constexpr int f32_query_bytes() { return G * DP * 4 + 8 * f32_rows<DP>() * G * 4; }  // of a warp: queries and weights
 
 template <int DP, int G>
-__global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP>()) attn_f32_kernel(const AttnArgs a) {
-  constexpr int R = f32_rows<DP>(), P = 8 * R, S = f32_stages<DP>(), PARTS = kBlock / P;  // stages of a block
+__global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP, G>()) attn_f32_kernel(const AttnArgs a) {
+  constexpr int R = f32_rows<DP>(), P = 8 * R, S = kF32Stages, PARTS = kBlock / P;  // stages of a block
   constexpr int C = DP / 16, PER = DP / 4 < 32 ? DP / 4 : 32, ROWS = 32 / PER, V = DP / 4 / PER;
   constexpr int PIECES = R * C + P / ROWS * V;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -1108,7 +1107,7 @@ int run_mma(AttnArgs& a, cudaStream_t st) {
 }
 template <int DP, int G>
 int launch_f32(const AttnArgs& a, cudaStream_t st) {
-  return launch<attn_f32_kernel<DP, G>>(a, DP, f32_ctas<DP>(), kAttnWarps * (f32_ring_bytes<DP>() + f32_query_bytes<DP, G>()), st);
+  return launch<attn_f32_kernel<DP, G>>(a, DP, f32_ctas<DP, G>(), kAttnWarps * (f32_ring_bytes<DP>() + f32_query_bytes<DP, G>()), st);
 }
 int run_f32(AttnArgs& a, cudaStream_t st) {
   a.group_size = std::min(a.rep, 8);
