@@ -270,7 +270,8 @@ int mllm_rope_append(const mllm_paged_kv* kv, int dtype, const void* d_qkv, int6
  * f32 over a cache of any type.  d_lse (nullable) is f32 [n_seq][n_heads].  A length of zero (or below)
  * gives out = 0 and lse = -inf.  Cache rows past a sequence's length, and table entries past its last
  * page, are never read.  A sequence whose length exceeds table_stride pages, or with a page id outside
- * the pool, gives NaN.  n_seq <= 65,535; n_heads / n_kv_heads <= 64; the table may hold up to about 2^31
+ * the pool, gives NaN.  A key whose score is -inf is left out; an infinite value gives infinity or NaN.
+ * n_seq <= 65,535; n_heads / n_kv_heads <= 64; the table may hold up to about 2^31
  * blocks of 32 positions over all sequences and kv heads.  Scores, sums and the joins are f32.
  * d_ws: mllm_paged_attn_workspace bytes, 16-byte aligned, zeroed once before its first use (each call
  * leaves its counters at zero again); one workspace serves one call at a time.  The result does not

@@ -140,14 +140,23 @@ struct Run {
 // Every warp on its own: lanes sum the lengths of neighbouring sequences.
 __device__ __forceinline__ Run find_run(const AttnArgs& a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (a.n_seq + 31) / 32, s0 = min(lane * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
+  const int per = ((a.n_seq + 31) / 32 + 3) & ~3, s0 = min(lane * per, a.n_seq), s1 = min(s0 + per, a.n_seq);
   uint32_t mine = 0, longest = 0;
-#pragma unroll 8
-  for (int s = s0; s < s1; ++s) {
-    const uint32_t nb = blocks_of(a, s);
+  auto add = [&](int len) {
+    const uint32_t nb = blocks_of_len(a, len);
     mine += nb;
     longest = max(longest, nb);
+  };
+  int s4 = s0;
+  if (((uintptr_t)a.len & 15) == 0) {  // four lengths at a time
+#pragma unroll 2
+    for (; s4 + 4 <= s1; s4 += 4) {
+      const int4 v = __ldg(reinterpret_cast<const int4*>(a.len + s4));
+      add(v.x), add(v.y), add(v.z), add(v.w);
+    }
   }
+#pragma unroll 4
+  for (; s4 < s1; ++s4) add(__ldg(a.len + s4));
   longest = __reduce_max_sync(0xffffffffu, longest);
   const uint32_t per_seq = a.n_kv * a.groups;
   Run r;

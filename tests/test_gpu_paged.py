@@ -156,6 +156,19 @@ def test_attention_long_and_ragged(act, cache, lens, hk, dim, cuda_ok):
     _check_attention(Pool(lens, 64, hk, dim, cache, seed=9), act, hk * 3, dim ** -0.5)
 
 
+@pytest.mark.parametrize("seqs,offset", [(31, 0), (33, 1), (130, 3), (300, 2), (1100, 1)])
+def test_attention_many_sequences_and_lengths_anywhere(seqs, offset, cuda_ok):
+    """More sequences than lanes, and lengths that do not begin on a 16-byte boundary."""
+    import torch
+    rng = np.random.default_rng(seqs)
+    lens = np.where(rng.random(seqs) < 0.1, 0, rng.integers(1, 90, seqs))
+    lens[rng.integers(seqs)] = 700
+    pool = Pool(lens.tolist(), 16, 1, 64, "bf16", seed=seqs)
+    d_len = torch.zeros(seqs + 4, dtype=torch.int32, device="cuda")[offset: offset + seqs]
+    d_len.copy_(pool.d_len)
+    _check_attention(pool, "bf16", 2, 0.125, d_len=d_len)
+
+
 def test_attention_scores_far_apart(cuda_ok):
     """Scores to +-1e4: the running maximum jumps in every direction and most weights vanish."""
     for act, cache in KINDS:
