@@ -17,7 +17,7 @@
 // second join.
 //
 // B200: 3 sequences to 100,003 positions, 32 heads over 8 of 128, f16: 151 us (5.9 TB/s, 90 % of the measured
-// copy); 256 sequences of 0 to 384, 9 heads over 3 of 64, bf16: 22.5 us, of which the copies need 7.2 (the rest
+// copy); 256 sequences of 0 to 384, 9 heads over 3 of 64, bf16: 22.2 us, of which the copies need 7.2 (the rest
 // is the latency of finding the runs, the first rows and the joins); 1 of 191, f32: 12.3 us.
 #include <algorithm>
 #include <atomic>
