@@ -904,7 +904,6 @@ int launch_sample(SampleArgs a, int rows, cudaStream_t st) {
   int ranks = 1;
   while (ranks < kMaxCluster && ((int64_t)ranks * room < a.vocab || ((int64_t)rows * ranks * 2 <= sms && a.vocab / (2 * ranks) >= 4096)))
     ranks *= 2;
-  if (const char* v = getenv("SR")) ranks = std::max(ranks, atoi(v));
   a.part = ((a.vocab + ranks - 1) / ranks + 31) / 32 * 32;
   a.rows = rows;
   a.long_first = (int64_t)rows * ranks > sms && rows <= kSampleThreads && a.top_k;
