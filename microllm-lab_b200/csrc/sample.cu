@@ -17,9 +17,11 @@
 //   - otherwise by a histogram of tokens or weight over 512 such steps, then among the tokens of one step,
 //     or of a 512th of it where they are too many for a list;
 //   - and by halving, one pass per bit, where those are too many as well (thousands of tokens of one value).
-// A short list is not sorted either: several threads per token count, and weigh, what precedes it.  A longer
-// one goes through the same two levels of steps until few enough are left, for the id by steps of the index;
-// it is sorted where one step holds too many.
+// A short list is not sorted either: several threads per token count, and weigh, what precedes it.  One of up to
+// 512 tokens is sorted in registers, for the id a second time by index (33 rows with top_p: 35.9 us, by steps 38.9;
+// lists of up to 1,024 sorted as well cost 256 rows 62.7 us instead of 59.8).  A longer one goes through the same
+// two levels of steps until few enough are left, for the id by steps of the index; it is sorted where one step
+// holds too many.
 // The CTAs of a cluster meet at a barrier only to exchange a maximum, a histogram, a list (the first one's) or
 // a sum.
 //
@@ -27,8 +29,8 @@
 // once is called, not inlined, and the passes over the row either test 16 bytes at a time and do the rest
 // for the few that pass, or take a token at a time.
 //
-// B200: 256 rows of 49,152 f32 with mixed settings 58 us, one row 14 us, 33 rows of 50,257 bf16 with top_p and
-// probabilities 40 us.  Bound by latency where rows are few (a chain of some 20 barriers), by instruction
+// B200: 256 rows of 49,152 f32 with mixed settings 60 us, one row 14 us, 33 rows of 50,257 bf16 with top_p and
+// probabilities 36 us.  Bound by latency where rows are few (a chain of some 20 barriers), by instruction
 // issue and colliding shared-memory atomics where every token's weight goes into a histogram (about 24,000
 // cycles of one SM for 49,152 tokens).
 #include <cooperative_groups.h>
@@ -50,8 +52,10 @@ constexpr int kSampleThreads = 1024;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleList = 2048;   // tokens of a list
 constexpr int kShortList = 192;     // tokens of a list that is counted at once (the square of them)
+constexpr int kSortList = 512;     // tokens of a list that is sorted in registers, one per thread
 constexpr int kMiniList = 64;       // tokens of a step of a longer list
 constexpr int kSampleMaxK = 512;    // top_k that starts from the threads' maxima
+constexpr int kFewTokens = 4 * kSampleThreads;  // of a CTA: all are counted for top_k
 constexpr int kSteps = 512;         // steps of a histogram level
 constexpr int kMaxCluster = 16;
 constexpr float kOne = 1099511627776.f;  // 2^40
@@ -167,6 +171,33 @@ __device__ __noinline__ void cta_sort(uint64_t* list, int n) {
     if (h >= 32) __syncthreads();  // smaller ones stay within a warp's 32 places
   }
   __syncthreads();
+}
+
+// Sorts one number per thread to falling order (bitonic), the first n of them; the others are 0 and come last.
+// Returns the thread's.  Exchanges between warps go through list, of 2 kSortList places, its halves in turn, so
+// that one barrier each is enough; only the warps that n reaches do more than meet them.
+__device__ __noinline__ uint64_t sort_one(uint64_t* list, uint64_t v, int n) {
+  const int t = threadIdx.x;
+  int size = 32, half = 0;
+  while (size < n) size <<= 1;
+#pragma unroll 1
+  for (int h = 2; h <= size; h <<= 1) {
+    const bool falls = (t & h) == 0;
+    auto keep = [&](uint64_t u, int j) { v = (u > v) == (((t & j) == 0) == falls) ? u : v; };
+#pragma unroll 1
+    for (int j = h >> 1; j >= 32; j >>= 1) {
+      if (t < size) list[half + t] = v;
+      __syncthreads();
+      if (t < size) keep(list[half + (t ^ j)], j);
+      half ^= kSortList;
+    }
+    if (t < size) {
+#pragma unroll 1
+      for (int j = min(h >> 1, 16); j > 0; j >>= 1) keep(__shfl_xor_sync(0xffffffffu, v, j), j);
+    }
+  }
+  __syncthreads();  // list may be written again
+  return v;
 }
 
 // (x - m) / T; m is finite here, and 1 / T above 0.
@@ -467,6 +498,14 @@ struct Sampler {
         const Place q = place_of(sh, n, m, r);
         const bool keep = q.t >= 0 && taken(mass, above + (mass ? q.weight_before : q.count_before));
         o = ~most(keep ? ~q.order : 0);
+      } else if (n <= kSortList) {
+        o = sort_one(sh.list, threadIdx.x < n ? sh.list[threadIdx.x] : 0, n);
+        uint64_t b = threadIdx.x;
+        if (mass) b = cta_scan(sh.wsum, threadIdx.x < n ? weight(value_of(o)) : 0).before;
+        const int c = max(__syncthreads_count(threadIdx.x < n && taken(mass, above + b)), 1);
+        if (threadIdx.x == c - 1) sh.word = o;
+        __syncthreads();
+        o = sh.word;
       } else if (edge_in_list(mass, n, above)) {
         o = order_of(xe, ie);
       } else {
@@ -573,6 +612,8 @@ struct Sampler {
         if (threadIdx.x == 0) sh.word = o;
       }
       w = keep && q.w >= least ? q.w : 0;
+    } else if (n <= kSortList) {
+      return finish_sort(a, rw, u, n);
     } else {
       return finish_long(a, rw, u, n);
     }
@@ -590,7 +631,28 @@ struct Sampler {
     if (b <= at && at < b + w) answer(a, rw, index_of(order), value_of(order), z, kept);
     if (threadIdx.x == 0) sh.word2 = z;
   }
-  // The same for a list that is not short.
+  // The same for a list that is sorted: what is kept are its first tokens, which are sorted again by index.
+  __device__ __forceinline__ void finish_sort(const SampleArgs& a, int rw, float u, int n) {
+    uint64_t o = sort_one(sh.list, threadIdx.x < n ? sh.list[threadIdx.x] : 0, n);
+    bool keep = threadIdx.x < n && threadIdx.x < k;
+    uint64_t w = keep ? weight(value_of(o)) : 0;
+    if (!(p >= 1.f)) {
+      const Scan q = cta_scan(sh.wsum, w);
+      want = (double)p * (double)q.all;
+      keep = keep && taken(true, q.before);
+    }
+    const int last = __syncthreads_count(keep) - 1;
+    if (threadIdx.x == last) sh.word = o;
+    keep = keep && w >= least && w > 0;
+    const int kept = __syncthreads_count(keep);
+    o = sort_one(sh.list, keep ? o << 32 | o >> 32 : 0, last + 1);
+    w = threadIdx.x < kept ? weight(of_key((uint32_t)o)) : 0;
+    const Scan q = cta_scan(sh.wsum, w);
+    const uint64_t z = q.all, at = aim(u, z);
+    if (q.before <= at && at < q.before + w) answer(a, rw, index_of(o >> 32), of_key((uint32_t)o), z, kept);
+    if (threadIdx.x == 0) sh.word2 = z;
+  }
+  // The same for a longer list.
   __device__ __forceinline__ void finish_long(const SampleArgs& a, int rw, float u, int n) {
     bool sure = (uint64_t)n <= k || edge_in_list(false, n, 0);
     auto kept_weight = [&](uint64_t o) -> uint64_t {
@@ -799,12 +861,17 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleArgs
     if (s.rank == 0 && tid == 0) s.answer(a, rw, s.ie, s.m, z, 1);
     done = true;
   } else if (k < a.vocab && k <= kSampleMaxK) {
-    // the step in which the k-th largest of the threads' maxima lies, and all that is above it
-    const float g = s.gap(mine);
-    if (g > kFar) atomicAdd(&sh.lo[0][whole(g * -16.f)], 1u);
+    // the step in which the k-th largest of the threads' maxima lies, and all that is above it; where a thread has
+    // few tokens these count themselves, as few threads have a maximum there (730 tokens, k 109: 19,600 cycles
+    // instead of 37,200)
+    const bool few = s.pieces * E <= kFewTokens;
+    for (int i = tid; i < (few ? s.pieces * E : kSampleThreads); i += kSampleThreads) {
+      const float g = s.gap(few ? to_f32(s.x[i]) : mine);
+      if (g > kFar) atomicAdd(&sh.lo[0][whole(g * -16.f)], 1u);
+    }
     uint64_t above = 0;
     float to = fmaxf(-0.0625f * (float)(s.pick(false, false, above) + 1), kFar);
-    if (s.total < s.k) to = kFar;  // fewer threads than k hold a token of weight
+    if (s.total < s.k) to = kFar;  // fewer than k of them have any weight
     const int c = s.gather([&](float v, int) { return s.gap(v) > to; });
     done = c <= kSampleList;
     if (done) {

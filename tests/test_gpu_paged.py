@@ -476,6 +476,22 @@ def test_sample_against_64_bits(dtype, vocab, cuda_ok):
     _check_sample(x, None, min_p=min_p, dtype=dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [200, 513, 730, 1657, 4097, 20011])
+def test_sample_long_lists(dtype, vocab, cuda_ok):
+    """top_k around the lengths at which a list is treated in another way, in rows shorter and longer than it."""
+    rng = np.random.default_rng(vocab)
+    k = np.array([100, 191, 192, 193, 255, 256, 257, 300, 384, 500, 511, 512, 513, 600, 1023, 1024])
+    x = (2.0 * rng.standard_normal((len(k), vocab))).astype(np.float32)
+    x[3::4, ::3] = x[3::4, :1]  # many equal values, at places among the others
+    temp = rng.uniform(0.5, 2.0, len(k))
+    top_p = np.where(rng.random(len(k)) < 0.7, rng.uniform(0.5, 1, len(k)), 1.0)
+    min_p = np.where(rng.random(len(k)) < 0.4, rng.uniform(0.001, 0.05, len(k)), 0.0)
+    _check_sample(x, temp, k, dtype=dtype)
+    _check_sample(x, temp, k, top_p, min_p, dtype=dtype)
+    _check_sample(x, temp, None, top_p, min_p, dtype=dtype, probs=False)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("vocab,rows", [(100003, 5), (262144, 3), (524288, 2), (49152, 1)])
 def test_sample_large_vocabularies(dtype, vocab, rows, cuda_ok):
