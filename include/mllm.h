@@ -274,15 +274,16 @@ int mllm_rope_append(const mllm_paged_kv* kv, int dtype, const void* d_qkv, int6
  * n_seq <= 65,535; n_heads / n_kv_heads <= 64; the table may hold up to about 2^31
  * blocks of 32 positions over all sequences and kv heads.  Scores, sums and the joins are f32.
  * d_ws: mllm_paged_attn_workspace bytes, 16-byte aligned, zeroed once before its first use (each call
- * leaves its counters at zero again); one workspace serves one call at a time.  The result does not
- * depend on timing: a length's parts are joined in the order of their positions.
+ * leaves its counters at zero again); one workspace serves one call at a time, and calls of any numbers of
+ * sequences, heads and head_dim one after another, as long as it has room for the largest.  The result does
+ * not depend on timing: a length's parts are joined in the order of their positions.
  */
 int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d_q, int64_t q_stride, int n_seq, int n_heads,
                     const int32_t* d_len, const int32_t* d_table, int table_stride, float scale, void* d_out,
                     int64_t out_stride, float* d_lse, void* d_ws, size_t ws_bytes, void* stream);
 
-/* Workspace bytes of mllm_paged_attn for up to n_seq sequences and n_heads query heads of head_dim on
- * any device (0 when an argument is out of range). */
+/* Workspace bytes of mllm_paged_attn for up to n_heads query heads of up to head_dim, on any device and for
+ * any number of sequences (0 when an argument is out of range). */
 size_t mllm_paged_attn_workspace(int n_seq, int n_heads, int head_dim);
 
 /*

@@ -53,7 +53,7 @@ struct AttnArgs {
   void* out;
   int64_t out_stride;
   float* lse;
-  uint32_t* counter;  // [n_seq][n_kv][groups]
+  uint32_t* counter;  // [CTA]: of the segment that begins in it and ends in another
   uint32_t* counter2; // [CTA][2]
   float2* top;        // [CTA][2][kMaxGroup]: (m, l) of joined parts
   float* part;        // [CTA][2]: o [group][dim], (m, l) [group]
@@ -232,7 +232,6 @@ __device__ __forceinline__ int64_t row_offset(const AttnArgs& a, const Place& c,
 // A part of a segment: what one run holds of it.
 struct Part {
   int seq, kv, group, b0, blocks, nb;  // blocks 0: none
-  __device__ __forceinline__ uint32_t segment(const AttnArgs& a) const { return ((uint32_t)seq * a.n_kv + kv) * a.groups + group; }
   __device__ __forceinline__ int first_head(const AttnArgs& a) const { return kv * a.rep + group * a.group_size; }
   __device__ __forceinline__ int heads(const AttnArgs& a) const { return min(a.rep - group * a.group_size, a.group_size); }
 };
@@ -340,7 +339,7 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Run& r, const Join
       const uint32_t start = side ? r.u0 + r.q - have : r.u0 - p.b0, begin = start / r.q;
       const int parts = (int)((start + p.nb - 1) / r.q - begin) + 1;
       if (parts <= 2 * kFan) {
-        if (arrive(a.counter + p.segment(a), parts)) open[side] = Open{p, (int)begin, (int)begin, parts, 1, 0};
+        if (arrive(a.counter + begin, parts)) open[side] = Open{p, (int)begin, (int)begin, parts, 1, 0};
       } else {
         const int k = (blockIdx.x - begin) / kFan * kFan, n = min(kFan, parts - k);
         if (arrive(a.counter2 + (begin + k) * 2 + (k == 0), n))
@@ -386,7 +385,7 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Run& r, const Join
       __syncthreads();
       if (tid == 0) {
         open[side].parts = 0;
-        if (s.groups && arrive(a.counter + s.p.segment(a), s.groups)) open[side] = Open{s.p, s.begin, s.begin, s.groups, kFan, 0};
+        if (s.groups && arrive(a.counter + s.begin, s.groups)) open[side] = Open{s.p, s.begin, s.begin, s.groups, kFan, 0};
       }
       __syncthreads();
     }
@@ -1068,9 +1067,12 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP, G>()) attn_f32_kern
 // ---------------------------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------------------------
-// The workspace: counters of segments, then of groups of parts, (m, l) of joined parts, parts.
+// The workspace: counters of segments, then of groups of parts, (m, l) of joined parts, parts.  A segment's counter
+// is that of the CTA it begins in: a run ends once, so no more than one segment begins in it and goes on.  What
+// lies before the parts thus has the same place in every call, whatever its sequences, heads and head_dim, and no
+// call's data lies where another's counters are.
+constexpr size_t kCounterBytes = (size_t)kMaxCtas * 4;
 constexpr size_t kCounter2Bytes = (size_t)kMaxCtas * 2 * 4, kTopBytes = (size_t)kMaxCtas * 2 * kMaxGroup * 8;
-size_t counter_bytes(int n_seq, int n_heads) { return (((size_t)n_seq * n_heads * 4 + 255) / 256) * 256; }
 
 // Opt in to more than 48 KB of shared memory, once per kernel and device.
 template <auto KERNEL>
@@ -1133,7 +1135,7 @@ int run_f32(AttnArgs& a, cudaStream_t st) {
 extern "C" size_t mllm_paged_attn_workspace(int n_seq, int n_heads, int head_dim) {
   using namespace mllm;
   if (n_seq < 1 || n_heads < 1 || head_dim < 8 || head_dim > 256) return 0;
-  return counter_bytes(n_seq, n_heads) + kCounter2Bytes + kTopBytes + (size_t)kMaxCtas * 2 * std::min(n_heads, kMaxGroup) * (head_dim + 4) * 4;
+  return kCounterBytes + kCounter2Bytes + kTopBytes + (size_t)kMaxCtas * 2 * std::min(n_heads, kMaxGroup) * (head_dim + 4) * 4;
 }
 
 extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d_q, int64_t q_stride, int n_seq,
@@ -1168,7 +1170,7 @@ extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d
   a.page_shift = 31 + bits;
   a.page_mult = ((uint64_t)1 << a.page_shift) / kv->page_len + 1;
   a.counter = static_cast<uint32_t*>(d_ws);
-  uint8_t* at = static_cast<uint8_t*>(d_ws) + counter_bytes(n_seq, n_heads);
+  uint8_t* at = static_cast<uint8_t*>(d_ws) + kCounterBytes;
   a.counter2 = reinterpret_cast<uint32_t*>(at);
   a.top = reinterpret_cast<float2*>(at + kCounter2Bytes);
   a.part = reinterpret_cast<float*>(at + kCounter2Bytes + kTopBytes);
