@@ -416,7 +416,9 @@ __device__ __forceinline__ void finish_empty(const AttnArgs& a) {
 // The cached values are exact operands, and so are queries of their type.  f32 queries and weights are
 // split into as many 16-bit terms as f32 needs (3 in bf16, 2 in f16, where queries are first scaled by a
 // power of two to at most 1).  With queries of 16 bits the weights get two terms: one alone would add an
-// error of the size of the output's own rounding (bf16 2.1e-3 of the result against 1.7e-3).
+// error of the size of the output's own rounding (bf16 2.1e-3 of the result against 1.7e-3).  f16 ends at 2^-24, so
+// its weights are scaled to at most 2^15 before they are split, and the output's sums back at the end: a weight is
+// good to 2^-40 of the largest of its run, not to 2^-25 (which loses all of 32 positions 18 nats below one other).
 // ---------------------------------------------------------------------------------------------
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -461,6 +463,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+template <class T>
+constexpr float weight_scale() { return __is_same(T, __half) ? 32768.f : 1.f; }
 template <class T, class A>
 constexpr int terms_of() { return sizeof(A) == 2 ? 1 : (__is_same(T, __half) ? 2 : 3); }
 
@@ -716,7 +720,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             uint32_t w[WT];
-            split2<T, WT>(s[nt][2 * x], s[nt][2 * x + 1], w);
+            split2<T, WT>(s[nt][2 * x] * weight_scale<T>(), s[nt][2 * x + 1] * weight_scale<T>(), w);
 #pragma unroll
             for (int t = 0; t < WT; ++t) p[nt][t][x] = transpose8x8(w[t]);
           }
@@ -774,8 +778,9 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
             for (int v = 0; v < V; ++v) {
               const int d = v * 64 + row * 8;
               if (d >= a.dim) continue;
-              const float4 lo = make_float4(o[v][0][nt][e], o[v][0][nt][2 + e], o[v][1][nt][e], o[v][1][nt][2 + e]);
-              const float4 hi = make_float4(o[v][2][nt][e], o[v][2][nt][2 + e], o[v][3][nt][e], o[v][3][nt][2 + e]);
+              constexpr float back = 1.f / weight_scale<T>();
+              const float4 lo = rows4(make_float4(o[v][0][nt][e], o[v][0][nt][2 + e], o[v][1][nt][e], o[v][1][nt][2 + e]), back);
+              const float4 hi = rows4(make_float4(o[v][2][nt][e], o[v][2][nt][2 + e], o[v][3][nt][e], o[v][3][nt][2 + e]), back);
               if (done) {
                 write_out<A>(a, mine, h, d, lo, sum);
                 write_out<A>(a, mine, h, d + 4, hi, sum);
