@@ -414,11 +414,12 @@ __device__ __forceinline__ void finish_empty(const AttnArgs& a) {
 // and transposed by movmatrix, are the second product's operand.
 //
 // The cached values are exact operands, and so are queries of their type.  f32 queries and weights are
-// split into as many 16-bit terms as f32 needs (3 in bf16, 2 in f16, where queries are first scaled by a
-// power of two to at most 1).  With queries of 16 bits the weights get two terms: one alone would add an
-// error of the size of the output's own rounding (bf16 2.1e-3 of the result against 1.7e-3).  f16 ends at 2^-24, so
-// its weights are scaled to at most 2^15 before they are split, and the output's sums back at the end: a weight is
-// good to 2^-40 of the largest of its run, not to 2^-25 (which loses all of 32 positions 18 nats below one other).
+// split into 3 terms in bf16 (24 bits) or 2 in f16 (23 bits; queries are first scaled by a power of two to below
+// 2^15, so that an element is good to 2^-39 of the row's largest, or better).  With queries of 16 bits the
+// weights get two terms: one alone would add an error of the size of the output's own rounding (bf16 2.1e-3 of
+// the result against 1.7e-3).  f16 ends at 2^-24, so its weights are scaled to at most 2^15 before they are
+// split, and the output's sums back at the end: a weight is good to 2^-40 of the largest of its run, not to
+// 2^-25 (which loses all of 32 positions 18 nats below one other).
 // ---------------------------------------------------------------------------------------------
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -603,12 +604,12 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
               for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[x][e]));
             }
             float up = 1.f, down = 1.f;
-            if constexpr (TERMS == 2) {  // f16 terms: scaled to at most 1
+            if constexpr (TERMS == 2) {  // f16 terms: scaled to below 2^15
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-              int e = 0;
+              int e = 15;
               if (top > 0.f && top < INFINITY) (void)frexpf(top, &e);
-              e = max(min(e, 126), -126);
+              e = max(e - 15, -126);  // at most 113
               up = ldexpf(1.f, e);
               down = ldexpf(1.f, -e);
             }

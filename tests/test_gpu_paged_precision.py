@@ -7,7 +7,8 @@ u = 2^-24 (half an f32 ulp), D the head size and n the length:
 - weights of 16-bit queries have two terms of the cache's type: 2^-16 of a weight in bf16, 2^-22 in f16; f32 queries
   over f16 have two as well, and 2^-22 as well;
 - f16 ends at 2^-24, which is 2^-39 of the largest weight or query element where those are scaled to 2^15: half
-  of that, 2^-40, for each position, or each element;
+  of that, 2^-40, for each position, or each element (a row of queries is scaled to between 2^14 and 2^15, which
+  may double its share: ds holds that many times over);
 - the output is rounded once: half an ulp of it, for f16 at least half of 2^-24.
 """
 import math
@@ -79,3 +80,19 @@ def test_attention_keeps_the_bits_of_its_weights(act, cache, dim, hk, rep, cuda_
     pool = Pool([7, 10, 24, 60], 16, hk, dim, cache, seed=dim + rep)
     q = np.random.default_rng(rep).standard_normal((4, hk * rep, dim)).astype(np.float32)
     _compare(pool, act, hk * rep, dim ** -0.5, q)
+
+
+@pytest.mark.parametrize("act,cache", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_queries_with_one_large_element(act, cache, dim, cuda_ok):
+    """The large element meets keys of 0, so the scores hang on elements 2^-17 of it and less."""
+    rng = np.random.default_rng(dim)
+    lens = [20, 300]
+    pool = Pool(lens, 16, 2, dim, cache, seed=dim)
+    q = 2.0 ** -17 * rng.uniform(0.25, 1.0, (2, 6, dim)) * rng.choice([-1, 1], (2, 6, dim))
+    q[:, :, 5] = 1.0
+    for s, n in enumerate(lens):
+        k = 4096 * rng.standard_normal((2, n, dim))
+        k[:, :, 5] = 0.0
+        _put(pool, 0, s, k)
+    _compare(pool, act, 6, 4.0, q.astype(np.float32))
