@@ -1080,11 +1080,12 @@ __global__ void __launch_bounds__(kAttnThreads, f32_ctas<DP, G>()) attn_f32_kern
 constexpr size_t kCounterBytes = (size_t)kMaxCtas * 4;
 constexpr size_t kCounter2Bytes = (size_t)kMaxCtas * 2 * 4, kTopBytes = (size_t)kMaxCtas * 2 * kMaxGroup * 8;
 
-// Opt in to more than 48 KB of shared memory, once per kernel and device.
+// Opt in to more than 48 KB of shared memory, once per kernel and device, whatever the call needs: what the
+// kernel has statically counts too, so that 48 KB is not the limit of the dynamic part.
 template <auto KERNEL>
-bool allow_smem(int dev, size_t smem) {
+bool allow_smem(int dev) {
   static std::atomic<uint64_t> done{0};
-  if (smem <= 48 * 1024 || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return true;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return true;
   if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess) return false;
   if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   return true;
@@ -1097,7 +1098,7 @@ int launch(const AttnArgs& a, int dp, int per_sm, size_t smem, cudaStream_t st) 
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: no current CUDA device");
   smem += (size_t)kAttnWarps * a.group_size * (dp + 4) * 4;
-  if (!allow_smem<KERNEL>(dev, smem)) return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: not enough shared memory");
+  if (!allow_smem<KERNEL>(dev)) return refuse(MLLM_ERR_CUDA, "mllm_paged_attn: not enough shared memory");
   per_sm = std::min(per_sm, (int)(228 * 1024 / (smem + 1024 + 512)));
   // no more CTAs than runs of the shortest length over the whole table
   const int64_t blocks = ((int64_t)a.table_stride * a.page_len + kBlock - 1) / kBlock;
