@@ -289,7 +289,8 @@ size_t mllm_paged_attn_workspace(int n_seq, int n_heads, int head_dim);
 /*
  * Copy pages src[i] -> dst[i] (host arrays, i < n) of n_layers pools that lie layer_stride elements apart
  * (k and v alike), for forks that are about to be written and for compaction.  Pages must be contiguous
- * (kv-head-major or position-major without gaps).  Every page id must be in the pool, no page may be
+ * (kv-head-major or position-major without gaps), and layers apart from one another: one pool after the other, or
+ * side by side within page_stride (MLLM_ERR_ARG where they overlap).  Every page id must be in the pool, no page may be
  * written twice, and no page may be both read and written (MLLM_ERR_ARG): the copies run in no order.
  * The ids are read before the call returns.
  */

@@ -80,6 +80,10 @@ extern "C" int mllm_copy_pages(const mllm_paged_kv* kv, int n_layers, int64_t la
   const int per = 16 / esize(kv->dtype);
   if (n_layers > 1 && (layer_stride < page || layer_stride % per))
     return refuse(MLLM_ERR_ARG, "mllm_copy_pages: layer_stride below a page, or not 16-byte aligned");
+  // layers one after another, or side by side within a page's stride
+  if (n_layers > 1 && layer_stride < (__int128)(kv->n_pages - 1) * kv->page_stride + page &&
+      kv->page_stride < (__int128)(n_layers - 1) * layer_stride + page)
+    return refuse(MLLM_ERR_ARG, "mllm_copy_pages: layers overlap");
   if (n == 0) return MLLM_OK;
   if (!src || !dst) return refuse(MLLM_ERR_ARG, "mllm_copy_pages: null page list");
   try {
