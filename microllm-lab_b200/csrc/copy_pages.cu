@@ -62,6 +62,21 @@ void launch_copy(const mllm_paged_kv* kv, int layers, int64_t layer_stride, cons
   copy_pages_kernel<N><<<dim3((unsigned)n * a.chunks, layers, 2), kCopyThreads, 0, st>>>(a);
 }
 
+// Whether no destination is a source or another destination, for up to kSorted copies: by sorting them, so that a
+// few copies cost the same in a pool of any size.  More are marked in one byte per page of the pool.
+constexpr int kSorted = 64;
+bool destinations_apart(const int32_t* src, const int32_t* dst, int n) {
+  int64_t use[2 * kSorted];  // page id, and 1 for a destination
+  for (int i = 0; i < n; ++i) {
+    use[i] = 2 * (int64_t)src[i];
+    use[n + i] = 2 * (int64_t)dst[i] + 1;
+  }
+  std::sort(use, use + 2 * n);
+  for (int i = 1; i < 2 * n; ++i)
+    if ((use[i] & 1) && use[i] / 2 == use[i - 1] / 2) return false;
+  return true;
+}
+
 }  // namespace
 }  // namespace mllm
 
@@ -86,20 +101,25 @@ extern "C" int mllm_copy_pages(const mllm_paged_kv* kv, int n_layers, int64_t la
     return refuse(MLLM_ERR_ARG, "mllm_copy_pages: layers overlap");
   if (n == 0) return MLLM_OK;
   if (!src || !dst) return refuse(MLLM_ERR_ARG, "mllm_copy_pages: null page list");
-  try {
-    std::vector<uint8_t> used(kv->n_pages, 0);  // 1: read, 2: written
-    for (int i = 0; i < n; ++i) {
-      if (src[i] < 0 || src[i] >= kv->n_pages || dst[i] < 0 || dst[i] >= kv->n_pages)
-        return refuse(MLLM_ERR_ARG, "mllm_copy_pages: page id outside the pool");
-      used[src[i]] |= 1;
+  for (int i = 0; i < n; ++i)
+    if (src[i] < 0 || src[i] >= kv->n_pages || dst[i] < 0 || dst[i] >= kv->n_pages)
+      return refuse(MLLM_ERR_ARG, "mllm_copy_pages: page id outside the pool");
+  bool apart = true;
+  if (n <= kSorted) {
+    apart = destinations_apart(src, dst, n);
+  } else {
+    try {
+      std::vector<uint8_t> used(kv->n_pages, 0);
+      for (int i = 0; i < n; ++i) used[src[i]] = 1;
+      for (int i = 0; i < n; ++i) {
+        apart &= !used[dst[i]];
+        used[dst[i]] = 1;
+      }
+    } catch (const std::bad_alloc&) {
+      return refuse(MLLM_ERR_OOM, "mllm_copy_pages: no host memory for one byte per page of the pool");
     }
-    for (int i = 0; i < n; ++i) {
-      if (used[dst[i]]) return refuse(MLLM_ERR_ARG, "mllm_copy_pages: a page is written twice, or read and written");
-      used[dst[i]] = 2;
-    }
-  } catch (const std::bad_alloc&) {
-    return MLLM_ERR_OOM;
   }
+  if (!apart) return refuse(MLLM_ERR_ARG, "mllm_copy_pages: a page is written twice, or read and written");
   constexpr int kFew = 32, kMany = 2048;  // 16 KB of parameters
   for (int i = 0; i < n; i += kMany) {
     const int m = std::min(kMany, n - i);

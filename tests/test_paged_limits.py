@@ -1,7 +1,10 @@
 """Host side of the paged serving operators: workspaces, page lists and sizes at their limits (no GPU needed)."""
+import subprocess
+import sys
+
 import pytest
 
-from conftest import pkg
+from conftest import ROOT, pkg
 
 
 @pytest.mark.parametrize("heads,dim", [(1, 8), (4, 64), (32, 128), (64, 256)])
@@ -34,3 +37,44 @@ def test_copy_pages_refuses_layers_that_overlap(layers, page_stride, stride):
     """Copies run in no order, so no page of a layer may be part of another layer's."""
     kv = pkg().paged_kv(A, A, "f32", 8, 16, 2, 64, (page_stride, 16 * 64, 64))
     _refused(-3, kv, [0], [1], layers, stride)
+
+
+LIMITED = """
+import ctypes, importlib, resource, sys
+sys.path.insert(0, %r)
+P = importlib.import_module("microllm-lab_b200")
+L = P.load_library()
+kv = P.paged_kv(1 << 20, 1 << 20, "f32", 2**31 - 1, 1, 1, 8)
+now = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (now + (256 << 20), now + (256 << 20)))
+for n in (1, 30, 64):  # every destination but the last is another page; the last is written twice, or read as well
+    src, dst = (ctypes.c_int * n)(*range(n)), (ctypes.c_int * n)(*range(1000, 1000 + n))
+    for bad in (0, 1000)[: n]:
+        dst[n - 1] = bad
+        rc = L.mllm_copy_pages(ctypes.byref(kv), 1, 0, ctypes.addressof(src), ctypes.addressof(dst), n, None)
+        assert rc == -3 and b"written twice" in L.mllm_last_error(None), (n, bad, rc, L.mllm_last_error(None))
+"""
+
+
+def test_copy_pages_of_a_few_pages_does_not_depend_on_the_pool():
+    """A pool of 2^31 - 1 pages: the check of one page's copy takes no memory for all of them."""
+    r = subprocess.run([sys.executable, "-c", LIMITED % ROOT], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("n", [2, 64, 65, 300])
+def test_copy_pages_finds_a_conflict_wherever_it_is(n):
+    """A destination that is also the first, the last or a middle source or destination, in short and long lists."""
+    kv = pkg().paged_kv(A, A, "f32", 4096, 16, 2, 64)
+    src, dst = [(7 * i) % 2048 for i in range(n)], [2048 + (5 * i) % 2048 for i in range(n)]
+    for at in (0, n // 2, n - 1):
+        for other in (0, n // 2, n - 1):
+            bad = list(dst)
+            bad[at] = src[other]
+            _refused(-3, kv, src, bad)
+            if at != other:
+                bad[at] = dst[other]
+                _refused(-3, kv, src, bad)
+    for outside in (-1, 4096):
+        _refused(-3, kv, src[:-1] + [outside], dst)
+        _refused(-3, kv, src, [outside] + dst[1:])
