@@ -86,12 +86,14 @@ extern "C" int mllm_copy_pages(const mllm_paged_kv* kv, int n_layers, int64_t la
   using namespace mllm::paged;
   if (int rc = check_kv(kv)) return rc;
   if (n < 0 || n_layers < 1 || n_layers > 65535) return refuse(MLLM_ERR_ARG, "mllm_copy_pages: bad page or layer count");
+  constexpr int64_t kMostOfPage = (int64_t)1 << 30;
+  if ((int64_t)kv->n_kv_heads * kv->page_len > kMostOfPage / kv->head_dim)
+    return refuse(MLLM_ERR_UNSUPPORTED, "mllm_copy_pages: pages above 2^30 elements");
   const int64_t page = (int64_t)kv->n_kv_heads * kv->page_len * kv->head_dim;
   const bool by_head = kv->pos_stride == kv->head_dim && kv->head_stride == (int64_t)kv->page_len * kv->head_dim;
   const bool by_pos = kv->head_stride == kv->head_dim && kv->pos_stride == (int64_t)kv->n_kv_heads * kv->head_dim;
   if (!(by_head || by_pos) || kv->page_stride < page)
     return refuse(MLLM_ERR_UNSUPPORTED, "mllm_copy_pages: pages must be contiguous");
-  if (page > (int64_t)1 << 30) return refuse(MLLM_ERR_UNSUPPORTED, "mllm_copy_pages: pages above 2^30 elements");
   const int per = 16 / esize(kv->dtype);
   if (n_layers > 1 && (layer_stride < page || layer_stride % per))
     return refuse(MLLM_ERR_ARG, "mllm_copy_pages: layer_stride below a page, or not 16-byte aligned");

@@ -78,3 +78,10 @@ def test_copy_pages_finds_a_conflict_wherever_it_is(n):
     for outside in (-1, 4096):
         _refused(-3, kv, src[:-1] + [outside], dst)
         _refused(-3, kv, src, [outside] + dst[1:])
+
+
+@pytest.mark.parametrize("heads,page_len,dim", [(2**31 - 1, 2**31 - 1, 8), (2**31 - 1, 2**31 - 1, 256), (1 << 30, 1 << 30, 16),
+                                                (1, 2**31 - 1, 8), (1 << 20, 1 << 8, 8)])
+def test_copy_pages_refuses_pages_whose_size_passes_64_bits(heads, page_len, dim):
+    kv = pkg().paged_kv(A, A, "f32", 8, page_len, heads, dim, (1 << 62, page_len * dim, dim))
+    _refused(-2, kv, [0], [1])
