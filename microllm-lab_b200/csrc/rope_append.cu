@@ -232,7 +232,10 @@ extern "C" int mllm_rope_append(const mllm_paged_kv* kv, int dtype, const void* 
     return refuse(MLLM_ERR_ARG, "mllm_rope_append: a row stride is shorter than a row");
   if (((uintptr_t)d_qkv & 15) || ((uintptr_t)d_q & 15) || row_stride * es % 16 || q_stride * es % 16)
     return refuse(MLLM_ERR_ARG, "mllm_rope_append: rows must be 16-byte aligned");
-  if ((int64_t)n_tok * (width / kv->head_dim) > (int64_t)1 << 31)
+  const int64_t row_heads = width / kv->head_dim;
+  if (row_heads > (int64_t)1 << 30)  // a warp counts them in 31 bits, two rounds ahead
+    return refuse(MLLM_ERR_ARG, "mllm_rope_append: more than 2^30 heads in a row");
+  if (n_tok * row_heads > (int64_t)1 << 31)
     return refuse(MLLM_ERR_ARG, "mllm_rope_append: more than 2^31 heads in one call");
   if (n_tok == 0) return MLLM_OK;
   const RopeArgs a = {kv->k, kv->v, kv->page_stride, kv->head_stride, kv->pos_stride, kv->n_pages, kv->page_len,

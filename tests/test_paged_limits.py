@@ -85,3 +85,13 @@ def test_copy_pages_finds_a_conflict_wherever_it_is(n):
 def test_copy_pages_refuses_pages_whose_size_passes_64_bits(heads, page_len, dim):
     kv = pkg().paged_kv(A, A, "f32", 8, page_len, heads, dim, (1 << 62, page_len * dim, dim))
     _refused(-2, kv, [0], [1])
+
+
+@pytest.mark.parametrize("heads", [2**31 - 2, 2**30, 2**30 - 1])
+def test_rope_append_refuses_rows_of_too_many_heads(heads):
+    """A row's heads are counted, two rounds ahead, in 31 bits."""
+    P = pkg()
+    kv = P.paged_kv(A, A, "f32", 8, 16, 1, 8)
+    with pytest.raises(P.MllmError) as e:
+        P.rope_append_device(kv, "f32", A, 1 << 40, 1, heads, 0, A, A, 1, 8, A, A, 100, 8, A, 1 << 40)
+    assert e.value.code == -3 and "2^30 heads" in str(e.value)
