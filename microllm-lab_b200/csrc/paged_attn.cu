@@ -1162,6 +1162,8 @@ extern "C" int mllm_paged_attn(const mllm_paged_kv* kv, int dtype, const void* d
   const int64_t row = (int64_t)n_heads * kv->head_dim;
   const int es = esize(dtype);
   if (q_stride < row || out_stride < row) return refuse(MLLM_ERR_ARG, "mllm_paged_attn: a row stride is shorter than a row");
+  if (row > (int64_t)1 << 30)  // empty sequences count a row's elements in 31 bits
+    return refuse(MLLM_ERR_UNSUPPORTED, "mllm_paged_attn: more than 2^30 elements in a row");
   if (((uintptr_t)d_q & 15) || ((uintptr_t)d_out & 15) || q_stride * es % 16 || out_stride * es % 16)
     return refuse(MLLM_ERR_ARG, "mllm_paged_attn: rows must be 16-byte aligned");
   if (n_seq == 0) return MLLM_OK;

@@ -95,3 +95,13 @@ def test_rope_append_refuses_rows_of_too_many_heads(heads):
     with pytest.raises(P.MllmError) as e:
         P.rope_append_device(kv, "f32", A, 1 << 40, 1, heads, 0, A, A, 1, 8, A, A, 100, 8, A, 1 << 40)
     assert e.value.code == -3 and "2^30 heads" in str(e.value)
+
+
+def test_paged_attn_refuses_rows_of_too_many_elements():
+    """A row's elements are counted in 31 bits where a sequence is empty."""
+    P = pkg()
+    kv = P.paged_kv(A, A, "f32", 8, 16, 1 << 25, 8)
+    for heads in (1 << 28, 1 << 30):
+        with pytest.raises(P.MllmError) as e:
+            P.paged_attn_device(kv, "f32", A, 1 << 40, 4, heads, A, A, 8, 0.125, A, 1 << 40, A, 1 << 40)
+        assert e.value.code == -2 and "2^30 elements" in str(e.value)
