@@ -64,9 +64,21 @@ def paged_attn_device(kv: PagedKV, dtype: str, q_ptr: int, q_stride: int, n_seq:
                                           ws_ptr, ws_bytes, stream or None))
 
 
+def _page_ids(ids) -> np.ndarray:
+    """Page ids as contiguous int32, refused where that would change one."""
+    ids = np.asarray(ids)
+    if ids.dtype != np.int32 and ids.size:
+        if ids.dtype.kind not in "iu":
+            raise TypeError(f"page ids are whole numbers, not {ids.dtype}")
+        low, high = int(ids.min()), int(ids.max())
+        if low < -1 << 31 or high >= 1 << 31:
+            raise ValueError(f"page ids from {low} to {high} do not fit 32 bits")
+    return np.ascontiguousarray(ids, np.int32)
+
+
 def copy_pages_device(kv: PagedKV, src, dst, n_layers: int = 1, layer_stride: int = 0, stream: int = 0) -> None:
     """Copy pages src[i] -> dst[i] (host ids) in every layer's pool (mllm_copy_pages)."""
-    src, dst = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
+    src, dst = _page_ids(src), _page_ids(dst)
     if src.shape != dst.shape or src.ndim != 1:
         raise ValueError("src and dst are page lists of one length")
     _check(load_library().mllm_copy_pages(ctypes.byref(kv), n_layers, layer_stride, src.ctypes.data, dst.ctypes.data,

@@ -2,6 +2,7 @@
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 
 from conftest import ROOT, pkg
@@ -105,3 +106,20 @@ def test_paged_attn_refuses_rows_of_too_many_elements():
         with pytest.raises(P.MllmError) as e:
             P.paged_attn_device(kv, "f32", A, 1 << 40, 4, heads, A, A, 8, 0.125, A, 1 << 40, A, 1 << 40)
         assert e.value.code == -2 and "2^30 elements" in str(e.value)
+
+
+@pytest.mark.parametrize("ids", [np.array([1 << 32]), np.array([-(1 << 32)]), np.array([(1 << 32) + 1]), [2.5], np.array([1.0]), ["1"], [None],
+                                 np.array([1 << 63], np.uint64), np.array([True])])
+def test_copy_pages_takes_page_ids_as_they_are(ids):
+    """Ids that are no 32-bit numbers are refused, not rounded or cut to some other page's."""
+    for src, dst in ((ids, [3]), ([3], ids)):
+        with pytest.raises((ValueError, TypeError, OverflowError)):
+            pkg().copy_pages_device(pkg().paged_kv(A, A, "f32", 8, 16, 2, 64), src, dst)
+
+
+def test_copy_pages_takes_ids_of_any_whole_type():
+    """A conflict that the library finds shows that the ids came through."""
+    kv = pkg().paged_kv(A, A, "f32", 8, 16, 2, 64)
+    for ids in ([5], (5,), np.array([5]), np.array([5], np.uint8), np.array([5], np.uint64), np.array([0, 5, 0, 6])[1::2]):
+        _refused(-3, kv, ids, ids)
+    pkg().copy_pages_device(kv, [], [])
