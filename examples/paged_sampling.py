@@ -65,13 +65,13 @@ class PagedDecoder:
             P.copy_pages_device(self.kv[0], *moves, n_layers=len(self.kv), layer_stride=self.k.stride(0))
 
     def step(self, seqs, ids: torch.Tensor) -> torch.Tensor:
-        """Append one token to each of ``seqs`` (each once) and return the logits after it [len(seqs)][vocab]."""
+        """Append one token to each of ``seqs`` (each once) and return the logits after it [len(seqs)][vocab].  Raises
+        MemoryError, changing nothing, when the pool has too few free pages."""
         n = len(seqs)
         if n > self.max_seqs:
             raise ValueError(f"{n} sequences in a decoder made for {self.max_seqs}")
         pos = torch.tensor([self.pages.length(s) for s in seqs], dtype=torch.int32, device="cuda")
-        for s in seqs:
-            self.copy(self.pages.grow(s))
+        self.copy(self.pages.grow_all(seqs))
         table = torch.from_numpy(self.pages.table(seqs)).cuda()
         length = pos + 1
         x = self.embed[ids.long()]

@@ -165,6 +165,33 @@ class PageTable:
         self._len[seq] = have + n
         return moved
 
+    def grow_all(self, seqs, n: int = 1):
+        """``grow`` for each of ``seqs`` (each once), or for none: MemoryError when the pool has too few free
+        pages for all of them.  Returns the copies of all as one (src, dst)."""
+        if n < 0:
+            raise ValueError("n counts positions")
+        seqs = list(seqs)
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is there twice")
+        want, refs = 0, {}  # refs: what those before leave of a shared last page's references
+        for s in seqs:
+            pages, have = self._pages[s], self._len[s]
+            want += -(-(have + n) // self.page_len) - len(pages)
+            if n and have % self.page_len:
+                last = pages[-1]
+                left = refs.get(last, self._refs[last])
+                if left > 1:
+                    want += 1
+                    refs[last] = left - 1
+        if want > len(self._free):
+            raise MemoryError(f"{want} pages wanted, {len(self._free)} free")
+        src, dst = [], []
+        for s in seqs:
+            a, b = self.grow(s, n)
+            src += a
+            dst += b
+        return src, dst
+
     def fork(self, seq: int) -> int:
         """A new sequence with the same contents, sharing every page."""
         new = self.new()

@@ -123,3 +123,41 @@ def test_copy_pages_takes_ids_of_any_whole_type():
     for ids in ([5], (5,), np.array([5]), np.array([5], np.uint8), np.array([5], np.uint64), np.array([0, 5, 0, 6])[1::2]):
         _refused(-3, kv, ids, ids)
     pkg().copy_pages_device(kv, [], [])
+
+
+def test_sequences_grow_together_or_not_at_all():
+    P = pkg()
+    t = P.PageTable(8, 4)
+    a = t.new()
+    t.grow(a, 6)  # two pages, the second half full
+    b, c = t.fork(a), t.fork(a)
+    assert t.grow_all([a, b, c], 0) == ([], []) and t.free_pages == 6
+    last = t.pages(a)[-1]
+    src, dst = t.grow_all([a, b, c])  # two copies: the third may write the shared page itself
+    assert src == [last, last] and t.pages(c)[-1] == last and [t.pages(s)[-1] for s in (a, b)] == dst and t.free_pages == 4
+    assert [t.length(s) for s in (a, b, c)] == [7, 7, 7]
+    assert t.grow_all([a, b, c]) == ([], [])  # eight positions in two pages each
+    d = t.new()
+    t.grow(d, 7)  # two of the four left
+    before = [(t.length(s), t.pages(s)) for s in (a, b, c, d)]
+    with pytest.raises(MemoryError):
+        t.grow_all([d, a, b, c])  # one position is there in d's page, three pages are wanted, two are free
+    with pytest.raises(ValueError):
+        t.grow_all([d, d])
+    with pytest.raises(ValueError):
+        t.grow_all([d], -1)
+    with pytest.raises(KeyError):
+        t.grow_all([d, 99])
+    assert [(t.length(s), t.pages(s)) for s in (a, b, c, d)] == before and t.free_pages == 2
+    assert t.grow_all([d, a, b]) == ([], []) and t.free_pages == 0
+    assert t.grow_all([]) == ([], [])
+
+
+def test_sequences_that_share_a_page_outside_the_list_copy_it():
+    P = pkg()
+    t = P.PageTable(5, 4)
+    a = t.new()
+    t.grow(a, 2)
+    b, c = t.fork(a), t.fork(a)
+    src, dst = t.grow_all([b, c])  # a keeps the page
+    assert src == [t.pages(a)[0]] * 2 and dst == [t.pages(b)[0], t.pages(c)[0]] and len({*dst, src[0]}) == 3
