@@ -70,6 +70,8 @@ class PagedDecoder:
         n = len(seqs)
         if n > self.max_seqs:
             raise ValueError(f"{n} sequences in a decoder made for {self.max_seqs}")
+        if any(self.pages.length(s) >= self.cos.shape[0] for s in seqs):
+            raise ValueError(f"a sequence holds its {self.cos.shape[0]} positions")
         pos = torch.tensor([self.pages.length(s) for s in seqs], dtype=torch.int32, device="cuda")
         self.copy(self.pages.grow_all(seqs))
         table = torch.from_numpy(self.pages.table(seqs)).cuda()
@@ -93,9 +95,14 @@ class PagedDecoder:
 
     def read(self, prompt) -> tuple[int, torch.Tensor]:
         """A new sequence that holds the prompt, and the logits after it."""
+        prompt = [int(t) for t in prompt]
+        if not 0 < len(prompt) <= self.cos.shape[0]:
+            raise ValueError(f"a prompt of {len(prompt)} ids, not 1 to {self.cos.shape[0]}")
+        if not all(0 <= t < self.embed.shape[0] for t in prompt):
+            raise ValueError("a prompt id outside the vocabulary")
         s = self.pages.new()
         for t in prompt:
-            logits = self.step([s], torch.tensor([int(t)], device="cuda"))
+            logits = self.step([s], torch.tensor([t], device="cuda"))
         return s, logits
 
 

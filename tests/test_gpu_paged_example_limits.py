@@ -28,3 +28,26 @@ def test_a_step_without_enough_pages_changes_nothing(cuda_ok):
             model.pages.free(taken)
         logits.append(model.step(seqs, ids))
     assert torch.equal(*logits)
+
+
+def test_a_step_past_the_last_position_is_refused(cuda_ok):
+    import torch
+    P, E = pkg(), _example()
+    model = E.PagedDecoder(P.synthetic_pgw("tiny-llama", 6), 60, 16, "f32", 2)
+    most = model.cfg["maxSeqLen"]
+    a, b = model.pages.new(), model.pages.new()
+    model.pages.grow(a, most)
+    model.pages.grow(b, 1)
+    with pytest.raises(ValueError):
+        model.step([b, a], torch.tensor([1, 2], device="cuda"))
+    assert [model.pages.length(s) for s in (a, b)] == [most, 1]
+    assert torch.isfinite(model.step([b], torch.tensor([1], device="cuda"))).all()
+
+
+def test_a_prompt_is_checked_before_it_is_read(cuda_ok):
+    P, E = pkg(), _example()
+    model = E.PagedDecoder(P.synthetic_pgw("tiny-llama", 6), 60, 16, "f32", 2)
+    for prompt in ([], [1, 2, -1], [1] * (model.cfg["maxSeqLen"] + 1)):
+        with pytest.raises(ValueError):
+            model.read(prompt)
+    assert model.pages.free_pages == 60
