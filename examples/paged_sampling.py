@@ -76,7 +76,8 @@ class PagedDecoder:
         self.copy(self.pages.grow_all(seqs))
         table = torch.from_numpy(self.pages.table(seqs)).cuda()
         length = pos + 1
-        x = self.embed[ids.long()]
+        known = (ids >= 0) & (ids < self.embed.shape[0])  # an id that is none makes its own sequence NaN
+        x = self.embed[ids.long().where(known, 0)].where(known[:, None], float("nan"))
         q = torch.empty(n, self.d, device="cuda")
         att = torch.empty(n, self.d, device="cuda")
         for i, kv in enumerate(self.kv):

@@ -51,3 +51,21 @@ def test_a_prompt_is_checked_before_it_is_read(cuda_ok):
         with pytest.raises(ValueError):
             model.read(prompt)
     assert model.pages.free_pages == 60
+
+
+@pytest.mark.parametrize("bad", [-1, 512, 2**31 - 1, -600])
+def test_an_id_that_is_none_shows_in_its_own_sequence(bad, cuda_ok):
+    """What a row with no token to draw gives (-1), or an id past the vocabulary: NaN for that sequence alone."""
+    import torch
+    P, E = pkg(), _example()
+    model = E.PagedDecoder(P.synthetic_pgw("tiny-llama", 6), 60, 4, "f32", 3)
+    first, _ = model.read(P.seeded_prompt(6, 512, 4))
+    seqs = [first] + [model.pages.fork(first) for _ in range(2)]
+    twins = [model.pages.fork(first) for _ in range(3)]
+    logits = model.step(seqs, torch.tensor([7, bad, 9], device="cuda"))
+    want = model.step(twins, torch.tensor([7, 8, 9], device="cuda"))
+    assert torch.isnan(logits[1]).all() and torch.equal(logits[[0, 2]], want[[0, 2]])
+    ids, lp = E.sample(logits, torch.full((3,), 0.5, device="cuda"), temperature=0.0)
+    assert ids[1] == -1 and (ids[[0, 2]] >= 0).all()
+    logits, want = model.step(seqs, ids), model.step(twins, torch.stack([ids[0], ids[0], ids[2]]))
+    assert torch.isnan(logits[1]).all() and torch.equal(logits[[0, 2]], want[[0, 2]])
