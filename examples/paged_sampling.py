@@ -102,8 +102,12 @@ class PagedDecoder:
         if not all(0 <= t < self.embed.shape[0] for t in prompt):
             raise ValueError("a prompt id outside the vocabulary")
         s = self.pages.new()
-        for t in prompt:
-            logits = self.step([s], torch.tensor([t], device="cuda"))
+        try:
+            for t in prompt:
+                logits = self.step([s], torch.tensor([t], device="cuda"))
+        except Exception:
+            self.pages.free(s)
+            raise
         return s, logits
 
 
@@ -129,14 +133,16 @@ def continuations(model: PagedDecoder, prompt, forks: int, new: int, seed: int =
     seqs = [first] + [model.pages.fork(first) for _ in range(forks - 1)]
     logits = logits.expand(forks, -1).contiguous()
     ids, logprobs = [], []
-    for i in range(new):
-        t, lp = sample(logits, torch.rand(forks, generator=gen, device="cuda"), **settings)
-        ids.append(t)
-        logprobs.append(lp)
-        if i + 1 < new:
-            logits = model.step(seqs, t)
-    for s in seqs:
-        model.pages.free(s)
+    try:
+        for i in range(new):
+            t, lp = sample(logits, torch.rand(forks, generator=gen, device="cuda"), **settings)
+            ids.append(t)
+            logprobs.append(lp)
+            if i + 1 < new:
+                logits = model.step(seqs, t)
+    finally:
+        for s in seqs:
+            model.pages.free(s)
     return torch.stack(ids, 1), torch.stack(logprobs, 1)
 
 

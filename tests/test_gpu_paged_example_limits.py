@@ -69,3 +69,16 @@ def test_an_id_that_is_none_shows_in_its_own_sequence(bad, cuda_ok):
     assert ids[1] == -1 and (ids[[0, 2]] >= 0).all()
     logits, want = model.step(seqs, ids), model.step(twins, torch.stack([ids[0], ids[0], ids[2]]))
     assert torch.isnan(logits[1]).all() and torch.equal(logits[[0, 2]], want[[0, 2]])
+
+
+def test_pages_are_given_back_where_they_run_out(cuda_ok):
+    P, E = pkg(), _example()
+    model = E.PagedDecoder(P.synthetic_pgw("tiny-llama", 6), 6, 4, "f32", 3)
+    with pytest.raises(MemoryError):
+        model.read(P.seeded_prompt(25, 512, 1))
+    assert model.pages.free_pages == 6
+    with pytest.raises(MemoryError):
+        E.continuations(model, P.seeded_prompt(8, 512, 1), 3, 12, temperature=0.5)
+    assert model.pages.free_pages == 6
+    ids, _ = E.continuations(model, P.seeded_prompt(8, 512, 1), 3, 4, temperature=0.5)
+    assert ids.shape == (3, 4) and model.pages.free_pages == 6
