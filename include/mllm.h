@@ -255,7 +255,8 @@ typedef struct {
  * table_stride; NULL: row t belongs to sequence t.  A row with a negative sequence is padding: nothing
  * of it is read or written.  A row whose sequence, position or page id is out of range writes no cache
  * row, and its q is NaN.  No two rows may have the same sequence and position.  `dtype` is f32 or the
- * cache's type.  d_q may be the q part of d_qkv itself.  Sums and rotations are f32.
+ * cache's type.  d_q may be the q part of d_qkv itself.  A row has at most 2^30 heads, a call 2^31.  Sums and
+ * rotations are f32.
  */
 int mllm_rope_append(const mllm_paged_kv* kv, int dtype, const void* d_qkv, int64_t row_stride, int n_tok, int n_heads,
                      const int32_t* d_seq, const int32_t* d_pos, const int32_t* d_table, int n_seq, int table_stride,
@@ -272,7 +273,9 @@ int mllm_rope_append(const mllm_paged_kv* kv, int dtype, const void* d_qkv, int6
  * page, are never read.  A sequence whose length exceeds table_stride pages, or with a page id outside
  * the pool, gives NaN.  A key whose score is -inf is left out; an infinite value gives infinity or NaN.
  * n_seq <= 65,535; n_heads / n_kv_heads <= 64; the table may hold up to about 2^31
- * blocks of 32 positions over all sequences and kv heads.  Scores, sums and the joins are f32.
+ * blocks of 32 positions over all sequences, kv heads and groups of query heads; a row of queries has at most
+ * 2^30 elements.  A kv head's query heads go in groups of up to 16 (f32 caches and head_dim above 128: 8), each of
+ * which reads the cached rows.  Scores, sums and the joins are f32.
  * d_ws: mllm_paged_attn_workspace bytes, 16-byte aligned, zeroed once before its first use (each call
  * leaves its counters at zero again); one workspace serves one call at a time, and calls of any numbers of
  * sequences, heads and head_dim one after another, as long as it has room for the largest.  The result does
@@ -309,7 +312,8 @@ int mllm_copy_pages(const mllm_paged_kv* kv, int n_layers, int64_t layer_stride,
  * T <= 0 (or NaN) takes the top token, lowest index on ties, as engine/infer.js:240-250; top_k <= 0 or
  * >= vocab, top_p >= 1 and min_p <= 0 are off.  d_u [rows]: in [0, 1).
  * Out: d_id [rows]; nullable d_logprob [rows] (of the drawn id in the kept distribution), d_kept [rows]
- * (tokens kept), d_probs [rows][vocab] f32 (the kept distribution).  A row that keeps no token (every
+ * (kept tokens that weigh something: one with w_i = 0 has no share and is not counted), d_probs
+ * [rows][vocab] f32 (the kept distribution).  A row that keeps no token (every
  * logit -inf or NaN, or min_p above 1) gives id -1, logprob -inf, kept 0 and probs 0.  vocab <= 524,288.
  */
 int mllm_sample(int dtype, const void* d_logits, int64_t row_stride, int rows, int vocab, const float* d_temperature,

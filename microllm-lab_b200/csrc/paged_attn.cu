@@ -16,8 +16,8 @@
 // another.  Where every segment is short and can have a CTA of its own, it gets one, which saves the
 // second join.
 //
-// B200: 3 sequences to 100,003 positions, 32 heads over 8 of 128, f16: 151 us (5.9 TB/s, 90 % of the measured
-// copy); 256 sequences of 0 to 384, 9 heads over 3 of 64, bf16: 22.2 us, of which the copies need 7.2 (the rest
+// B200: 3 sequences to 100,003 positions, 32 heads over 8 of 128, f16: 155 us (5.7 TB/s, 87 % of the measured
+// copy); 256 sequences of 0 to 384, 9 heads over 3 of 64, bf16: 22.1 us, of which the copies need 7.2 (the rest
 // is the latency of finding the runs, the first rows and the joins); 1 of 191, f32: 12.3 us.
 #include <algorithm>
 #include <atomic>
@@ -37,7 +37,10 @@ constexpr int kMinBlocks = 4;    // a CTA's run is at least one block per warp
 constexpr int kWholeBlocks = 16; // segments up to this long get a CTA of their own where there are enough CTAs
 constexpr int kFan = 16;         // a segment in more than twice as many parts is joined by so many of them first
 constexpr int kMaxCtas = 1024;   // partial slots in the workspace
-constexpr int kMaxGroup = 16;    // query heads of a group
+// Query heads of a group, at most (8 for f32 caches and for head_dim above 128, by registers).  Each group of a kv head
+// walks the segment on its own, so that more heads than that read the cache several times (16 sequences to 32,768,
+// 2 kv heads of 128, f32: 170 us for 8 heads each, 304 for 16; bf16: 91 us for 16, 146 for 32).
+constexpr int kMaxGroup = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnArgs {

@@ -6,8 +6,8 @@
 // which few enough tokens (top-k) or little enough weight (top-p) lies.  The id is found in index order, at
 // the place where the running kept weight passes floor(u Z).  Weights are integers of at most 2^40 (a sum
 // of 2^19 of them fits 64 bits), so every sum is exact and no result depends on the order in which threads
-// add.  The 2^-40 that a weight loses is 2^-40 of the top token's: over 2^18 tokens at most 2^-22 of the
-// row, the size of an f32 rounding.
+// add.  What the whole part cuts off a weight is below 2^-40 of the top token's: over the 2^19 tokens that a row may
+// have less than 2^-21 of its weight, a few f32 roundings.
 //
 // A row is read once, into the shared memory of one CTA, or of a cluster's CTAs, each of which has a
 // contiguous part, where rows are fewer than SMs or do not fit.  The edge is found without sorting the row:
@@ -18,8 +18,8 @@
 //     or of a 512th of it where they are too many for a list;
 //   - and by halving, one pass per bit, where those are too many as well (thousands of tokens of one value).
 // A short list is not sorted either: several threads per token count, and weigh, what precedes it.  One of up to
-// 512 tokens is sorted in registers, for the id a second time by index (33 rows with top_p: 35.9 us, by steps 38.9;
-// lists of up to 1,024 sorted as well cost 256 rows 62.7 us instead of 59.8).  A longer one goes through the same
+// 512 tokens is sorted in registers, for the id a second time by index (33 rows with top_p, medians of five: 37.2 us,
+// by steps 38.9, with runs of either up to 2.4 apart; 256 rows 58.7 and 58.6).  A longer one goes through the same
 // two levels of steps until few enough are left, for the id by steps of the index; it is sorted where one step
 // holds too many.
 // The CTAs of a cluster meet at a barrier only to exchange a maximum, a histogram, a list (the first one's) or
@@ -29,8 +29,8 @@
 // once is called, not inlined, and the passes over the row either test 16 bytes at a time and do the rest
 // for the few that pass, or take a token at a time.
 //
-// B200: 256 rows of 49,152 f32 with mixed settings 60 us, one row 14 us, 33 rows of 50,257 bf16 with top_p and
-// probabilities 36 us.  Bound by latency where rows are few (a chain of some 20 barriers), by instruction
+// B200: 256 rows of 49,152 f32 with mixed settings 59 us, one row 14 us, 33 rows of 50,257 bf16 with top_p and
+// probabilities 37 us (36 to 39).  Bound by latency where rows are few (a chain of some 20 barriers), by instruction
 // issue and colliding shared-memory atomics where every token's weight goes into a histogram (about 24,000
 // cycles of one SM for 49,152 tokens).
 #include <cooperative_groups.h>

@@ -51,7 +51,8 @@ def rope_append_device(kv: PagedKV, dtype: str, qkv_ptr: int, row_stride: int, n
 
 
 def paged_attn_workspace(n_seq: int, n_heads: int, head_dim: int) -> int:
-    """Bytes of the zeroed workspace ``paged_attn_device`` needs (mllm_paged_attn_workspace)."""
+    """Bytes of the workspace, zeroed once, that ``paged_attn_device`` needs (mllm_paged_attn_workspace).  One of
+    the largest ``n_heads`` and ``head_dim`` serves calls of any shape, one after another."""
     return int(load_library().mllm_paged_attn_workspace(n_seq, n_heads, head_dim))
 
 
