@@ -449,6 +449,15 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&w)[TERMS]) {
     }
   }
 }
+// An element too small for f16 keeps its sign in the first term, as the smallest number there is, and the second
+// takes that off again: with an infinite key the first term alone decides (below).
+template <int TERMS>
+__device__ __forceinline__ void signed_zero(uint32_t (&w)[TERMS], float v, int at) {
+  if (v == 0.f || (w[0] >> at & 0x7FFFu)) return;
+  const uint32_t sign = v < 0.f ? 0x8000u : 0u;
+  w[0] = (w[0] & ~(0xFFFFu << at)) | (sign | 1u) << at;
+  w[1] = (w[1] & ~(0xFFFFu << at)) | ((sign ^ 0x8000u) | 1u) << at;
+}
 template <class T>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (sizeof(T) == 2 && __is_same(T, __half))
@@ -592,7 +601,7 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
             }
             sc[nt][0] = sc[nt][1] = a.scale * kLog2e;
           } else {
-            float f[C][8], top = 0.f;
+            float f[C][8], top = 0.f, low = INFINITY;
 #pragma unroll
             for (int x = 0; x < C; ++x) {
               const int d = x * 32 + quad * 8;
@@ -604,7 +613,10 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
               f[x][0] = u.x, f[x][1] = u.y, f[x][2] = u.z, f[x][3] = u.w;
               f[x][4] = v.x, f[x][5] = v.y, f[x][6] = v.z, f[x][7] = v.w;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[x][e]));
+              for (int e = 0; e < 8; ++e) {
+                top = fmaxf(top, fabsf(f[x][e]));
+                if constexpr (TERMS == 2) low = fminf(low, fabsf(f[x][e]));
+              }
             }
             float up = 1.f, down = 1.f;
             if constexpr (TERMS == 2) {  // f16 terms: scaled to below 2^15
@@ -616,13 +628,20 @@ __global__ void __launch_bounds__(kAttnThreads, mma_ctas<DP, NT>()) attn_mma_ker
               up = ldexpf(1.f, e);
               down = ldexpf(1.f, -e);
             }
+            const bool tiny = h < heads && low * down < 0x1p-24f;  // some element is 0 in f16, as few are
             sc[nt][0] = a.scale * __shfl_sync(0xffffffffu, up, quad * 8) * kLog2e;
             sc[nt][1] = a.scale * __shfl_sync(0xffffffffu, up, quad * 8 + 4) * kLog2e;
 #pragma unroll
             for (int x = 0; x < C; ++x) {
               uint32_t w[4][TERMS];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) split2<T, TERMS>(f[x][2 * e] * down, f[x][2 * e + 1] * down, w[e]);
+              for (int e = 0; e < 4; ++e) {
+                split2<T, TERMS>(f[x][2 * e] * down, f[x][2 * e + 1] * down, w[e]);
+                if (TERMS == 2 && tiny) {
+                  signed_zero(w[e], f[x][2 * e], 0);
+                  signed_zero(w[e], f[x][2 * e + 1], 16);
+                }
+              }
 #pragma unroll
               for (int t = 0; t < TERMS; ++t) {
                 const uint4 v = make_uint4(w[0][t], w[1][t], w[2][t], w[3][t]);
